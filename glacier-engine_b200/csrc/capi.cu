@@ -5,7 +5,7 @@
 #include <mutex>
 #include <vector>
 
-#include "common.cuh"
+#include "kv_q4.cuh"
 
 namespace glacier {
 
@@ -148,6 +148,23 @@ size_t argmax_workspace_bytes(size_t batch, size_t n);
 int argmax_rows(const float* logits, size_t ld, size_t batch, size_t n, const uint64_t* words, size_t word_count,
                 glacier_argmax_result* out, int32_t* tokens, int32_t* status, void* workspace, size_t ws_bytes,
                 cudaStream_t stream);
+
+int qkv_rope_append_q4(const float* qkv, size_t ld, size_t split_stride, int nsplit, const float* bias,
+                       const float* cos_t, const float* sin_t, size_t positions, const int32_t* pos,
+                       const int64_t* slots, size_t batch, size_t num_heads, size_t num_kv_heads, size_t head_dim,
+                       float* q_out, size_t ldq, void* pool, size_t num_pages, size_t num_layers, size_t layer,
+                       cudaStream_t stream);
+int kv_q4_read(const void* pool, size_t num_pages, size_t num_layers, size_t layer, size_t num_kv_heads,
+               size_t head_dim, const int64_t* slots, size_t rows, float* k_out, float* v_out, cudaStream_t stream);
+size_t attention_q4_workspace_floats(size_t num_heads, size_t num_kv_heads, size_t head_dim);
+int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_pages, size_t num_layers,
+                       const int32_t* block_tables, size_t max_pages, const int32_t* ctx_lens, size_t lanes,
+                       size_t layer, size_t num_heads, size_t num_kv_heads, size_t head_dim, float* out, size_t ldo,
+                       float* workspace, size_t workspace_floats, cudaStream_t stream);
+int kv_resize(int32_t* lens, const int32_t* targets, size_t lanes, int32_t* block_tables, size_t max_pages,
+              int32_t* free_pages, size_t capacity, int32_t* free_count, int32_t* status, size_t row_stride,
+              size_t rows, int32_t* positions, int32_t* row_lanes, int64_t* slots, int32_t* row_offsets,
+              cudaStream_t stream);
 
 size_t gemm_split_bytes(size_t np, size_t K);
 bool gemm_tc_supported(const Int4Weight& w);
@@ -343,6 +360,49 @@ int glacier_cuda_argmax_eligible_f32(const float* logits, size_t batch, size_t n
                                      void* stream) {
   return argmax_rows(logits, n, batch, n, words, word_count, results, tokens, status, workspace, workspace_bytes,
                      (cudaStream_t)stream);
+}
+
+size_t glacier_cuda_kv_q4_page_bytes(size_t num_layers, size_t num_kv_heads, size_t head_dim) {
+  return num_layers * num_kv_heads * q4_block_bytes(head_dim);
+}
+
+int glacier_cuda_qkv_rope_append_q4(const float* qkv, size_t ld, const float* bias, const float* cos_table,
+                                    const float* sin_table, size_t positions, const int32_t* pos,
+                                    const int64_t* slots, size_t batch, size_t num_heads, size_t num_kv_heads,
+                                    size_t head_dim, float* q_out, size_t ldq, void* pool, size_t num_pages,
+                                    size_t num_layers, size_t layer, void* stream) {
+  return qkv_rope_append_q4(qkv, ld, 0, 1, bias, cos_table, sin_table, positions, pos, slots, batch, num_heads,
+                            num_kv_heads, head_dim, q_out, ldq, pool, num_pages, num_layers, layer,
+                            (cudaStream_t)stream);
+}
+
+int glacier_cuda_kv_q4_read_f32(const void* pool, size_t num_pages, size_t num_layers, size_t layer,
+                                size_t num_kv_heads, size_t head_dim, const int64_t* slots, size_t rows,
+                                float* k_out, float* v_out, void* stream) {
+  return kv_q4_read(pool, num_pages, num_layers, layer, num_kv_heads, head_dim, slots, rows, k_out, v_out,
+                    (cudaStream_t)stream);
+}
+
+size_t glacier_cuda_paged_attention_q4_workspace(size_t num_heads, size_t num_kv_heads, size_t head_dim) {
+  return attention_q4_workspace_floats(num_heads, num_kv_heads, head_dim);
+}
+
+int glacier_cuda_paged_attention_q4(const float* q, const void* pool, size_t num_pages, size_t num_layers,
+                                    const int32_t* block_tables, size_t max_pages, const int32_t* ctx_lens,
+                                    size_t lanes, size_t layer, size_t num_heads, size_t num_kv_heads,
+                                    size_t head_dim, float* out, float* workspace, size_t workspace_floats,
+                                    void* stream) {
+  return paged_attention_q4(q, num_heads * head_dim, pool, num_pages, num_layers, block_tables, max_pages, ctx_lens,
+                            lanes, layer, num_heads, num_kv_heads, head_dim, out, num_heads * head_dim, workspace,
+                            workspace_floats, (cudaStream_t)stream);
+}
+
+int glacier_cuda_kv_resize(int32_t* lens, const int32_t* targets, size_t lanes, int32_t* block_tables,
+                           size_t max_pages, int32_t* free_pages, size_t capacity, int32_t* free_count,
+                           int32_t* status, size_t row_stride, size_t rows, int32_t* positions, int32_t* row_lanes,
+                           int64_t* slots, int32_t* row_offsets, void* stream) {
+  return kv_resize(lens, targets, lanes, block_tables, max_pages, free_pages, capacity, free_count, status,
+                   row_stride, rows, positions, row_lanes, slots, row_offsets, (cudaStream_t)stream);
 }
 
 }  // extern "C"

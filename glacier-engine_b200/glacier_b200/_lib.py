@@ -52,6 +52,13 @@ SIGNATURES = {
                                           sz, vp], i32),
     "glacier_cuda_paged_attention_workspace": ([sz, sz, sz, sz, sz], sz),
     "glacier_cuda_paged_attention_f32": ([vp, vp, sz, vp, sz, vp, sz, sz, sz, sz, sz, sz, vp, vp, sz, vp], i32),
+    "glacier_cuda_kv_q4_page_bytes": ([sz, sz, sz], sz),
+    "glacier_cuda_qkv_rope_append_q4": ([vp, sz, vp, vp, vp, sz, vp, vp, sz, sz, sz, sz, vp, sz, vp, sz, sz, sz, vp],
+                                        i32),
+    "glacier_cuda_kv_q4_read_f32": ([vp, sz, sz, sz, sz, sz, vp, sz, vp, vp, vp], i32),
+    "glacier_cuda_paged_attention_q4_workspace": ([sz, sz, sz], sz),
+    "glacier_cuda_paged_attention_q4": ([vp, vp, sz, sz, vp, sz, vp, sz, sz, sz, sz, sz, vp, vp, sz, vp], i32),
+    "glacier_cuda_kv_resize": ([vp, vp, sz, vp, sz, vp, sz, vp, vp, sz, sz, vp, vp, vp, vp, vp], i32),
     "glacier_cuda_argmax_workspace": ([sz, sz], sz),
     "glacier_cuda_argmax_eligible_f32": ([vp, sz, sz, vp, sz, vp, vp, vp, vp, sz, vp], i32),
     "glacier_cuda_argmax_eligible_f32_noalloc": ([vp, sz, sz, vp, sz, vp, vp, vp, vp], i32),

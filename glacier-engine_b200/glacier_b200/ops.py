@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import call
+from ._lib import EINVAL, GlacierCudaError, call, lib
 
 
 def _ptr(t):
@@ -41,7 +41,6 @@ def linear_int4_on_the_fly(x: torch.Tensor, packed: torch.Tensor, scales: torch.
 def linear_int4_tensor_core(x: torch.Tensor, packed: torch.Tensor, scales_f16: torch.Tensor, out_f: int,
                             in_f: int, group: int, bias: torch.Tensor | None = None, out=None, stream=None):
     """Batched linearInt4OnTheFly on the tcgen05 dequant GEMM (int4_neon.c:1439 M4 GEMM role)."""
-    from ._lib import lib
     x = x.reshape(-1, in_f)
     b = x.shape[0]
     out = torch.empty((b, out_f), dtype=torch.float32, device=x.device) if out is None else out
@@ -102,7 +101,6 @@ def qkv_rope_append(qkv, bias, cos, sin, pos, num_heads, num_kv_heads, head_dim,
 def paged_attention_f32(q, kv_pages, page_floats, block_tables, ctx_lens, max_ctx, layer, num_heads, num_kv_heads,
                         head_dim, stream=None):
     """paged_attention.zig:108 attentionMultiHead, one query row per lane."""
-    from ._lib import lib
     lanes = q.shape[0]
     ws_n = lib().glacier_cuda_paged_attention_workspace(lanes, num_heads, num_kv_heads, head_dim, max_ctx)
     ws = torch.empty(ws_n, dtype=torch.float32, device=q.device)
@@ -115,7 +113,6 @@ def paged_attention_f32(q, kv_pages, page_floats, block_tables, ctx_lens, max_ct
 
 def argmax_eligible(logits, words=None, stream=None):
     """sampling.zig:55 argmaxEligible per row -> (tokens int32, status int32)."""
-    from ._lib import lib
     b, n = logits.shape
     ws_n = lib().glacier_cuda_argmax_workspace(b, n)
     ws = torch.empty(ws_n, dtype=torch.uint8, device=logits.device)
@@ -125,3 +122,138 @@ def argmax_eligible(logits, words=None, stream=None):
     call("glacier_cuda_argmax_eligible_f32", logits.data_ptr(), b, n, _ptr(words), wc, tokens.data_ptr(),
          status.data_ptr(), None, ws.data_ptr(), ws_n, _stream(stream))
     return tokens, status
+
+
+# ---- the KV cache held in 4 bits ----
+# These run on the device their tensors are on, whichever is current; what they allocate belongs
+# to the stream they run on.  Tensors of another type, shape, layout or device are refused.
+
+def _check(dev, **tensors):
+    """Raises unless every (tensor, dtype, shape) is contiguous on `dev` with that type and shape
+    (None: any extent)."""
+    for name, (t, dtype, shape) in tensors.items():
+        if (t.dtype is not dtype or t.device != dev or not t.is_contiguous() or t.dim() != len(shape)
+                or any(w is not None and w != n for n, w in zip(t.shape, shape))):
+            raise GlacierCudaError(EINVAL, f"{name}: {str(t.dtype)[6:]} {tuple(t.shape)} on {t.device}, expected a "
+                                           f"contiguous {str(dtype)[6:]} {tuple(shape)} on {dev}")
+
+
+class _on:
+    """The device of `dev` and `stream` (None: that device's current one) made current."""
+
+    def __init__(self, dev, stream):
+        if dev.type != "cuda":
+            raise GlacierCudaError(EINVAL, f"tensors on {dev}: the 4-bit cache is on a GPU")
+        if stream is not None and stream.device != dev:
+            raise GlacierCudaError(EINVAL, f"a stream of {stream.device} for tensors on {dev}")
+        if stream is None and dev.index != torch.cuda.current_device():
+            stream = torch.cuda.current_stream(dev)
+        self.ctx = None if stream is None else torch.cuda.stream(stream)
+        self.stream = stream
+
+    def __enter__(self):
+        if self.ctx is None:
+            return torch.cuda.current_stream().cuda_stream
+        self.ctx.__enter__()
+        return self.stream.cuda_stream
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def kv_q4_page_bytes(num_layers: int, num_kv_heads: int, head_dim: int) -> int:
+    """Bytes of one 16-position page of a 4-bit pool (all layers)."""
+    return lib().glacier_cuda_kv_q4_page_bytes(num_layers, num_kv_heads, head_dim)
+
+
+def qkv_rope_append_q4(qkv, bias, cos, sin, pos, slots, num_heads, num_kv_heads, head_dim, pages, num_layers, layer,
+                       q_out=None, stream=None):
+    """qkv_rope_append into a 4-bit pool: ``pages`` uint8 [num_pages, kv_q4_page_bytes], row b's K and V
+    quantised into position ``slots[b]`` (int64: page * 16 + row; -1: a padding row).  Returns the rotated q
+    [batch, num_heads * head_dim].  ``qkv`` may be a view with a row stride."""
+    dev, b, qd = qkv.device, qkv.shape[0], num_heads * head_dim
+    width, half = qd + 2 * num_kv_heads * head_dim, head_dim // 2
+    if qkv.dtype is not torch.float32 or qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
+        raise GlacierCudaError(EINVAL, f"qkv: {qkv.dtype} {tuple(qkv.shape)}, expected float32 rows of {width}")
+    _check(dev, cos=(cos, torch.float32, (None, half)), sin=(sin, torch.float32, (cos.shape[0], half)),
+           pos=(pos, torch.int32, (b,)), slots=(slots, torch.int64, (b,)),
+           pages=(pages, torch.uint8, (None, kv_q4_page_bytes(num_layers, num_kv_heads, head_dim))))
+    if bias is not None:
+        _check(dev, bias=(bias, torch.float32, (width,)))
+    with _on(dev, stream) as s:
+        if q_out is None:
+            q_out = torch.empty((b, qd), dtype=torch.float32, device=dev)
+        else:
+            _check(dev, q_out=(q_out, torch.float32, (b, qd)))
+        call("glacier_cuda_qkv_rope_append_q4", qkv.data_ptr(), max(qkv.stride(0), width) if b < 2 else qkv.stride(0),
+             _ptr(bias), cos.data_ptr(), sin.data_ptr(), cos.shape[0], pos.data_ptr(), slots.data_ptr(), b, num_heads,
+             num_kv_heads, head_dim, q_out.data_ptr(), qd, pages.data_ptr(), pages.shape[0], num_layers, layer, s)
+    return q_out
+
+
+def kv_q4_read(pages, slots, num_layers, layer, num_kv_heads, head_dim, stream=None):
+    """The K and V values held at ``slots``: two float32 [rows, num_kv_heads * head_dim] (zeros for slot -1)."""
+    dev, rows = pages.device, slots.numel()
+    _check(dev, slots=(slots, torch.int64, (rows,)),
+           pages=(pages, torch.uint8, (None, kv_q4_page_bytes(num_layers, num_kv_heads, head_dim))))
+    with _on(dev, stream) as s:
+        k = torch.empty((rows, num_kv_heads * head_dim), dtype=torch.float32, device=dev)
+        v = torch.empty_like(k)
+        call("glacier_cuda_kv_q4_read_f32", pages.data_ptr(), pages.shape[0], num_layers, layer, num_kv_heads,
+             head_dim, slots.data_ptr(), rows, k.data_ptr(), v.data_ptr(), s)
+    return k, v
+
+
+def paged_attention_q4_workspace(num_heads, num_kv_heads, head_dim, device=None):
+    """Workspace of paged_attention_q4, for calls that do not run at the same time."""
+    n = lib().glacier_cuda_paged_attention_q4_workspace(num_heads, num_kv_heads, head_dim)
+    return torch.empty(n, dtype=torch.float32, device="cuda" if device is None else device)
+
+
+def paged_attention_q4(q, pages, block_tables, ctx_lens, num_layers, layer, num_heads, num_kv_heads, head_dim,
+                       out=None, workspace=None, stream=None):
+    """paged_attention_f32 over a 4-bit pool, one query row per lane."""
+    dev, lanes, qd = q.device, q.shape[0], num_heads * head_dim
+    _check(dev, q=(q, torch.float32, (lanes, qd)), block_tables=(block_tables, torch.int32, (lanes, None)),
+           ctx_lens=(ctx_lens, torch.int32, (lanes,)),
+           pages=(pages, torch.uint8, (None, kv_q4_page_bytes(num_layers, num_kv_heads, head_dim))))
+    with _on(dev, stream) as s:
+        if workspace is None:
+            workspace = paged_attention_q4_workspace(num_heads, num_kv_heads, head_dim, dev)
+        else:
+            _check(dev, workspace=(workspace, torch.float32, (None,)))
+        if out is None:
+            out = torch.empty((lanes, qd), dtype=torch.float32, device=dev)
+        else:
+            _check(dev, out=(out, torch.float32, (lanes, qd)))
+        call("glacier_cuda_paged_attention_q4", q.data_ptr(), pages.data_ptr(), pages.shape[0], num_layers,
+             block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), lanes, layer, num_heads,
+             num_kv_heads, head_dim, out.data_ptr(), workspace.data_ptr(), workspace.numel(), s)
+    return out
+
+
+def kv_resize(lens, targets, block_tables, free_pages, free_count, status, positions=None, row_lanes=None, slots=None,
+              row_offsets=None, row_stride=0, stream=None):
+    """Brings every lane from ``lens`` to ``targets`` positions in place: pages move between the
+    ``block_tables`` and the ``free_pages`` stack of ``free_count`` entries, and the new positions are written
+    as rows (positions, row_lanes int32, slots int64; packed, or row_stride rows per lane).  All int32 but slots;
+    see glacier_cuda_kv_resize for the order in which lanes are served and the statuses."""
+    dev, lanes = lens.device, lens.shape[0]
+    i32 = torch.int32
+    _check(dev, lens=(lens, i32, (lanes,)), targets=(targets, i32, (lanes,)),
+           block_tables=(block_tables, i32, (lanes, None)), free_pages=(free_pages, i32, (None,)),
+           free_count=(free_count, i32, (1,)), status=(status, i32, (lanes,)))
+    rows = 0
+    if slots is not None and positions is not None and row_lanes is not None:
+        rows = slots.numel()
+        _check(dev, slots=(slots, torch.int64, (rows,)), positions=(positions, i32, (rows,)),
+               row_lanes=(row_lanes, i32, (rows,)))
+    elif not (slots is positions is row_lanes is None):
+        raise GlacierCudaError(EINVAL, "kv_resize: positions, row_lanes and slots go together")
+    if row_offsets is not None:
+        _check(dev, row_offsets=(row_offsets, i32, (lanes + 1,)))
+    with _on(dev, stream) as s:
+        call("glacier_cuda_kv_resize", lens.data_ptr(), targets.data_ptr(), lanes, block_tables.data_ptr(),
+             block_tables.shape[1], free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
+             status.data_ptr(), row_stride, rows, _ptr(positions), _ptr(row_lanes), _ptr(slots), _ptr(row_offsets), s)

@@ -203,6 +203,77 @@ int glacier_cuda_argmax_eligible_f32_noalloc(const float *logits, size_t batch, 
                                              int32_t *status, glacier_argmax_result *results, void *stream);
 
 /* ------------------------------------------------------------------------
+ * (f) the KV cache held in 4 bits.  No counterpart in the reference, whose pages are FP32; the
+ * numbers are its INT4 ones (two codes per byte, low nibble first, zero point 7, groups of 32
+ * dims with an fp16 scale).
+ *
+ * A pool is num_pages pages of glacier_cuda_kv_q4_page_bytes() bytes, 16-byte aligned; a page
+ * holds 16 positions of every layer, one block of 18 * head_dim bytes per (layer, kv head):
+ *   K codes  [16 positions][4 t][head_dim/32 g] u32, dims 32g+8t..+7
+ *   V codes  [8 position pairs][head_dim/4 w][2 positions] u16, dims 4w..+3
+ *   K scales [8 position pairs][head_dim/32 g][2 positions] fp16, then the V scales
+ * value = scale * (code - 7).  A group's scale is the smallest multiple of 2^-21 of at most 7
+ * significant bits with 7 * scale >= max|x|, at most 7168 (values beyond +-8 * 7168 saturate); its
+ * codes are 7 + x / scale to the nearest integer, ties to even, within [0, 15].  A group that holds a
+ * NaN or an infinity gets a NaN scale: whatever attends it comes out NaN.  Caches written by the
+ * caller keep to that: finite scales, 7 significant bits, at most 7168.
+ * head_dim 64 or 128, at most 8 query heads per kv head; other shapes return GLACIER_CUDA_EINVAL.
+ * ---------------------------------------------------------------------- */
+
+size_t glacier_cuda_kv_q4_page_bytes(size_t num_layers, size_t num_kv_heads, size_t head_dim);
+
+/* glacier_cuda_qkv_rope_append_f32 into a 4-bit pool: bias, rotation (each product and sum rounded
+ * to float32), q to q_out [batch, num_heads * head_dim], k and v quantised into position
+ * slots[b] = physical page * 16 + row of `layer`.  slots[b] == -1 is a padding row: nothing is
+ * cached and its q_out row is zero.  A slot outside the pool or a position outside the RoPE table does
+ * the same and raises the bad-input device status (glacier_cuda_device_status = 2).  The slots of
+ * one call are distinct. */
+int glacier_cuda_qkv_rope_append_q4(const float *qkv, size_t ld, const float *bias, const float *cos_table,
+                                    const float *sin_table, size_t positions, const int32_t *pos,
+                                    const int64_t *slots, size_t batch, size_t num_heads, size_t num_kv_heads,
+                                    size_t head_dim, float *q_out, size_t ldq, void *pool, size_t num_pages,
+                                    size_t num_layers, size_t layer, void *stream);
+
+/* The values held at `slots` as float32: k_out and v_out [rows, num_kv_heads * head_dim], 16-byte
+ * aligned; zeros for slot -1, and zeros with the bad-input status for a slot outside the pool. */
+int glacier_cuda_kv_q4_read_f32(const void *pool, size_t num_pages, size_t num_layers, size_t layer,
+                                size_t num_kv_heads, size_t head_dim, const int64_t *slots, size_t rows,
+                                float *k_out, float *v_out, void *stream);
+
+/* glacier_cuda_paged_attention_f32 over a 4-bit pool, for up to 1024 lanes: lane b attends
+ * positions 0..ctx_lens[b]-1, clamped to the block table; a lane of context 0 gets zeros.  The positions
+ * of a page id outside the pool are left out and raise the bad-input status.  Scores, the softmax
+ * and its sums are float32; held values enter the products exactly.  q, out and workspace are
+ * 16-byte aligned; workspace: glacier_cuda_paged_attention_q4_workspace() floats, any contents,
+ * not shared with a call that may run at the same time. */
+size_t glacier_cuda_paged_attention_q4_workspace(size_t num_heads, size_t num_kv_heads, size_t head_dim);
+int glacier_cuda_paged_attention_q4(const float *q, const void *pool, size_t num_pages, size_t num_layers,
+                                    const int32_t *block_tables, size_t max_pages, const int32_t *ctx_lens,
+                                    size_t lanes, size_t layer, size_t num_heads, size_t num_kv_heads,
+                                    size_t head_dim, float *out, float *workspace, size_t workspace_floats,
+                                    void *stream);
+
+/* Page bookkeeping of a batch on the device (the page tables of src/paged_kv_cache.zig:44-48):
+ * brings every lane from lens[b] to targets[b] positions (16 per page), for up to 1024 lanes.
+ *   lens         [lanes] in and out: positions held; becomes targets[b] for each lane served
+ *   block_tables [lanes, max_pages] in and out: a growing lane's new pages are appended; entries past
+ *                a lane's pages are left as they were
+ *   free_pages   [capacity] stack of free page ids, free_count[0] of them: pages come off the top in lane
+ *                order.  Shrinking lanes give theirs back first, in the order that lets the same growth take
+ *                the same pages again
+ *   status       [lanes]: 0; GLACIER_CUDA_ENOMEM when the free pages (or rows) run out at this lane or
+ *                before it; GLACIER_CUDA_EINVAL for a length outside [0, 16 * max_pages] or growth past
+ *                row_stride.  A lane not served keeps its length, pages and table.
+ * The new positions as rows (all three arrays or none): positions, row_lanes and slots (page * 16 + row)
+ * of `rows` rows, -1 in rows without a position.  row_stride 0 packs the lanes' rows one after another;
+ * row_stride s gives lane b the rows from b * s (rows = lanes * s).  row_offsets [lanes + 1] (may be
+ * NULL): each lane's first row and the end.  lens, targets and the outputs are different arrays. */
+int glacier_cuda_kv_resize(int32_t *lens, const int32_t *targets, size_t lanes, int32_t *block_tables,
+                           size_t max_pages, int32_t *free_pages, size_t capacity, int32_t *free_count,
+                           int32_t *status, size_t row_stride, size_t rows, int32_t *positions,
+                           int32_t *row_lanes, int64_t *slots, int32_t *row_offsets, void *stream);
+
+/* ------------------------------------------------------------------------
  * Persistent model, paged KV pool and the batched decode step.  Replaces the
  * compute of generate.zig forwardLayerCached (:1511-1967) + the decode loop
  * (:5366-5450) + projectLmHead (:3665), and decode_lane4.generate's per-wave

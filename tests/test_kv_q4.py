@@ -1,0 +1,688 @@
+"""The 4-bit paged KV cache (kv_resize, qkv_rope_append_q4, kv_q4_read, paged_attention_q4)
+against plain 64-bit implementations, at the sizes and masks where it can go wrong.
+
+Tolerances.  Codes, scales and the page bookkeeping are exact: no tolerance.  The rotated q is a
+product sum of two float32 roundings each plus the sum's: at most 3 half steps of 2^-24 relative to
+|x0| + |x1|.  An attention output is a weighted mean of held values, which are exact.  A score of
+n products carries at most n + 16 half steps of 2^-24 of sum |q k|: its additions (a tensor core that
+cuts instead of rounding takes two for each of fewer, longer ones), 4 for q as the sum of two fp16 numbers
+(2^-22), the rest for scale, maximum and exponent.  A score's error is its weight's relative error, and
+a weighted mean moves by at most twice that times max |v|.  The sums over positions are cut into
+warps and tiles of 16 or more, so 2 * 32 half steps cover them at the lengths below:
+
+    tol = 2^-24 * (2 * (n + 16) * max_p sum |q k| / sqrt(n) + 64) * max |v|,   n = head_dim
+"""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+gpu = pytest.mark.gpu
+MAX_SCALE = 7168.0
+EINVAL, ENOMEM = -1, -3
+
+
+# ---- the format, in numpy ----
+
+def scale_of(top):
+    """Smallest multiple of 2^-21 of at most 7 significant bits with 7 s >= top, at most 7168."""
+    if top == 0:
+        return 0.0
+    t = top / 7
+    step = max(2.0 ** (math.floor(math.log2(t)) - 6), 2.0 ** -21)
+    s = math.floor(t / step) * step
+    while 7 * s < top:
+        s += step
+    return min(s, MAX_SCALE)
+
+
+def quantise(row):
+    """(scales [n/32], codes [n]) of one float32 row."""
+    g = np.asarray(row, np.float64).reshape(-1, 32)
+    scales, codes = [], []
+    for x in g:
+        if not np.isfinite(x).all():
+            scales.append(np.nan)
+            codes.append(np.full(32, 7, np.int64))
+            continue
+        s = scale_of(np.abs(x).max())
+        scales.append(s)
+        codes.append(np.clip(np.rint(x / s), -7, 8).astype(np.int64) + 7 if s else np.full(32, 7, np.int64))
+    return np.array(scales), np.concatenate(codes)
+
+
+def held(row):
+    s, u = quantise(row)
+    return np.repeat(s, 32) * (u - 7)
+
+
+class Pool:
+    """A host copy of a pool and its cells, read by the documented byte layout."""
+
+    def __init__(self, data, layers, hkv, hd):
+        self.data = np.ascontiguousarray(data).reshape(-1)
+        self.layers, self.hkv, self.hd = layers, hkv, hd
+
+    def block(self, page, layer, head):
+        n = 18 * self.hd
+        o = ((page * self.layers + layer) * self.hkv + head) * n
+        return self.data[o:o + n]
+
+    def row(self, page, r, layer, head, kind):
+        hd, blk = self.hd, self.block(page, layer, head)
+        out = np.empty(hd)
+        for d in range(hd):
+            if kind == 0:
+                byte = r * hd // 2 + ((d % 32 // 8) * (hd // 32) + d // 32) * 4 + d % 8 // 2
+            else:
+                byte = 8 * hd + r // 2 * hd + d // 4 * 4 + r % 2 * 2 + d % 4 // 2
+            at = (16 + kind) * hd + 2 * (r // 2 * 2 * (hd // 32) + d // 32 * 2 + r % 2)
+            s = np.frombuffer(blk[at:at + 2].tobytes(), np.float16)[0]
+            out[d] = float(s) * (int(blk[byte] >> (d % 2 * 4)) % 16 - 7)
+        return out
+
+    def rows(self, table, ctx, layer, head, kind):
+        return np.stack([self.row(table[p // 16], p % 16, layer, head, kind) for p in range(ctx)])
+
+
+def attend64(q, k, v):
+    """softmax(q k^T / sqrt(n)) v in 64 bits."""
+    s = q.astype(np.float64) @ k.T / math.sqrt(q.shape[1])
+    e = np.exp(s - s.max(1, keepdims=True))
+    return e / e.sum(1, keepdims=True) @ v
+
+
+def tolerance(q, k, v):
+    n = q.shape[1]
+    size = (np.abs(q.astype(np.float64)) @ np.abs(k).T).max() / math.sqrt(n)
+    return 2.0 ** -24 * (2 * (n + 16) * size + 64) * np.abs(v).max()
+
+
+def random_pool(rng, pages, layers, hkv, hd, spread=0.3):
+    """Random codes; scales of 7 significant bits."""
+    blk = np.empty((pages * layers * hkv, 18 * hd), np.uint8)
+    blk[:, :16 * hd] = rng.integers(0, 256, (len(blk), 16 * hd))
+    s = (rng.random((len(blk), hd)) * spread + 0.05).astype(np.float16)
+    blk[:, 16 * hd:] = (s.view(np.int16) & -16).view(np.uint8).reshape(len(blk), -1)
+    return blk.reshape(pages, -1)
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def host(t):
+    torch.cuda.synchronize()
+    return t.cpu().numpy()
+
+
+def status_word():
+    from glacier_b200._lib import lib
+    return lib().glacier_cuda_device_status(1)
+
+
+# ---- refusals (no GPU: every check comes before a launch) ----
+
+def capi(name, *args):
+    from glacier_b200._lib import lib
+    return getattr(lib(), name)(*args)
+
+
+def attend_args(**over):
+    a = dict(q=4096, pool=4096, num_pages=8, num_layers=2, tables=4096, max_pages=4, ctx=4096, lanes=2, layer=1,
+             h=8, hkv=2, hd=64, out=4096, ws=4096, ws_floats=1 << 24)
+    a.update(over)
+    return tuple(a.values()) + (None,)
+
+
+@pytest.mark.parametrize("over", [
+    dict(hd=96), dict(hd=32), dict(h=7), dict(h=18), dict(hkv=0), dict(layer=2), dict(num_pages=0), dict(lanes=0),
+    dict(lanes=1025), dict(max_pages=0), dict(pool=4104), dict(q=4100), dict(out=4100), dict(ws=4100),
+    dict(ws_floats=16), dict(q=None), dict(tables=None), dict(ctx=None), dict(out=None), dict(ws=None)])
+def test_attention_refusals(over):
+    assert capi("glacier_cuda_paged_attention_q4", *attend_args(**over)) == EINVAL
+
+
+@pytest.mark.parametrize("over", [
+    dict(hd=96), dict(h=7), dict(h=24), dict(hkv=0), dict(layer=2), dict(num_pages=0), dict(pool=4104), dict(ld=10),
+    dict(ldq=10), dict(positions=0), dict(qkv=None), dict(cos=None), dict(pos=None), dict(slots=None), dict(q=None)])
+def test_append_refusals(over):
+    a = dict(qkv=4096, ld=768, bias=None, cos=4096, sin=4096, positions=64, pos=4096, slots=4096, batch=2, h=8, hkv=2,
+             hd=64, q=4096, ldq=512, pool=4096, num_pages=8, num_layers=2, layer=1)
+    a.update(over)
+    assert capi("glacier_cuda_qkv_rope_append_q4", *a.values(), None) == EINVAL
+
+
+@pytest.mark.parametrize("over", [dict(hd=80), dict(layer=2), dict(slots=None), dict(k=4100), dict(v=None)])
+def test_read_refusals(over):
+    a = dict(pool=4096, num_pages=8, num_layers=2, layer=1, hkv=2, hd=64, slots=4096, rows=3, k=4096, v=4096)
+    a.update(over)
+    assert capi("glacier_cuda_kv_q4_read_f32", *a.values(), None) == EINVAL
+
+
+@pytest.mark.parametrize("over", [
+    dict(lanes=0), dict(lanes=1025), dict(max_pages=0), dict(capacity=0), dict(lens=None), dict(targets=None),
+    dict(targets=4096), dict(tables=None), dict(free=None), dict(count=None), dict(status=None), dict(positions=None),
+    dict(slots=None), dict(row_lanes=None), dict(stride=2, rows=7), dict(rows=0)])
+def test_resize_refusals(over):
+    a = dict(lens=4096, targets=8192, lanes=4, tables=4096, max_pages=4, free=4096, capacity=16, count=4096,
+             status=4096, stride=0, rows=8, positions=4096, row_lanes=4096, slots=4096, offsets=None)
+    a.update(over)
+    assert capi("glacier_cuda_kv_resize", *a.values(), None) == EINVAL
+
+
+def test_page_bytes_and_workspace():
+    assert capi("glacier_cuda_kv_q4_page_bytes", 28, 4, 128) == 28 * 4 * 2304
+    assert capi("glacier_cuda_kv_q4_page_bytes", 1, 2, 64) == 2 * 1152
+    assert capi("glacier_cuda_paged_attention_q4_workspace", 28, 4, 128) > 0
+    assert capi("glacier_cuda_paged_attention_q4_workspace", 28, 0, 128) == 0
+
+
+def test_wrappers_refuse_other_types_layouts_and_devices():
+    from glacier_b200 import ops
+    from glacier_b200._lib import GlacierCudaError
+    z = lambda *s, d=torch.float32: torch.zeros(s, dtype=d)  # noqa: E731
+    i = torch.int32
+    pages = z(4, ops.kv_q4_page_bytes(2, 2, 64), d=torch.uint8)
+    good = dict(q=z(2, 512), pages=pages, block_tables=z(2, 3, d=i), ctx_lens=z(2, d=i))
+    for bad in (dict(q=z(2, 512, d=torch.float16)), dict(q=z(2, 500)), dict(q=z(512, 2).t()),
+                dict(pages=pages[:, :-2]), dict(pages=z(4, 7, d=torch.uint8)), dict(block_tables=z(3, 3, d=i)),
+                dict(block_tables=z(2, 6, d=i)[:, ::2]), dict(ctx_lens=z(2, d=torch.int64)), {}):  # {}: on the CPU
+        with pytest.raises(GlacierCudaError):
+            ops.paged_attention_q4(**{**good, **bad}, num_layers=2, layer=0, num_heads=8, num_kv_heads=2, head_dim=64)
+    with pytest.raises(GlacierCudaError):
+        ops.kv_resize(z(2, d=i), z(2, d=i), z(2, 3, d=i), z(8, d=i), z(1, d=i), z(2, d=i), positions=z(4, d=i))
+    with pytest.raises(GlacierCudaError):
+        ops.qkv_rope_append_q4(z(2, 700), None, z(16, 32), z(16, 32), z(2, d=i), z(2, d=torch.int64), 8, 2, 64, pages,
+                               2, 0)
+    with pytest.raises(GlacierCudaError):
+        ops.kv_q4_read(pages, z(2, d=i), 2, 0, 2, 64)
+
+
+# ---- append and read ----
+
+EDGE_ROWS = [
+    np.zeros(32), np.full(32, 1e-30), np.full(32, 2.0 ** -21 * 7), np.linspace(-1, 1, 32), np.full(32, 7.0),
+    np.arange(32) - 15.5, np.full(32, 5e4), np.full(32, 50176.0), np.linspace(-1e6, 1e6, 32), np.full(32, 3.4e38),
+    np.r_[np.full(31, 0.5), 7.0], np.r_[np.full(31, -2.5), 7.0], np.r_[np.full(31, 3.5), -7.0],
+    np.r_[np.full(31, 1.0 + 2.0 ** -23), 7.0 + 2.0 ** -21], np.r_[np.zeros(31), np.inf], np.r_[np.nan, np.ones(31)],
+    np.r_[np.full(31, 3e-6), 1e-5], np.full(32, -1e-7)]
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_append_holds_what_the_format_says_at_its_edges(hd):
+    """No rotation (position 0), no bias: K and V rows of edge values are held exactly as defined."""
+    from glacier_b200 import ops
+    hkv, h, layers = 2, 2, 2
+    n = len(EDGE_ROWS)
+    x = np.zeros((n, (h + 2 * hkv) * hd), np.float32)
+    for i in range(n):
+        groups = [EDGE_ROWS[(i + j) % n] for j in range(2 * hkv * hd // 32)]
+        x[i, h * hd:] = np.concatenate(groups).astype(np.float32)
+    cos, sin = np.ones((4, hd // 2), np.float32), np.zeros((4, hd // 2), np.float32)
+    # a rotation by 0 of a NaN or an infinity multiplies it by sin 0: NaN in the partner's group too
+    pages = dev(np.full((3, ops.kv_q4_page_bytes(layers, hkv, hd)), 0xA5, np.uint8))
+    slots = dev(np.arange(n, dtype=np.int64) + 5)
+    ops.qkv_rope_append_q4(dev(x), None, dev(cos), dev(sin), dev(np.zeros(n, np.int32)), slots, h, hkv, hd, pages,
+                           layers, 1)
+    k, v = (host(t).reshape(n, hkv, hd) for t in ops.kv_q4_read(pages, slots, layers, 1, hkv, hd))
+    pool = Pool(host(pages), layers, hkv, hd)
+    for i in range(n):
+        for j in range(hkv):
+            row = x[i, (h + j) * hd:(h + j + 1) * hd]
+            a, b = row[:hd // 2], row[hd // 2:]
+            with np.errstate(invalid="ignore"):
+                rot = np.concatenate((a * 1 - b * np.float32(0), a * np.float32(0) + b * 1))
+            ref_k, ref_v = held(rot), held(x[i, (h + hkv + j) * hd:(h + hkv + j + 1) * hd])
+            np.testing.assert_array_equal(k[i, j], ref_k)
+            np.testing.assert_array_equal(v[i, j], ref_v)
+            slot = i + 5
+            np.testing.assert_array_equal(pool.row(slot // 16, slot % 16, 1, j, 0), ref_k)
+            np.testing.assert_array_equal(pool.row(slot // 16, slot % 16, 1, j, 1), ref_v)
+    # the other layer, and positions that no slot names, are as they were
+    data = host(pages).reshape(3, layers, -1)
+    assert (data[:, 0] == 0xA5).all()
+    for slot in (4, 5 + n):
+        for j in range(hkv):
+            blk = pool.block(slot // 16, 1, j)
+            r = slot % 16
+            assert (blk[r * hd // 2:(r + 1) * hd // 2] == 0xA5).all()
+            assert (blk[8 * hd + r // 2 * hd:][:hd].reshape(-1, 2, 2)[:, r % 2] == 0xA5).all()
+    assert status_word() == 0
+
+
+@gpu
+@pytest.mark.parametrize("h,hkv,hd,batch", [(14, 2, 64, 1), (28, 4, 128, 5), (8, 8, 64, 3), (3, 3, 128, 33),
+                                            (16, 2, 128, 128), (5, 1, 64, 2)])
+@pytest.mark.parametrize("odd", [False, True])  # odd: row strides and pointers off 16 bytes
+def test_append_rotates_and_quantises(h, hkv, hd, batch, odd):
+    from glacier_b200 import ops
+    rng = np.random.default_rng(h * 1000 + batch)
+    width, layers, P = (h + 2 * hkv) * hd, 3, 600
+    x = rng.standard_normal((batch, width + 3), dtype=np.float32) * 2
+    bias = rng.standard_normal(width, dtype=np.float32)
+    ang = rng.random((P, hd // 2)) * 6.3
+    cos, sin = np.cos(ang).astype(np.float32), np.sin(ang).astype(np.float32)
+    pos = rng.integers(0, P, batch).astype(np.int32)
+    slots = rng.permutation(16 * 40)[:batch].astype(np.int64)
+    if batch > 2:
+        slots[1] = -1
+    pages = dev(rng.integers(0, 256, (40, ops.kv_q4_page_bytes(layers, hkv, hd)), dtype=np.uint8))
+    t = dev(x)[:, 1:1 + width] if odd else dev(x[:, 1:1 + width])
+    q = host(ops.qkv_rope_append_q4(t, dev(bias), dev(cos), dev(sin), dev(pos), dev(slots), h, hkv, hd, pages, layers,
+                                    2))
+    k, v = (host(a) for a in ops.kv_q4_read(pages, dev(slots), layers, 2, hkv, hd))
+    y = (x[:, 1:1 + width] + bias).reshape(batch, h + 2 * hkv, hd)
+    c, s = cos[pos][:, None], sin[pos][:, None]
+    a, b = y[:, :h + hkv, :hd // 2], y[:, :h + hkv, hd // 2:]
+    r32 = np.concatenate((a * c - b * s, a * s + b * c), -1)  # float32, each operation rounded
+    r64 = np.concatenate((a.astype(np.float64) * c - b.astype(np.float64) * s,
+                          a.astype(np.float64) * s + b.astype(np.float64) * c), -1)
+    size = np.concatenate((np.abs(a) + np.abs(b),) * 2, -1)
+    for i in range(batch):
+        if slots[i] < 0:
+            assert not q[i].any() and not k[i].any() and not v[i].any()
+            continue
+        assert (np.abs(q[i].reshape(h, hd) - r64[i, :h]) <= 3 * 2.0 ** -24 * size[i, :h]).all()
+        np.testing.assert_array_equal(k[i], np.concatenate([held(r32[i, h + j]) for j in range(hkv)]))
+        np.testing.assert_array_equal(v[i], np.concatenate([held(y[i, h + hkv + j]) for j in range(hkv)]))
+    assert status_word() == 0
+
+
+@gpu
+def test_append_and_read_report_slots_and_positions_out_of_range():
+    from glacier_b200 import ops
+    h, hkv, hd = 4, 2, 64
+    pages = dev(np.full((2, ops.kv_q4_page_bytes(1, hkv, hd)), 0x5A, np.uint8))
+    x = torch.ones((4, (h + 2 * hkv) * hd), device="cuda")
+    cos, sin = torch.ones((8, hd // 2), device="cuda"), torch.zeros((8, hd // 2), device="cuda")
+    for slots, pos in (([32, -1, -1, -1], [0] * 4), ([-2, -1, -1, -1], [0] * 4), ([0, -1, -1, -1], [8, 0, 0, 0]),
+                       ([0, -1, -1, -1], [-1, 0, 0, 0]), ([2 ** 40, -1, -1, -1], [0] * 4)):
+        q = ops.qkv_rope_append_q4(x, None, cos, sin, dev(np.array(pos, np.int32)), dev(np.array(slots, np.int64)), h,
+                                   hkv, hd, pages, 1, 0)
+        assert not host(q).any()
+        assert status_word() == 2
+    assert (host(pages) == 0x5A).all()
+    k, v = ops.kv_q4_read(pages, dev(np.array([32, -1], np.int64)), 1, 0, hkv, hd)
+    assert not host(k).any() and not host(v).any() and status_word() == 2
+
+
+# ---- page bookkeeping ----
+
+def resize_ref(lens, targets, table, free, count, stride, rows):
+    lens, table, free = list(lens), table.copy(), free.copy()
+    lanes, max_pages = table.shape
+    pg = lambda n: -(-n // 16)  # noqa: E731
+    status = [0] * lanes
+    valid = []
+    for b in range(lanes):
+        ok = 0 <= lens[b] <= 16 * max_pages and 0 <= targets[b] <= 16 * max_pages
+        valid.append(ok and not (stride and targets[b] - lens[b] > stride))
+    back = [table[b, j] for b in range(lanes) if valid[b] for j in range(pg(targets[b]), pg(lens[b]))]
+    stack = list(free[:count]) + back[::-1]
+    top = len(stack)
+    free[:top] = stack
+    out, wanted_pages, wanted_rows, used, off = [], 0, 0, 0, [0]
+    new = list(lens)
+    for b in range(lanes):
+        got = []
+        if not valid[b]:
+            status[b] = EINVAL
+        else:
+            need, grow = max(0, pg(targets[b]) - pg(lens[b])), max(0, targets[b] - lens[b])
+            wanted_pages += need
+            wanted_rows += grow
+            if (need and wanted_pages > top) or (grow and not stride and wanted_rows > rows):
+                status[b] = ENOMEM
+            else:
+                for i in range(need):
+                    table[b, pg(lens[b]) + i] = stack[top - 1 - used - i]
+                used += need
+                got = list(range(lens[b], targets[b]))
+                new[b] = targets[b]
+        cells = [(p, b, int(table[b, p // 16]) * 16 + p % 16) for p in got]
+        out += cells + [(-1, -1, -1)] * (stride - len(cells) if stride else 0)
+        off.append(len(out))
+    out += [(-1, -1, -1)] * (rows - len(out))
+    return new, table, free, top - used, status, np.array(out), off
+
+
+RESIZES = {
+    "one lane from nothing": dict(lens=[0], targets=[1]),
+    "page borders": dict(lens=[0, 15, 16, 17, 31, 32], targets=[16, 16, 17, 32, 33, 49]),
+    "unchanged and empty": dict(lens=[0, 5, 16, 0], targets=[0, 5, 16, 0]),
+    "shrink and release": dict(lens=[40, 16, 33, 100, 1], targets=[33, 0, 32, 0, 0]),
+    "pages of one lane go to another": dict(lens=[100, 0, 64, 0], targets=[0, 90, 1, 60], spare=0),
+    "pages run out": dict(lens=[10, 0, 16, 5, 0], targets=[11, 40, 17, 6, 1], spare=2),
+    "rows run out": dict(lens=[0, 0, 0, 3], targets=[20, 30, 5, 3], rows=27),
+    "bad lengths": dict(lens=[5, -1, 4, 300, 7], targets=[6, 3, -2, 10, 10 ** 9], max_pages=8),
+    "one row each": dict(lens=[0, 15, 16, 7, 47], targets=[1, 16, 17, 7, 40], stride=1),
+    "three rows each, one too many": dict(lens=[0, 15, 16, 7], targets=[3, 16, 20, 9], stride=3),
+    "a full house": dict(lens=[i * 7 % 50 for i in range(1024)], targets=[i * 13 % 60 for i in range(1024)]),
+    "many rows": dict(lens=[0] * 37, targets=[(i * 397) % 1500 for i in range(37)]),
+    "many padded rows": dict(lens=[3] * 9, targets=[(i * 97) % 1000 for i in range(9)], stride=1000),
+}
+
+
+@gpu
+@pytest.mark.parametrize("name", list(RESIZES))
+def test_resize(name):
+    from glacier_b200 import ops
+    c = RESIZES[name]
+    rng = np.random.default_rng(len(name))
+    lens, targets, stride = c["lens"], c["targets"], c.get("stride", 0)
+    lanes = len(lens)
+    sane = [n for n in lens + targets if 0 <= n < 10 ** 6]
+    max_pages = c.get("max_pages", max(1, -(-max(sane) // 16)) + 1)
+    held_pages = [-(-min(max(n, 0), 16 * max_pages) // 16) for n in lens]
+    spare = c.get("spare", sum(-(-max(0, t) // 16) for t in targets if t < 10 ** 6) + 3)
+    perm = rng.permutation(sum(held_pages) + spare).astype(np.int32)
+    table = np.full((lanes, max_pages), -9, np.int32)
+    at = 0
+    for b, n in enumerate(held_pages):
+        table[b, :n] = perm[at:at + n]
+        at += n
+    free = np.full(len(perm) + 2, -7, np.int32)
+    free[:spare] = perm[at:]
+    rows = lanes * stride if stride else c.get("rows", max(1, sum(max(0, t - n) for n, t in zip(lens, targets)
+                                                                  if t < 10 ** 6)) + 5)
+    t = dict(lens=dev(np.array(lens, np.int32)), table=dev(table), free=dev(free), count=dev(np.array([spare], np.int32)))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    status, offsets = torch.full((lanes,), 99, **i32), torch.full((lanes + 1,), 99, **i32)
+    pos, who = torch.full((rows,), 99, **i32), torch.full((rows,), 99, **i32)
+    slots = torch.full((rows,), 99, dtype=torch.int64, device="cuda")
+    ops.kv_resize(t["lens"], dev(np.array(targets, np.int32)), t["table"], t["free"], t["count"], status,
+                  positions=pos, row_lanes=who, slots=slots, row_offsets=offsets, row_stride=stride)
+    new, table2, free2, count2, st, cells, off = resize_ref(lens, targets, table, free, spare, stride, rows)
+    assert host(status).tolist() == st
+    assert host(t["lens"]).tolist() == new
+    np.testing.assert_array_equal(host(t["table"]), table2)
+    assert host(t["count"])[0] == count2
+    np.testing.assert_array_equal(host(t["free"])[:count2], free2[:count2])
+    np.testing.assert_array_equal(np.stack([host(pos), host(who), host(slots)], 1), cells)
+    assert host(offsets).tolist() == off
+    # back to where it was: the pages return so that the same growth takes the same ones again
+    if all(s == 0 for s in st) and all(a <= b for a, b in zip(lens, targets)):
+        ops.kv_resize(t["lens"], dev(np.array(lens, np.int32)), t["table"], t["free"], t["count"], status)
+        assert host(t["lens"]).tolist() == lens and host(t["count"])[0] == spare
+        np.testing.assert_array_equal(host(t["free"])[:spare], free[:spare])
+
+
+# ---- attention ----
+
+CTX = {
+    "one position": [1],
+    "page borders": [15, 16, 17, 31, 32, 33, 47, 48, 49],
+    "an empty lane among others": [5, 0, 64, 0, 200, 0],
+    "all empty": [0, 0],
+    "one long": [2111],
+    "ragged": [1, 700, 33, 1290, 64, 2, 255, 16],
+    "many short lanes": [(i * 37) % 90 for i in range(300)],
+}
+HEADS = [(14, 2, 64), (28, 4, 128), (8, 8, 64), (3, 3, 128), (16, 2, 128), (5, 1, 64), (8, 2, 64), (6, 1, 128)]
+
+
+def attention_case(rng, h, hkv, hd, ctxs, layers=2, layer=1):
+    lanes = len(ctxs)
+    max_pages = max(1, max(-(-c // 16) for c in ctxs)) + 1
+    total = sum(-(-c // 16) for c in ctxs) + 2
+    perm = rng.permutation(total)
+    table = np.full((lanes, max_pages), 2 ** 30, np.int32)  # entries past a lane's pages name nothing
+    at = 0
+    for b, c in enumerate(ctxs):
+        n = -(-c // 16)
+        table[b, :n] = perm[at:at + n]
+        at += n
+    data = random_pool(rng, total, layers, hkv, hd)
+    pool = Pool(data, layers, hkv, hd)
+    # what lies behind a lane's last position is left over from others: NaN and infinite scales
+    for b, c in enumerate(ctxs):
+        for p in range(c, -(-c // 16) * 16):
+            for j in range(hkv):
+                blk = pool.block(table[b, p // 16], layer, j)
+                for kind in (0, 1):
+                    for g in range(hd // 32):
+                        at = (16 + kind) * hd + 2 * (p % 16 // 2 * 2 * (hd // 32) + 2 * g + p % 2)
+                        blk[at:at + 2] = np.frombuffer(np.float16([np.nan, np.inf][(p + g) % 2]).tobytes(), np.uint8)
+    q = rng.standard_normal((lanes, h * hd), dtype=np.float32) * 1.5
+    return q, pool, table
+
+
+def check_attention(out, q, pool, table, ctxs, h, hkv, hd, layer=1, lanes=None):
+    G = h // hkv
+    for b in (range(len(ctxs)) if lanes is None else lanes):
+        if ctxs[b] == 0:
+            assert not out[b].any()
+            continue
+        for j in range(hkv):
+            k, v = (pool.rows(table[b], ctxs[b], layer, j, kind) for kind in (0, 1))
+            qs = q[b].reshape(h, hd)[j * G:(j + 1) * G]
+            err = np.abs(out[b].reshape(h, hd)[j * G:(j + 1) * G] - attend64(qs, k, v)).max()
+            assert err <= tolerance(qs, k, v), (b, j, err, tolerance(qs, k, v))
+
+
+@gpu
+@pytest.mark.parametrize("name", list(CTX))
+@pytest.mark.parametrize("h,hkv,hd", HEADS[:4])
+def test_attention_contexts(name, h, hkv, hd):
+    from glacier_b200 import ops
+    ctxs = CTX[name]
+    rng = np.random.default_rng(len(name) + h)
+    q, pool, table = attention_case(rng, h, hkv, hd, ctxs)
+    pages = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd)))
+    out = host(ops.paged_attention_q4(dev(q), pages, dev(table), dev(np.array(ctxs, np.int32)), 2, 1, h, hkv, hd))
+    lanes = None if len(ctxs) < 20 else list(range(0, len(ctxs), 29)) + [len(ctxs) - 1]
+    if sum(ctxs) > 1000 and lanes is None:  # the layout is read cell by cell in Python: a few lanes suffice
+        lanes = [b for b in range(len(ctxs)) if ctxs[b] < 800 or len(ctxs) == 1]
+    check_attention(out, q, pool, table, ctxs, h, hkv, hd, lanes=lanes)
+    assert status_word() == 0
+
+
+@gpu
+@pytest.mark.parametrize("h,hkv,hd", HEADS)
+def test_attention_heads(h, hkv, hd):
+    from glacier_b200 import ops
+    ctxs = [77, 3, 160]
+    rng = np.random.default_rng(h * hd)
+    q, pool, table = attention_case(rng, h, hkv, hd, ctxs, layers=1, layer=0)
+    pages = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(1, hkv, hd)))
+    out = host(ops.paged_attention_q4(dev(q), pages, dev(table), dev(np.array(ctxs, np.int32)), 1, 0, h, hkv, hd))
+    check_attention(out, q, pool, table, ctxs, h, hkv, hd, layer=0)
+
+
+@gpu
+@pytest.mark.parametrize("scale_q", [1e-6, 30.0, 3e4])
+def test_attention_of_tiny_and_huge_queries(scale_q):
+    """A flat softmax, and ones that put all their weight on one position; one head of zeros."""
+    from glacier_b200 import ops
+    h, hkv, hd, ctxs = 7, 1, 128, [130]
+    rng = np.random.default_rng(3)
+    q, pool, table = attention_case(rng, h, hkv, hd, ctxs)
+    q = (q * np.float32(scale_q)).astype(np.float32)
+    q[0, 2 * hd:3 * hd] = 0
+    pages = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd)))
+    out = host(ops.paged_attention_q4(dev(q), pages, dev(table), dev(np.array(ctxs, np.int32)), 2, 1, h, hkv, hd))
+    k, v = (pool.rows(table[0], ctxs[0], 1, 0, kind) for kind in (0, 1))
+    for g in range(h):
+        qs = q.reshape(h, hd)[g:g + 1]
+        err = np.abs(out.reshape(h, hd)[g] - attend64(qs, k, v)[0]).max()
+        assert err <= tolerance(qs, k, v), g
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_of_small_and_large_held_values(hd):
+    """Scales over the format's whole range, mixed within a lane and from lane to lane."""
+    from glacier_b200 import ops
+    h, hkv, ctxs = 4, 2, [50, 50, 50]
+    rng = np.random.default_rng(hd)
+    q, pool, table = attention_case(rng, h, hkv, hd, ctxs)
+    for b, (lo, hi) in enumerate(((-21, -15), (8, 12.8), (-21, 12.8))):
+        for page in table[b, :4]:
+            for j in range(hkv):
+                blk = pool.block(page, 1, j)
+                for kind in (0, 1):
+                    at = slice((16 + kind) * hd, (17 + kind) * hd)
+                    s = np.ldexp(1.0, 0) * 2.0 ** rng.uniform(lo, hi, hd // 2)
+                    step = np.maximum(2.0 ** (np.floor(np.log2(s)) - 6), 2.0 ** -21)
+                    s = np.minimum(np.floor(s / step) * step, MAX_SCALE)
+                    blk[at] = np.frombuffer(s.astype(np.float16).tobytes(), np.uint8)
+                    assert (s.astype(np.float16).astype(np.float64) == s).all()
+    q[1:] *= 1e-4
+    pages = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd)))
+    out = host(ops.paged_attention_q4(dev(q), pages, dev(table), dev(np.array(ctxs, np.int32)), 2, 1, h, hkv, hd))
+    check_attention(out, q, pool, table, ctxs, h, hkv, hd)
+
+
+@gpu
+def test_attention_poison_stays_in_its_lane_and_head():
+    """A NaN scale makes the heads that attend it NaN, and nothing else."""
+    from glacier_b200 import ops
+    h, hkv, hd, ctxs = 8, 2, 64, [40, 40]
+    rng = np.random.default_rng(8)
+    q, pool, table = attention_case(rng, h, hkv, hd, ctxs)
+    bad = np.frombuffer(np.float16(np.nan).tobytes(), np.uint8)
+    blk = pool.block(table[0, 1], 1, 0)  # lane 0, kv head 0, K of position 16 + 2, group 1
+    blk[16 * hd + 2 * (1 * 4 + 2):][:2] = bad
+    blk = pool.block(table[1, 0], 1, 1)  # lane 1, kv head 1, V of position 5, group 0
+    blk[17 * hd + 2 * (2 * 4 + 1):][:2] = bad
+    pages = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd)))
+    out = host(ops.paged_attention_q4(dev(q), pages, dev(table), dev(np.array(ctxs, np.int32)), 2, 1, h, hkv, hd))
+    nan = np.isnan(out.reshape(2, hkv, h // hkv, hd))
+    assert nan[0, 0].all() and not nan[0, 1].any() and not nan[1, 0].any()
+    assert nan[1, 1][:, :32].all() and not nan[1, 1][:, 32:].any()
+
+
+@gpu
+def test_attention_clamps_the_context_and_leaves_out_bad_pages():
+    from glacier_b200 import ops
+    h, hkv, hd = 4, 2, 128
+    rng = np.random.default_rng(12)
+    q, pool, table = attention_case(rng, h, hkv, hd, [48, 64, 30])
+    table = np.ascontiguousarray(table[:, :4])
+    pages = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd)))
+    run = lambda t, c: host(ops.paged_attention_q4(dev(q), pages, dev(t), dev(np.array(c, np.int32)), 2, 1, h, hkv, hd))  # noqa: E731
+    good = run(table, [48, 64, 30])
+    np.testing.assert_array_equal(run(table, [48, 2 ** 31 - 1, 30])[1], good[1])  # past the table: clamped
+    np.testing.assert_array_equal(run(table, [48, 64, -5])[2], 0)
+    assert status_word() == 0
+    # lane 0 loses its middle page, lane 2 every page
+    broken = table.copy()
+    broken[0, 1], broken[2] = -1, 2 ** 31 - 1
+    out = run(broken, [48, 64, 30])
+    assert status_word() == 2
+    np.testing.assert_array_equal(out[1], good[1])
+    assert not out[2].any()
+    keep = np.r_[0:16, 32:48]
+    for j in range(hkv):
+        k, v = (pool.rows(table[0], 48, 1, j, kind)[keep] for kind in (0, 1))
+        qs = q[0].reshape(h, hd)[j * 2:j * 2 + 2]
+        err = np.abs(out[0].reshape(h, hd)[j * 2:j * 2 + 2] - attend64(qs, k, v)).max()
+        assert err <= tolerance(qs, k, v)
+
+
+@gpu
+def test_attention_is_the_same_every_time_and_on_any_stream():
+    """Bit-identical results from a reused workspace, another stream, and a captured graph that is
+    replayed on new inputs."""
+    from glacier_b200 import ops
+    h, hkv, hd, ctxs = 28, 4, 128, [500, 0, 1200, 17, 90]
+    rng = np.random.default_rng(21)
+    q, pool, table = attention_case(rng, h, hkv, hd, ctxs)
+    pages, t, c = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd))), dev(table), dev(np.array(ctxs, np.int32))
+    qd, ws = dev(q), ops.paged_attention_q4_workspace(h, hkv, hd)
+    args = (pages, t, c, 2, 1, h, hkv, hd)
+    ref = host(ops.paged_attention_q4(qd, *args, workspace=ws))
+    ws.fill_(float("nan"))
+    np.testing.assert_array_equal(host(ops.paged_attention_q4(qd, *args, workspace=ws)), ref)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    out = ops.paged_attention_q4(qd, *args, stream=side)
+    side.synchronize()
+    np.testing.assert_array_equal(out.cpu().numpy(), ref)
+    graph = torch.cuda.CUDAGraph()
+    qg, cg, og = qd.clone(), c.clone(), torch.empty_like(qd)
+    with torch.cuda.graph(graph):
+        ops.paged_attention_q4(qg, pages, t, cg, 2, 1, h, hkv, hd, out=og, workspace=ws)
+    graph.replay()
+    np.testing.assert_array_equal(host(og), ref)
+    other = rng.standard_normal(q.shape, dtype=np.float32)
+    qg.copy_(dev(other))
+    cg.copy_(dev(np.array([16, 300, 7, 0, 33], np.int32).clip(0, np.array(ctxs, np.int32))))
+    graph.replay()
+    got = host(og)
+    np.testing.assert_array_equal(got, host(ops.paged_attention_q4(dev(other), pages, t, cg, 2, 1, h, hkv, hd)))
+
+
+@gpu
+def test_attention_offsets_past_32_bits():
+    """A pool of more than 4 GiB whose used pages lie at its far end."""
+    from glacier_b200 import ops
+    h, hkv, hd, ctxs, layers = 4, 1, 128, [40], 64
+    rng = np.random.default_rng(5)
+    q, pool, table = attention_case(rng, h, hkv, hd, ctxs, layers=layers, layer=63)
+    pb = ops.kv_q4_page_bytes(layers, hkv, hd)
+    n = (1 << 32) // pb + 40
+    pages = torch.zeros((n, pb), dtype=torch.uint8, device="cuda")
+    used = pool.data.reshape(-1, pb)
+    pages[n - len(used):] = dev(used)
+    t = np.where(table < len(used), table + (n - len(used)), table).astype(np.int32)
+    out = host(ops.paged_attention_q4(dev(q), pages, dev(t), dev(np.array(ctxs, np.int32)), layers, 63, h, hkv, hd))
+    check_attention(out, q, pool, table, ctxs, h, hkv, hd, layer=63)
+    slot = torch.tensor([n * 16 - 1], device="cuda")
+    x = torch.randn((1, (h + 2 * hkv) * hd), device="cuda")
+    one = torch.ones((1, hd // 2), device="cuda")
+    ops.qkv_rope_append_q4(x, None, one, one * 0, torch.zeros(1, dtype=torch.int32, device="cuda"), slot, h, hkv, hd,
+                           pages, layers, 63)
+    _, v = ops.kv_q4_read(pages, slot, layers, 63, hkv, hd)
+    np.testing.assert_array_equal(host(v)[0], held(x[0, -hd:].cpu().numpy()))
+
+
+# ---- together, as a decode loop uses them ----
+
+@gpu
+@pytest.mark.parametrize("h,hkv,hd", [(14, 2, 64), (28, 4, 128)])
+def test_a_decode_loop_over_a_shared_pool(h, hkv, hd):
+    """Requests of different ages grow position by position, end, and give their pages to new ones; every
+    step's attention equals the 64-bit one over the rows that the requests appended themselves."""
+    from glacier_b200 import ops
+    rng = np.random.default_rng(h)
+    lanes, max_pages, P, width = 3, 4, 64, (h + 2 * hkv) * hd
+    i32 = dict(dtype=torch.int32, device="cuda")
+    pages = torch.full((7, ops.kv_q4_page_bytes(1, hkv, hd)), 0xEE, dtype=torch.uint8, device="cuda")
+    table, free = torch.full((lanes, max_pages), -1, **i32), torch.arange(7, **i32)
+    lens, count, status = torch.zeros(lanes, **i32), torch.tensor([7], **i32), torch.zeros(lanes, **i32)
+    pos, who = torch.empty(lanes, **i32), torch.empty(lanes, **i32)
+    slots = torch.empty(lanes, dtype=torch.int64, device="cuda")
+    ang = np.arange(P)[:, None] * 1e4 ** (-np.arange(hd // 2) / (hd // 2))
+    cos, sin = np.cos(ang).astype(np.float32), np.sin(ang).astype(np.float32)
+    kept = [[] for _ in range(lanes)]
+    ends = [19, 33, 40]
+    for step in range(45):
+        target = [0 if len(kept[b]) >= ends[b] else len(kept[b]) + 1 for b in range(lanes)]
+        ops.kv_resize(lens, dev(np.array(target, np.int32)), table, free, count, status, positions=pos,
+                      row_lanes=who, slots=slots, row_stride=1)
+        assert host(status).tolist() == [0] * lanes
+        x = rng.standard_normal((lanes, width), dtype=np.float32)
+        q = ops.qkv_rope_append_q4(dev(x), None, dev(cos), dev(sin), pos, slots, h, hkv, hd, pages, 1, 0)
+        out = host(ops.paged_attention_q4(q, pages, table, lens, 1, 0, h, hkv, hd))
+        qh = host(q)
+        for b in range(lanes):
+            if target[b] == 0:
+                kept[b] = []
+                assert not out[b].any()
+                continue
+            p = len(kept[b])
+            y = x[b].reshape(-1, hd)
+            a, c = y[h:h + hkv, :hd // 2], y[h:h + hkv, hd // 2:]
+            k = np.concatenate((a * cos[p] - c * sin[p], a * sin[p] + c * cos[p]), -1)
+            kept[b].append(([held(r) for r in k], [held(r) for r in y[h + hkv:]]))
+            for j in range(hkv):
+                ks, vs = (np.stack([r[i][j] for r in kept[b]]) for i in (0, 1))
+                qs = qh[b].reshape(h, hd)[j * h // hkv:(j + 1) * h // hkv]
+                err = np.abs(out[b].reshape(h, hd)[j * h // hkv:(j + 1) * h // hkv] - attend64(qs, ks, vs)).max()
+                assert err <= tolerance(qs, ks, vs), (step, b, j)
+    assert status_word() == 0
