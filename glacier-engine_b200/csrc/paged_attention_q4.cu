@@ -7,8 +7,7 @@
 // G <= 8 query heads of a group need 4 G hd products on them: on the fp32 pipe that
 // is more time than the bytes take, so both products run as mma.sync m16n8k16
 // (fp16 in, fp32 sums).  M is the query heads, and eight of them would leave half of the
-// sixteen rows idle: rows 0-7 hold the high and rows 8-15 the low fp16 part of the same
-// float32 numbers, so q and the weights enter with 22 bits at no extra instruction.  (A
+// sixteen rows idle: X  (A
 // tcgen05.mma needs 64 or 128 rows and its operands in shared memory as fp16: the codes
 // would be unpacked, written and read once more, which is what bounds this kernel.)
 //   * K: a code c is used as the fp16 number whose bits are the code: c * 2^-24, or c * 2^-20
@@ -24,16 +23,16 @@
 
 namespace glacier {
 
-__device__ int g_attn_q4_error;
-
 namespace {
 
 constexpr int kMaxLanes = 1024;
-constexpr int kStagePages = 2;  // pages per pipeline stage of a warp
-constexpr int kStagePos = kStagePages * kQ4Page;
 constexpr int kWarps = 12;
+constexpr int kStages = 3;  // stages in a warp's ring: 166 KB of K/V in flight per SM
+// Pages per stage: 4608 bytes at either head size.
 template <int HD>
-constexpr int kStages = HD == 128 ? 3 : 6;  // 166 KB of K/V in flight per SM
+constexpr int kStagePages = HD == 128 ? 2 : 4;
+template <int HD>
+constexpr int kStagePos = kStagePages<HD> * kQ4Page;
 
 struct AttnQ4Params {
   const float* q;
@@ -50,7 +49,6 @@ struct AttnQ4Params {
   int lanes, max_pages, num_pages, layer, num_heads, num_kv_heads;
   float scale_log2;
   int* bad;
-  int* err;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -71,11 +69,11 @@ __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cas
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
 // (hi, lo) fp16 pairs of two float32 numbers: x = hi + lo to 22 bits.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
+__device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x.x, x.y);
+  const float2 r = __ffma2_rn(__half22float2(h), make_float2(-1.f, -1.f), x);
   hi = h2_bits(h);
-  lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
+  lo = h2_bits(__floats2half2_rn(r.x, r.y));
 }
 
 // fp16 bits of 64 + (15 - c) for the nibbles c at bits 4-7 of both halves of x.
@@ -85,12 +83,14 @@ __device__ __forceinline__ uint32_t v_bits(uint32_t x) {
   return d;
 }
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
-          smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
-      : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 template <int N>
@@ -153,7 +153,7 @@ __device__ __forceinline__ void load_q(const AttnQ4Params& p, int lid, int kvh, 
     for (int i = 0; i < 4; ++i) {
       const float m = (i & 1) ? inv * 0.0625f : inv;
       uint32_t hi, lo;
-      split2(v[g][i] * m, v[g][i + 4] * m, hi, lo);
+      split2(make_float2(v[g][i] * m, v[g][i + 4] * m), hi, lo);
       q.a[2 * g + (i >> 1)][(i & 1) * 2] = hi;
       q.a[2 * g + (i >> 1)][(i & 1) * 2 + 1] = lo;
       const float w = (i & 1) ? 16.f : 1.f;
@@ -170,19 +170,21 @@ __device__ __forceinline__ void load_q(const AttnQ4Params& p, int lid, int kvh, 
   }
 }
 
-// One stage (two pages) of one warp: scores, online softmax, and the weighted V.  m is the
-// running maximum (base 2) of head lane / 4, l this thread's share of its sum; weights carry
-// 2^15 so that their low parts stay normal fp16 numbers, o carries 2^15 / 8.
+// One stage of one warp: scores, online softmax, and the weighted V.  Weights are 2^(7 + s - m)
+// in base-2 scores s: m is a reference near the running maximum of head lane / 4, moved
+// (and everything rescaled) only when a score passes it by more than 2^8, so the weights stay
+// below 2^15 and their low parts normal fp16 numbers.  l: this thread's share of their
+// sum; o: sums of weight * v / 8.
 // nvalid: positions of the stage inside the context; pages: bit i set when page i was loaded.
 template <int HD, bool MASK>
-__device__ __forceinline__ void stage_math(const uint8_t* __restrict__ buf, const QFrag<HD>& q, float& m, float& l,
-                                           float (&o)[HD / 8][4], int nvalid, uint32_t pages, int lane) {
+__device__ __forceinline__ void stage_math(const uint8_t* __restrict__ buf, const QFrag<HD>& q, float& m, float2& l,
+                                           float (&o)[HD / 16][4], int nvalid, uint32_t pages, int lane) {
   constexpr int NG = HD / 32, NW = HD / 32;  // scale groups; words per thread and position (K) or pair (V)
-  constexpr int BLK = 18 * HD;
+  constexpr int BLK = 18 * HD, SP = kStagePages<HD>;
   const int n = lane >> 2, t = lane & 3;
-  float2 sc[kStagePages * 2];
+  float2 sc[SP * 2];
 #pragma unroll
-  for (int pg = 0; pg < kStagePages; ++pg) {
+  for (int pg = 0; pg < SP; ++pg) {
     const uint8_t* K = buf + pg * BLK;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -199,8 +201,6 @@ __device__ __forceinline__ void stage_math(const uint8_t* __restrict__ buf, cons
         r = __ffma2_rn(f, make_float2(d[0], d[1]), r);
         r = __ffma2_rn(f, make_float2(d[2], d[3]), r);
       }
-      r.x *= q.f;
-      r.y *= q.f;
       if constexpr (MASK) {
         const int at = pg * kQ4Page + 8 * j + 2 * t;
         const bool here = (pages >> pg) & 1;
@@ -212,28 +212,36 @@ __device__ __forceinline__ void stage_math(const uint8_t* __restrict__ buf, cons
   }
   float mx = fmaxf(sc[0].x, sc[0].y);
 #pragma unroll
-  for (int i = 1; i < 2 * kStagePages; ++i) mx = fmaxf(mx, fmaxf(sc[i].x, sc[i].y));
+  for (int i = 1; i < 2 * SP; ++i) mx = fmaxf(mx, fmaxf(sc[i].x, sc[i].y));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-  if (__any_sync(0xffffffffu, mx > m)) {
-    const float mn = fmaxf(m, mx);
-    const float a = m == -INFINITY ? 0.f : ex2(m - mn);
+  const bool move = (mx - m) * q.f > 8.f;  // false for NaN: no score yet
+  if (__any_sync(0xffffffffu, move)) {
+    const float mn = move ? mx : m;
+    const float a = m == -INFINITY ? 0.f : ex2((m - mn) * q.f);
     m = mn;
-    l *= a;
+    l.x *= a;
+    l.y *= a;
+    const float a0 = __shfl_sync(0xffffffffu, a, 8 * t), a1 = __shfl_sync(0xffffffffu, a, 8 * t + 4);
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[i][c] *= a;
+    for (int i = 0; i < HD / 16; ++i) {
+      o[i][0] *= a0;
+      o[i][1] *= a1;
+      o[i][2] *= a0;
+      o[i][3] *= a1;
+    }
   }
-  const float base = m == -INFINITY ? 15.f : 15.f - m;
+  const float base = m == -INFINITY ? 7.f : fmaf(-m, q.f, 7.f);
 #pragma unroll
-  for (int pg = 0; pg < kStagePages; ++pg) {
-    uint32_t a[4];
+  for (int pg = 0; pg < SP; ++pg) {
+    uint32_t hi[2], lo[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const float x = ex2(sc[2 * pg + j].x + base), y = ex2(sc[2 * pg + j].y + base);
-      l += x + y;
-      split2(x, y, a[2 * j], a[2 * j + 1]);
+      float2 e = __ffma2_rn(sc[2 * pg + j], make_float2(q.f, q.f), make_float2(base, base));
+      e.x = ex2(e.x);
+      e.y = ex2(e.y);
+      l = __fadd2_rn(l, e);
+      split2(e, hi[j], lo[j]);
     }
     const uint8_t* V = buf + pg * BLK + 8 * HD;
     const uint8_t* S = buf + pg * BLK + 17 * HD + (n / (8 / NG)) * 4;
@@ -252,38 +260,41 @@ __device__ __forceinline__ void stage_math(const uint8_t* __restrict__ buf, cons
       s9[j] = __hmul2(bits_h2(sb), __float2half2_rn(9.f));
       s8[j] = __hmul2(bits_h2(sb), __float2half2_rn(-0.125f));
     }
+    // A tile's rows g and g + 8 are dims 4k + i and 4k + i + 1 of this thread's sixteen (eight at hd 64).
 #pragma unroll
     for (int k = 0; k < NW; ++k) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t b[2];
+      for (int i = 0; i < 4; i += 2) {
+        uint32_t a[4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t x = w[j].w[k];
-          const uint32_t y = i == 0 ? x << 4 : i == 1 ? x : i == 2 ? x >> 4 : x >> 8;
-          b[j] = h2_bits(__hfma2(bits_h2(v_bits(y)), s8[j], s9[j]));
+          a[2 * j] = h2_bits(__hfma2(bits_h2(v_bits(i == 0 ? x << 4 : x >> 4)), s8[j], s9[j]));
+          a[2 * j + 1] = h2_bits(__hfma2(bits_h2(v_bits(i == 0 ? x : x >> 8)), s8[j], s9[j]));
         }
-        mma_f16(o[4 * k + i], a, b[0], b[1], o[4 * k + i]);
+        mma_f16(o[2 * k + i / 2], a, hi[0], hi[1], o[2 * k + i / 2]);
+        mma_f16(o[2 * k + i / 2], a, lo[0], lo[1], o[2 * k + i / 2]);
       }
     }
   }
 }
 
-// The stages (32 positions of one kv head) of all (lane, kv head) pairs laid end to end,
-// lane-major; CTA c takes [c Q, (c + 1) Q), so every SM reads the same number of bytes.
-// Run by one warp: C[b] = first stage of lane b, ctx[b] its clamped context; returns Q.
-__device__ __forceinline__ void stage_plan(const AttnQ4Params& p, long long* C, int* ctx, long long* plan) {
+// The stages of all (lane, kv head) pairs laid end to end, lane-major; warp w of the grid takes
+// [w Q, (w + 1) Q), so every warp reads the same number of bytes.  Run by one warp:
+// C[b] = first stage of lane b, ctx[b] its clamped context; plan = {stages, Q}.
+template <int HD>
+__device__ __forceinline__ void stage_plan(const AttnQ4Params& p, int* C, int* ctx, int* plan) {
   const int lane = threadIdx.x & 31;
-  const long long cap = (long long)p.max_pages * kQ4Page;
-  long long total = 0;
+  const int cap = p.max_pages * kQ4Page;
+  int total = 0;
   for (int b0 = 0; b0 < p.lanes; b0 += 32) {
     const int b = b0 + lane;
-    const int c = b < p.lanes ? (int)min((long long)max(p.ctx_lens[b], 0), cap) : 0;
-    const long long mine = (long long)p.num_kv_heads * ((c + (long long)kStagePos - 1) / kStagePos);
-    long long incl = mine;
+    const int c = b < p.lanes ? min(max(p.ctx_lens[b], 0), cap) : 0;
+    const int mine = p.num_kv_heads * ((c + kStagePos<HD> - 1) / kStagePos<HD>);
+    int incl = mine;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, incl, s);
+      const int u = __shfl_up_sync(0xffffffffu, incl, s);
       if (lane >= s) incl += u;
     }
     if (b < p.lanes) {
@@ -295,219 +306,278 @@ __device__ __forceinline__ void stage_plan(const AttnQ4Params& p, long long* C, 
   if (lane == 0) {
     C[p.lanes] = total;
     plan[0] = total;
-    plan[1] = max((long long)kWarps, (total + gridDim.x - 1) / gridDim.x);  // one stage per warp at least
+    plan[1] = max(1u, ((unsigned)total + gridDim.x * kWarps - 1) / (gridDim.x * kWarps));
   }
 }
 
-// A walk over the pairs of a CTA's share [g0, g1), and this warp's stages [wb, we) of each:
-// the pair's segment [sb, se) is cut evenly over the CTA's warps.
+// A walk over the pairs of a warp's share [g0, g1) and its segment [sb, se) of each.
+template <int HD>
 struct PairWalk {
-  int lid, kvh, ns, sb, se, wb, we;
-  long long P;  // the pair's first stage
-  __device__ __forceinline__ void set(const int* ctx, long long g0, long long g1, int warp) {
-    ns = (int)((ctx[lid] + (long long)kStagePos - 1) / kStagePos);
-    sb = (int)max(0ll, g0 - P);
-    se = (int)min((long long)ns, g1 - P);
-    const int n = se - sb;
-    wb = sb + (int)((long long)n * warp / kWarps);
-    we = sb + (int)((long long)n * (warp + 1) / kWarps);
+  int lid, kvh, ns, sb, se;
+  int P;  // the pair's first stage
+  __device__ __forceinline__ void set(const int* ctx, int g0, int g1) {
+    ns = (ctx[lid] + kStagePos<HD> - 1) / kStagePos<HD>;
+    sb = max(0, g0 - P);
+    se = min(ns, g1 - P);
+  }
+  // The pair that holds stage g0 < total.
+  __device__ __forceinline__ void seek(const int* C, const int* ctx, int lanes, int g0, int g1) {
+    int lo = 0, hi = lanes - 1;  // the last lane with C <= g0, which is never an empty one
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (C[mid] <= g0) lo = mid; else hi = mid - 1;
+    }
+    lid = lo;
+    ns = (ctx[lo] + kStagePos<HD> - 1) / kStagePos<HD>;
+    kvh = (unsigned)(g0 - C[lo]) / (unsigned)ns;
+    P = C[lo] + kvh * ns;
+    set(ctx, g0, g1);
   }
   // False when the share is at its end.
-  __device__ __forceinline__ bool next(const int* ctx, int lanes, int hkv, long long g0, long long g1, int warp) {
+  __device__ __forceinline__ bool next(const int* ctx, int lanes, int hkv, int g0, int g1) {
     P += ns;
+    if (P >= g1) return false;
     if (++kvh == hkv) {
       kvh = 0;
       do ++lid;
-      while (lid < lanes && ctx[lid] == 0);
+      while (ctx[lid] == 0);  // a stage before g1 is some lane's
     }
-    if (lid >= lanes || P >= g1) return false;
-    set(ctx, g0, g1, warp);
+    set(ctx, g0, g1);
     return true;
   }
 };
 
+// A warp's share is one run of stages: whole pairs, which it finishes by itself, and at most
+// two pieces of pairs: one that continues a pair begun before it (state A), then one that
+// begins a pair which goes on behind it (state B).  At the end of the CTA the pieces
+// merge in shared memory in stage order; what is cut at the CTA's own ends goes to the
+// combine kernel, at most two partial segments per CTA.  (Cutting each pair over a CTA's warps
+// instead costs a block-wide merge per pair: 67 against 41 us on the 64-lane 7B layer.)
 template <int HD>
 __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Params p) {
-  constexpr int BLK = 18 * HD;
-  constexpr int NST = kStages<HD>;
-  constexpr int ROW = HD + 4;  // floats per (warp, head) of the merge buffer
+  constexpr int BLK = 18 * HD, SP = kStagePages<HD>, SPOS = kStagePos<HD>;
+  constexpr int NST = kStages, IDS = 32 / SP;
+  constexpr uint32_t ALL = (1u << SP) - 1;
+  constexpr int ROW = HD + 4;  // floats per head of a state
+  constexpr int RING = NST * SP * BLK;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[kWarps][NST];
-  __shared__ float s_ml[kWarps][8][2];
-  __shared__ long long C[kMaxLanes + 1];
-  __shared__ long long plan[2];
+  __shared__ float s_ml[2][kWarps][8][2];
+  __shared__ int s_state[kWarps];  // 1: state A, 2: and it ends its pair, 4: state B
+  __shared__ int s_pair[2][kWarps];
+  __shared__ int C[kMaxLanes + 1];
+  __shared__ int plan[2];
   __shared__ int ctx[kMaxLanes];
   griddep_launch();
   griddep_wait();  // q, the pages, tables and lengths come from earlier kernels
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hkv = p.num_kv_heads, G = p.num_heads / hkv;
-  uint8_t* ring = smem + (size_t)warp * NST * kStagePages * BLK;
-  float* merge = reinterpret_cast<float*>(smem + (size_t)kWarps * NST * kStagePages * BLK);  // [warps][G][ROW]
-  if (warp == 0) stage_plan(p, C, ctx, plan);
-  if (lane == 0) {
-    for (int i = 0; i < NST; ++i) mbar_init(&full[warp][i], 1);
-    fence_mbar_init();
-  }
+  uint8_t* ring = smem + (size_t)warp * RING;
+  float* state_a = reinterpret_cast<float*>(smem + (size_t)kWarps * RING);  // [warps][G][ROW]
+  if (warp == 0) stage_plan<HD>(p, C, ctx, plan);
+  if (lane == 0) s_state[warp] = 0;
   __syncthreads();
-  const long long total = plan[0], Q = plan[1];
-  const long long g0 = min(total, blockIdx.x * Q), g1 = min(total, g0 + Q);
+  const int total = plan[0], Q = plan[1];
   // Lanes of context 0 get zeros.
   for (int b = blockIdx.x; b < p.lanes; b += gridDim.x)
     if (ctx[b] == 0)
       for (int i = threadIdx.x; i < p.num_heads * HD; i += kWarps * 32) p.out[(size_t)b * p.ldo + i] = 0.f;
-  if (threadIdx.x == 0) p.meta[2 * blockIdx.x] = -1;
-  if (g0 >= g1) return;
+  const int gw = blockIdx.x * kWarps + warp;
+  const int g0 = gw < (total + Q - 1) / Q ? gw * Q : total, g1 = min(total - g0, Q) + g0;
 
-  PairWalk use;
-  {
-    int lo = 0, hi = p.lanes - 1;  // the lane whose stages hold g0: the last with C <= g0 (never an empty one)
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (C[mid] <= g0) lo = mid; else hi = mid - 1;
-    }
-    use.lid = lo;
-    use.ns = (int)((ctx[lo] + (long long)kStagePos - 1) / kStagePos);
-    use.kvh = (int)((g0 - C[lo]) / use.ns);
-    use.P = C[lo] + (long long)use.kvh * use.ns;
-    use.set(ctx, g0, g1, warp);
-  }
-  PairWalk ld = use;
-  bool ld_more = true;
-  const uint64_t pol = l2_evict_first_policy();
-  // ---- loads: the warp's stages in order, NST of them ahead of the arithmetic ----
-  int ld_st = ld.wb, ld_at = 0;  // next stage; its place among the 16 stages whose page ids `ids` holds
-  int32_t ids = 0;
-  auto fetch_ids = [&]() {  // page ids of 16 stages, one per thread
-    const long long j = (long long)kStagePages * ld_st + lane;
-    ids = j * kQ4Page < ctx[ld.lid] ? p.tables[(size_t)ld.lid * p.max_pages + j] : -2;  // -2: past the context
-    ld_at = 0;
-  };
-  fetch_ids();
-  uint32_t issued = 0, loaded = 0;  // loaded: two bits per ring slot, the pages that are there
-  int slot_in = 0;
-  auto issue = [&]() {
-    while (ld_more && ld_st >= ld.we) {
-      ld_more = ld.next(ctx, p.lanes, hkv, g0, g1, warp);
-      if (!ld_more) break;
-      ld_st = ld.wb;
-      if (ld_st < ld.we) fetch_ids();
-    }
-    if (!ld_more) return;
-    if (ld_at == 16) fetch_ids();
-    const int page = __shfl_sync(0xffffffffu, ids, kStagePages * ld_at + (lane & 1));
-    const bool there = (unsigned)page < (unsigned)p.num_pages;
-    const uint32_t got = __ballot_sync(0xffffffffu, there) & 3u;
-    if (lane < 2 && !there && page != -2) atomicExch(p.bad, 1);
-    uint64_t* bar = &full[warp][slot_in];
-    if (lane == 0) mbar_arrive_expect_tx(bar, BLK * __popc(got));
-    __syncwarp();
-    if (lane < kStagePages && there)
-      bulk_load(ring + (slot_in * kStagePages + lane) * BLK,
-                p.pool + (size_t)page * p.page_bytes + ((size_t)p.layer * hkv + ld.kvh) * BLK, BLK, bar, pol);
-    loaded = (loaded & ~(3u << (2 * slot_in))) | got << (2 * slot_in);
-    slot_in = slot_in + 1 == NST ? 0 : slot_in + 1;
-    ++issued;
-    ++ld_st;
-    ++ld_at;
-  };
+  if (g0 < g1) {
+    PairWalk<HD> use;
+    use.seek(C, ctx, p.lanes, g0, g1);
+    PairWalk<HD> ld = use;
+    const uint64_t pol = l2_evict_first_policy();
+    // ---- loads: the warp's stages in order, two of them ahead of the arithmetic ----
+    int ld_st = ld.sb, ld_at = 0;  // next stage; its place among the stages whose page ids `ids` holds
+    int32_t ids = 0;
+    const uint8_t* src0 = nullptr;  // this thread's 16 bytes of the head's block in page 0
+    auto fetch_ids = [&]() {  // page ids of the next 32 pages, one per thread
+      const int j = SP * ld_st + lane;
+      ids = j * kQ4Page < ctx[ld.lid] ? p.tables[(size_t)ld.lid * p.max_pages + j] : -2;  // -2: past the context
+      ld_at = 0;
+    };
+    auto enter = [&]() {
+      ld_st = ld.sb;
+      src0 = p.pool + ((size_t)p.layer * hkv + ld.kvh) * BLK + 16 * lane;
+      fetch_ids();
+    };
+    enter();
+    const uint32_t ring_at = smem_u32(ring) + 16 * lane;
+    uint32_t loaded = 0;  // SP bits per ring slot: the pages that are there
+    int slot_in = 0;
+    bool ld_more = true;
+    auto issue = [&]() {
+      if (ld_more && ld_st >= ld.se) {
+        ld_more = ld.next(ctx, p.lanes, hkv, g0, g1);
+        if (ld_more) enter();
+      }
+      if (ld_more) {
+        if (ld_at == IDS) fetch_ids();
+        uint32_t got = 0;
+        const uint8_t* src[SP];
+        int page[SP];
+#pragma unroll
+        for (int i = 0; i < SP; ++i) {
+          page[i] = __shfl_sync(0xffffffffu, ids, SP * ld_at + i);
+          got |= (unsigned)page[i] < (unsigned)p.num_pages ? 1u << i : 0u;
+          src[i] = src0 + (size_t)page[i] * p.page_bytes - i * BLK;
+        }
+        const uint32_t dst = ring_at + slot_in * (SP * BLK);
+        // A stage's pages follow one another in the ring: 288 chunks of 16 bytes, nine per thread.
+#pragma unroll
+        for (int i = 0; i < SP * BLK / 512; ++i) {
+          const int lo = 512 * i / BLK, cut = ((lo + 1) * BLK - 512 * i) / 16;  // threads from `cut` on: the next page
+          const int pg = cut < 32 && lane >= cut ? lo + 1 : lo;
+          const uint8_t* s = pg == lo ? src[lo] : src[lo + 1 < SP ? lo + 1 : lo];
+          if (got == ALL || (got >> pg & 1)) cp_async16(dst + 512 * i, s + 512 * i, pol);
+        }
+        if (got != ALL && lane == 0) {
+          bool bad = false;
+#pragma unroll
+          for (int i = 0; i < SP; ++i) bad |= !(got >> i & 1) && page[i] != -2;
+          if (bad) atomicExch(p.bad, 1);
+        }
+        loaded = (loaded & ~(ALL << (SP * slot_in))) | got << (SP * slot_in);
+        ++ld_st;
+        ++ld_at;
+      }
+      cp_async_commit();
+      slot_in = slot_in + 1 == NST ? 0 : slot_in + 1;
+    };
 #pragma unroll 1
-  for (int i = 0; i < NST; ++i) issue();
+    for (int i = 0; i < NST - 1; ++i) issue();
 
-  uint32_t consumed = 0, phase = 0;
-  int slot = 0;
-  bool ok = true;
-  while (true) {
-    QFrag<HD> q;
-    load_q<HD>(p, use.lid, use.kvh, G, lane, q);
-    float m = -INFINITY, l = 0.f;
-    float o[HD / 8][4];
-#pragma unroll
-    for (int i = 0; i < HD / 8; ++i)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
-    for (int st = use.wb; st < use.we && ok; ++st) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][slot], phase, p.err));
-      if (!ok) break;
-      const int nvalid = (int)min((long long)kStagePos, ctx[use.lid] - (long long)kStagePos * st);
-      const uint32_t pages = (loaded >> (2 * slot)) & 3u;
-      const uint8_t* buf = ring + slot * kStagePages * BLK;
-      if (nvalid == kStagePos && pages == 3u)
-        stage_math<HD, false>(buf, q, m, l, o, nvalid, pages, lane);
-      else
-        stage_math<HD, true>(buf, q, m, l, o, nvalid, pages, lane);
-      ++consumed;
-      if (++slot == NST) {
-        slot = 0;
-        phase ^= 1;
-      }
-      __syncwarp();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // reads of this slot before the next copy into it
-      issue();
-    }
-    // ---- merge the warps' states, in warp order ----
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    int slot = 0;
+    bool more = true;
     const int h = lane >> 2, t = lane & 3;
-    if (h < G) {
-      if (t == 0) {
-        s_ml[warp][h][0] = m;
-        s_ml[warp][h][1] = l;
+    while (more) {
+      QFrag<HD> q;
+      load_q<HD>(p, use.lid, use.kvh, G, lane, q);
+      float m = -INFINITY;
+      float2 l2 = make_float2(0.f, 0.f);
+      float o[HD / 16][4];
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
+      for (int st = use.sb; st < use.se; ++st) {
+        cp_async_wait<NST - 2>();
+        __syncwarp();  // this stage is there for every thread, and nobody reads the slot before it any more
+        issue();
+        const int nvalid = min(SPOS, ctx[use.lid] - SPOS * st);
+        const uint32_t pages = (loaded >> (SP * slot)) & ALL;
+        const uint8_t* buf = ring + slot * (SP * BLK);
+        if (nvalid == SPOS && pages == ALL)
+          stage_math<HD, false>(buf, q, m, l2, o, nvalid, pages, lane);
+        else
+          stage_math<HD, true>(buf, q, m, l2, o, nvalid, pages, lane);
+        slot = slot + 1 == NST ? 0 : slot + 1;
       }
-      float* d = merge + ((size_t)warp * G + h) * ROW + (HD / 4) * t;
+      float l = l2.x + l2.y;
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      const bool begins = use.sb == 0, ends = use.se == use.ns;
+      const int which = begins ? 1 : 0;
+      const int pair = use.lid * hkv + use.kvh;
+      // A whole pair goes out; a piece to its state (B only at the share's end, over the idle ring).
+      float* d = begins && ends ? p.out + (size_t)use.lid * p.ldo + (size_t)use.kvh * G * HD
+                 : begins       ? reinterpret_cast<float*>(ring)
+                                : state_a + (size_t)warp * G * ROW;
+      const int row = begins && ends ? HD : ROW;
+      const float r = begins && ends ? (l == 0.f ? 0.f : 8.f / l) : 1.f;
+      __syncwarp();  // the last stage is read
+      // This thread holds dims h hd/8 .. + hd/8 - 1 of heads 2t and 2t + 1.
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < 2; ++c) {
+        const float rc = __shfl_sync(0xffffffffu, r, 8 * t + 4 * c);
+        if (2 * t + c < G) {
+          float* dc = d + (2 * t + c) * row + (HD / 8) * h;
 #pragma unroll
-        for (int k = 0; k < HD / 32; ++k)
-          *reinterpret_cast<float4*>(d + (HD / 8) * c + 4 * k) =
-              make_float4(o[4 * k][c] + o[4 * k][c + 2], o[4 * k + 1][c] + o[4 * k + 1][c + 2],
-                          o[4 * k + 2][c] + o[4 * k + 2][c + 2], o[4 * k + 3][c] + o[4 * k + 3][c + 2]);
+          for (int k = 0; k < HD / 32; ++k)
+            *reinterpret_cast<float4*>(dc + 4 * k) = make_float4(o[2 * k][c] * rc, o[2 * k][c + 2] * rc,
+                                                                 o[2 * k + 1][c] * rc, o[2 * k + 1][c + 2] * rc);
+        }
+      }
+      if (h < G && t == 0 && !(begins && ends)) {
+        s_ml[which][warp][h][0] = m * q.f;
+        s_ml[which][warp][h][1] = l;
+      }
+      if (lane == 0 && !(begins && ends)) {
+        s_state[warp] |= begins ? 4 : ends ? 3 : 1;
+        s_pair[which][warp] = pair;
+      }
+      more = use.next(ctx, p.lanes, hkv, g0, g1);
     }
-    __syncthreads();
-    const bool whole = use.sb == 0 && use.se == use.ns;
-    const size_t part = 2 * (size_t)blockIdx.x + (use.sb == 0 ? 1 : 0);
-    for (int e = threadIdx.x; e < G * (HD / 4); e += kWarps * 32) {
-      const int g = e / (HD / 4), d4 = e % (HD / 4);
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_ml[w][g][0]);
-      float L = 0.f;
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float mw = s_ml[w][g][0];
-        const float x = mw == -INFINITY ? 0.f : ex2(mw - M);
-        L = fmaf(s_ml[w][g][1], x, L);
-        const float4 v = *reinterpret_cast<const float4*>(merge + ((size_t)w * G + g) * ROW + 4 * d4);
-        a.x = fmaf(v.x, x, a.x);
-        a.y = fmaf(v.y, x, a.y);
-        a.z = fmaf(v.z, x, a.z);
-        a.w = fmaf(v.w, x, a.w);
-      }
+  }
+  __syncthreads();
+
+  // ---- pieces, in stage order: A of warp 0, B of warp 0, A of warp 1, ... ----
+  int open_pair = -1;  // a pair begun in this CTA that goes on in the next
+  if (threadIdx.x < G * (HD / 4)) {
+    const int g = threadIdx.x / (HD / 4), d = 4 * (threadIdx.x % (HD / 4));
+    float M = -INFINITY, L = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    int pair = -1;
+    bool begun = false, any = false;
+    auto add = [&](float4 v, float m, float l) {
+      const float Mn = fmaxf(M, m);
+      const float x = M == -INFINITY ? 0.f : ex2(M - Mn), y = m == -INFINITY ? 0.f : ex2(m - Mn);
+      M = Mn;
+      L = L * x + l * y;
+      a.x = a.x * x + v.x * y;
+      a.y = a.y * x + v.y * y;
+      a.z = a.z * x + v.z * y;
+      a.w = a.w * x + v.w * y;
+      any = true;
+    };
+    auto flush = [&](bool whole) {
       if (whole) {
         const float r = L == 0.f ? 0.f : 8.f / L;
-        *reinterpret_cast<float4*>(p.out + (size_t)use.lid * p.ldo + (size_t)(use.kvh * G + g) * HD + 4 * d4) =
+        *reinterpret_cast<float4*>(p.out + (size_t)(pair / hkv) * p.ldo + (size_t)((pair % hkv) * G + g) * HD + d) =
             make_float4(a.x * r, a.y * r, a.z * r, a.w * r);
       } else {
-        *reinterpret_cast<float4*>(p.part_o + (part * G + g) * HD + 4 * d4) = a;
-        if (d4 == 0) {
+        const size_t part = 2 * (size_t)blockIdx.x + (begun ? 1 : 0);
+        *reinterpret_cast<float4*>(p.part_o + (part * G + g) * HD + d) = a;
+        if (d == 0) {
           p.part_ml[(part * G + g) * 2] = M;
           p.part_ml[(part * G + g) * 2 + 1] = L;
         }
       }
+      M = -INFINITY;
+      L = 0.f;
+      a = make_float4(0.f, 0.f, 0.f, 0.f);
+      begun = any = false;
+    };
+#pragma unroll 4
+    for (int w = 0; w < kWarps; ++w) {
+      const int st = s_state[w];
+      const float4 va = *reinterpret_cast<const float4*>(state_a + ((size_t)w * G + g) * ROW + d);
+      const float4 vb = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + (size_t)w * RING) + g * ROW + d);
+      const float2 ma = *reinterpret_cast<const float2*>(s_ml[0][w][g]), mb = *reinterpret_cast<const float2*>(s_ml[1][w][g]);
+      if (st & 1) {
+        pair = s_pair[0][w];
+        add(va, ma.x, ma.y);
+        if (st & 2) flush(begun);
+      }
+      if (st & 4) {
+        pair = s_pair[1][w];
+        begun = true;
+        add(vb, mb.x, mb.y);
+      }
     }
-    if (threadIdx.x == 0 && use.sb == 0 && use.se < use.ns) {
-      p.meta[2 * blockIdx.x] = use.lid * hkv + use.kvh;
-      p.meta[2 * blockIdx.x + 1] = (int)((use.P + use.ns - 1) / Q - use.P / Q + 1);
+    if (any) {
+      if (begun) open_pair = pair;
+      flush(false);
     }
-    if (!use.next(ctx, p.lanes, hkv, g0, g1, warp)) break;
-    __syncthreads();  // the merge buffer is free again
   }
-  // Leave no copy in flight (a wait that gave up leaves some outstanding).
-  for (uint32_t i = consumed; i < issued; ++i) {
-    mbar_wait(&full[warp][slot], phase, p.err);
-    if (++slot == NST) {
-      slot = 0;
-      phase ^= 1;
+  if (threadIdx.x == 0) {
+    p.meta[2 * blockIdx.x] = open_pair;
+    if (open_pair >= 0) {
+      const int b = open_pair / hkv;
+      const int ns = (ctx[b] + SPOS - 1) / SPOS, P = C[b] + (open_pair % hkv) * ns;
+      p.meta[2 * blockIdx.x + 1] = (P + ns - 1) / (Q * kWarps) - P / (Q * kWarps) + 1;
     }
   }
 }
@@ -565,16 +635,6 @@ __global__ void __launch_bounds__(1024) attn_q4_combine_kernel(const AttnQ4Param
 
 }  // namespace
 
-int attn_q4_device_error(int clear) {
-  int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_attn_q4_error, sizeof(int)) != cudaSuccess) return -1;
-  if (clear && v) {
-    int z = 0;
-    cudaMemcpyToSymbol(g_attn_q4_error, &z, sizeof(int));
-  }
-  return v;
-}
-
 // Two partial segments per CTA (one that begins a pair, one that continues it), and the
 // descriptors of cut pairs.
 size_t attention_q4_workspace_floats(size_t num_heads, size_t num_kv_heads, size_t head_dim) {
@@ -591,7 +651,9 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
   int rc = q4_check_pool("paged_attention_q4", pool, num_pages, num_layers, layer, num_heads, num_kv_heads, head_dim);
   if (rc) return rc;
   GLC_REQUIRE(lanes > 0 && lanes <= (size_t)kMaxLanes, "paged_attention_q4: %zu lanes (1 to %d)", lanes, kMaxLanes);
-  GLC_REQUIRE(max_pages > 0 && max_pages <= ((size_t)1 << 26), "paged_attention_q4: %zu pages per lane", max_pages);
+  GLC_REQUIRE(max_pages > 0 && max_pages <= ((size_t)1 << 26) &&
+                  lanes * num_kv_heads * max_pages < ((size_t)1 << 31),
+              "paged_attention_q4: %zu pages per lane (at most 2^26, and 2^31 with lanes * kv heads)", max_pages);
   GLC_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)workspace % 16 == 0 && ldq % 4 == 0 &&
                   ldo % 4 == 0,
               "paged_attention_q4: q, out and workspace must be 16-byte aligned");
@@ -619,11 +681,10 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
   p.num_kv_heads = (int)num_kv_heads;
   p.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   p.bad = ops_error_word();
-  p.err = device_symbol_address(g_attn_q4_error);
-  GLC_REQUIRE(p.bad && p.err, "paged_attention_q4: device status word unavailable");
+  GLC_REQUIRE(p.bad, "paged_attention_q4: device status word unavailable");
   auto kern = head_dim == 128 ? attn_q4_kernel<128> : attn_q4_kernel<64>;
-  const size_t stages = head_dim == 128 ? kStages<128> : kStages<64>;
-  const size_t smem = kWarps * (stages * kStagePages * q4_block_bytes(head_dim) + G * (head_dim + 4) * sizeof(float));
+  const size_t pages = head_dim == 128 ? kStagePages<128> : kStagePages<64>;
+  const size_t smem = kWarps * (kStages * pages * q4_block_bytes(head_dim) + G * (head_dim + 4) * sizeof(float));
   if ((rc = allow_dynamic_smem((const void*)kern, (int)smem))) return rc;
   if ((rc = launch_pdl(kern, dim3((unsigned)grid), dim3(kWarps * 32), smem, stream, 1, p))) return rc;
   return launch_pdl(attn_q4_combine_kernel, dim3((unsigned)grid), dim3(1024), 0, stream, 1, p, (int)head_dim);
