@@ -6,28 +6,36 @@
 // holds 18 hd / 16 bytes (144 at hd 128, against 1024 in the float32 pages), and the
 // G <= 8 query heads of a group need 4 G hd products on them: on the fp32 pipe that
 // is more time than the bytes take, so both products run as mma.sync m16n8k16
-// (fp16 in, fp32 sums).  M is the query heads, and eight of them would leave half of the
-// sixteen rows idle: X  (A
-// tcgen05.mma needs 64 or 128 rows and its operands in shared memory as fp16: the codes
-// would be unpacked, written and read once more, which is what bounds this kernel.)
-//   * K: a code c is used as the fp16 number whose bits are the code: c * 2^-24, or c * 2^-20
-//     one nibble higher (q's dims there carry 2^-4).  One shift and four ANDs make four
-//     operand registers of eight codes.  The zero point is the accumulator's initial value, -7 sum q
-//     of the group, and the group's scale multiplies the fp32 result.
-//   * V: the scale belongs to the summed index, so it has to be in the operand: s (c - 7) / 8 =
-//     (72 - h) s / 8 for the fp16 number h = 64 + (15 - c), whose bits one LOP3 makes.
-//     9 s and the result are fp16 numbers (scales have 7 significant bits), so the half FMA is exact.
+// (fp16 in, fp32 sums).  q and the softmax weights go in as a high and a low fp16 part, 22
+// bits together; the held values are exact.  (A tcgen05.mma needs 64 or 128 rows and its
+// operands in shared memory as fp16: the codes would be unpacked, written and read once more.)
+//   * q K^T: M is the query heads, and eight of them would leave half of the sixteen rows
+//     idle: rows 0-7 hold q's high and rows 8-15 its low parts.  A code c is used as the fp16
+//     number whose bits are the code, c * 2^-24, or c * 2^-20 one nibble higher (q's dims there
+//     carry 2^-4): one shift and four ANDs make four operand registers of eight codes.  The zero
+//     point is the accumulator's initial value, -7 sum q of the group, and the group's scale
+//     multiplies the fp32 result.
+//   * (P V)^T = V^T P^T: M is sixteen dims, N the heads, so that no accumulator is idle, and the
+//     score accumulators are the weights' operand as they stand.  The scale belongs to the summed
+//     index, so it has to be in the operand: (c - 7) s / 8 = (72 - h) s / 8 for the fp16 number
+//     h = 64 + (15 - c), whose bits one LOP3 makes from a code at bits 4-7.  9 s and the result
+//     are fp16 numbers (scales have 7 significant bits), so one half FMA is exact.
 // The cache's orders put every operand register's codes in one word of one thread: K's words
 // (t, g) and V's 16-bit units by position pair are the fragments of these instructions.
 #include "kv_q4.cuh"
 
 namespace glacier {
 
+__device__ int g_attn_q4_error;
+
 namespace {
 
 constexpr int kMaxLanes = 1024;
-constexpr int kWarps = 12;
-constexpr int kStages = 3;  // stages in a warp's ring: 166 KB of K/V in flight per SM
+constexpr int kWarps = 8;                     // warps that compute, two per SM partition
+constexpr int kThreads = 32 * (kWarps + 4);   // and a warpgroup whose first warp loads
+// Registers: 384 x 168 at launch = 256 x 232 + 128 x 40 after the split.
+constexpr int kRegsMath = 232, kRegsLoad = 40;
+constexpr int kStages = 5;  // stages in a warp's ring: 184 KB of K/V in flight per SM
 // Pages per stage: 4608 bytes at either head size.
 template <int HD>
 constexpr int kStagePages = HD == 128 ? 2 : 4;
@@ -49,6 +57,7 @@ struct AttnQ4Params {
   int lanes, max_pages, num_pages, layer, num_heads, num_kv_heads;
   float scale_log2;
   int* bad;
+  int* err;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -83,14 +92,12 @@ __device__ __forceinline__ uint32_t v_bits(uint32_t x) {
   return d;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint64_t policy) {
-  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
 }
 
 template <int N>
@@ -119,22 +126,26 @@ struct QFrag {
   float f;                // raw score -> base-2 score
 };
 
+// This thread's dims of head lane / 4: 8 t .. 8 t + 7 of every group (zeros past the last head).
 template <int HD>
-__device__ __forceinline__ void load_q(const AttnQ4Params& p, int lid, int kvh, int G, int lane, QFrag<HD>& q) {
-  constexpr int NG = HD / 32;
+__device__ __forceinline__ void load_q(const AttnQ4Params& p, int lid, int kvh, int G, int lane,
+                                       float (&v)[HD / 32][8]) {
   const int h = lane >> 2, t = lane & 3;
-  float v[NG][8];
-  float top = 0.f;
-  if (h < G) {
-    const float* src = p.q + (size_t)lid * p.ldq + (size_t)(kvh * G + h) * HD + 8 * t;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) load8(src + 32 * g, v[g]);
-  } else {
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
+  for (int g = 0; g < HD / 32; ++g) {
+    if (h < G) {
+      load8(p.q + (size_t)lid * p.ldq + (size_t)(kvh * G + h) * HD + 8 * t + 32 * g, v[g]);
+    } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[g][i] = 0.f;
+    }
   }
+}
+
+template <int HD>
+__device__ __forceinline__ void split_q(const AttnQ4Params& p, const float (&v)[HD / 32][8], QFrag<HD>& q) {
+  constexpr int NG = HD / 32;
+  float top = 0.f;
 #pragma unroll
   for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -147,7 +158,7 @@ __device__ __forceinline__ void load_q(const AttnQ4Params& p, int lid, int kvh, 
   q.f = __uint_as_float((uint32_t)(127 + e) << 23) * 0x1p24f * p.scale_log2;
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    float sh = 0.f, sl = 0.f;
+    float sum = 0.f;
     // The word's nibbles pair dims (i, i + 4); pairs 1 and 3 are used 2^4 higher.
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -156,17 +167,13 @@ __device__ __forceinline__ void load_q(const AttnQ4Params& p, int lid, int kvh, 
       split2(make_float2(v[g][i] * m, v[g][i + 4] * m), hi, lo);
       q.a[2 * g + (i >> 1)][(i & 1) * 2] = hi;
       q.a[2 * g + (i >> 1)][(i & 1) * 2 + 1] = lo;
-      const float w = (i & 1) ? 16.f : 1.f;
-      const float2 fh = __half22float2(bits_h2(hi)), fl = __half22float2(bits_h2(lo));
-      sh += w * (fh.x + fh.y);
-      sl += w * (fl.x + fl.y);
+      const float2 f = __fadd2_rn(__half22float2(bits_h2(hi)), __half22float2(bits_h2(lo)));
+      sum = fmaf((i & 1) ? 16.f : 1.f, f.x + f.y, sum);
     }
-    sh += __shfl_xor_sync(0xffffffffu, sh, 1);
-    sl += __shfl_xor_sync(0xffffffffu, sl, 1);
-    sh += __shfl_xor_sync(0xffffffffu, sh, 2);
-    sl += __shfl_xor_sync(0xffffffffu, sl, 2);
-    q.c[g][0] = q.c[g][1] = -7.f * 0x1p-24f * sh;
-    q.c[g][2] = q.c[g][3] = -7.f * 0x1p-24f * sl;
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    q.c[g][0] = q.c[g][1] = -7.f * 0x1p-24f * sum;
+    q.c[g][2] = q.c[g][3] = 0.f;  // the low rows' sum is in the high rows'
   }
 }
 
@@ -269,7 +276,7 @@ __device__ __forceinline__ void stage_math(const uint8_t* __restrict__ buf, cons
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t x = w[j].w[k];
-          a[2 * j] = h2_bits(__hfma2(bits_h2(v_bits(i == 0 ? x << 4 : x >> 4)), s8[j], s9[j]));
+          a[2 * j] = h2_bits(__hfma2(bits_h2(v_bits(i == 0 ? x * 16u : x >> 4)), s8[j], s9[j]));
           a[2 * j + 1] = h2_bits(__hfma2(bits_h2(v_bits(i == 0 ? x : x >> 8)), s8[j], s9[j]));
         }
         mma_f16(o[2 * k + i / 2], a, hi[0], hi[1], o[2 * k + i / 2]);
@@ -279,62 +286,21 @@ __device__ __forceinline__ void stage_math(const uint8_t* __restrict__ buf, cons
   }
 }
 
-// The stages of all (lane, kv head) pairs laid end to end, lane-major; warp w of the grid takes
-// [w Q, (w + 1) Q), so every warp reads the same number of bytes.  Run by one warp:
-// C[b] = first stage of lane b, ctx[b] its clamped context; plan = {stages, Q}.
-template <int HD>
-__device__ __forceinline__ void stage_plan(const AttnQ4Params& p, int* C, int* ctx, int* plan) {
-  const int lane = threadIdx.x & 31;
-  const int cap = p.max_pages * kQ4Page;
-  int total = 0;
-  for (int b0 = 0; b0 < p.lanes; b0 += 32) {
-    const int b = b0 + lane;
-    const int c = b < p.lanes ? min(max(p.ctx_lens[b], 0), cap) : 0;
-    const int mine = p.num_kv_heads * ((c + kStagePos<HD> - 1) / kStagePos<HD>);
-    int incl = mine;
-#pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, incl, s);
-      if (lane >= s) incl += u;
-    }
-    if (b < p.lanes) {
-      C[b] = total + incl - mine;
-      ctx[b] = c;
-    }
-    total += __shfl_sync(0xffffffffu, incl, 31);
-  }
-  if (lane == 0) {
-    C[p.lanes] = total;
-    plan[0] = total;
-    plan[1] = max(1u, ((unsigned)total + gridDim.x * kWarps - 1) / (gridDim.x * kWarps));
-  }
-}
-
-// A walk over the pairs of a warp's share [g0, g1) and its segment [sb, se) of each.
+// A walk over the pairs of a warp's share [g0, g1) and its segment [sb, se) of each.  The
+// stages of all (lane, kv head) pairs are laid end to end, lane-major, and warp w of the
+// grid takes [w Q, (w + 1) Q): every warp reads the same number of bytes.
 template <int HD>
 struct PairWalk {
   int lid, kvh, ns, sb, se;
   int P;  // the pair's first stage
+  __device__ __forceinline__ static int stages(int ctx) { return (ctx + kStagePos<HD> - 1) / kStagePos<HD>; }
   __device__ __forceinline__ void set(const int* ctx, int g0, int g1) {
-    ns = (ctx[lid] + kStagePos<HD> - 1) / kStagePos<HD>;
+    ns = stages(ctx[lid]);
     sb = max(0, g0 - P);
     se = min(ns, g1 - P);
   }
-  // The pair that holds stage g0 < total.
-  __device__ __forceinline__ void seek(const int* C, const int* ctx, int lanes, int g0, int g1) {
-    int lo = 0, hi = lanes - 1;  // the last lane with C <= g0, which is never an empty one
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (C[mid] <= g0) lo = mid; else hi = mid - 1;
-    }
-    lid = lo;
-    ns = (ctx[lo] + kStagePos<HD> - 1) / kStagePos<HD>;
-    kvh = (unsigned)(g0 - C[lo]) / (unsigned)ns;
-    P = C[lo] + kvh * ns;
-    set(ctx, g0, g1);
-  }
   // False when the share is at its end.
-  __device__ __forceinline__ bool next(const int* ctx, int lanes, int hkv, int g0, int g1) {
+  __device__ __forceinline__ bool next(const int* ctx, int hkv, int g0, int g1) {
     P += ns;
     if (P >= g1) return false;
     if (++kvh == hkv) {
@@ -347,114 +313,199 @@ struct PairWalk {
   }
 };
 
+// Shares of the warps, found by every warp for itself: the sum of all stages, then the lane that
+// holds the share's first one.  ctx: clamped contexts, for the block.  Returns Q; start.lid = -1 when
+// the share is empty.  A chunk of 128 lanes is four consecutive ones per thread; the first chunk
+// stays in registers.
+template <int HD>
+__device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ctx, PairWalk<HD>& start, int& g0,
+                                          int& g1) {
+  const int lane = threadIdx.x & 31;
+  const int cap = p.max_pages * kQ4Page;
+  int ns[4], incl = 0;
+  auto chunk = [&](int b0) {  // stages of lanes b0 + 4 lane ..; incl: running sum over the threads
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int b = b0 + 4 * lane + i;
+      const int c = b < p.lanes ? min(max(p.ctx_lens[b], 0), cap) : 0;
+      if (b < p.lanes) ctx[b] = c;  // every warp writes the same values
+      ns[i] = PairWalk<HD>::stages(c);
+    }
+    incl = ns[0] + ns[1] + ns[2] + ns[3];
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, s);
+      if (lane >= s) incl += u;
+    }
+  };
+  int total = 0;
+  for (int b0 = (p.lanes - 1) / 128 * 128; b0 >= 0; b0 -= 128) {
+    chunk(b0);
+    total += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  total *= p.num_kv_heads;
+  const int warps = gridDim.x * kWarps;
+  const int Q = max(1, (int)(((unsigned)total + warps - 1) / (unsigned)warps));
+  start.lid = -1;
+  g0 = g1 = 0;
+  if ((long long)gw * Q >= total) return Q;
+  g0 = gw * Q;
+  g1 = min(total - g0, Q) + g0;
+  const int at = (unsigned)g0 / (unsigned)p.num_kv_heads;  // lane b holds g0 when its sums straddle `at`
+  int before = 0;
+  for (int b0 = 0;; b0 += 128) {
+    const uint32_t hit = __ballot_sync(0xffffffffu, before + incl > at);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      int first = before + incl - (ns[0] + ns[1] + ns[2] + ns[3]), i = 0, n = ns[0];
+#pragma unroll
+      for (int k = 1; k < 4; ++k)
+        if (i == k - 1 && first + n <= at) {
+          first += n;
+          i = k;
+          n = ns[k];
+        }
+      first = __shfl_sync(0xffffffffu, first, src) * p.num_kv_heads;
+      start.lid = b0 + 4 * src + __shfl_sync(0xffffffffu, i, src);
+      start.ns = __shfl_sync(0xffffffffu, n, src);
+      start.kvh = (unsigned)(g0 - first) / (unsigned)start.ns;
+      start.P = first + start.kvh * start.ns;
+      start.sb = g0 - start.P;
+      start.se = min(start.ns, g1 - start.P);
+      return Q;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+    chunk(b0 + 128);
+  }
+}
+
 // A warp's share is one run of stages: whole pairs, which it finishes by itself, and at most
 // two pieces of pairs: one that continues a pair begun before it (state A), then one that
 // begins a pair which goes on behind it (state B).  At the end of the CTA the pieces
 // merge in shared memory in stage order; what is cut at the CTA's own ends goes to the
-// combine kernel, at most two partial segments per CTA.  (Cutting each pair over a CTA's warps
-// instead costs a block-wide merge per pair: 67 against 41 us on the 64-lane 7B layer.)
+// combine kernel, at most two partial segments per CTA.
+// The last warp loads: its thread w keeps the ring of warp w filled by bulk copies, one per
+// page, so the arithmetic warps spend no instruction on page tables and addresses.
 template <int HD>
-__global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Params p) {
+__global__ void __launch_bounds__(kThreads, 1) attn_q4_kernel(const AttnQ4Params p) {
   constexpr int BLK = 18 * HD, SP = kStagePages<HD>, SPOS = kStagePos<HD>;
-  constexpr int NST = kStages, IDS = 32 / SP;
+  constexpr int NST = kStages;
   constexpr uint32_t ALL = (1u << SP) - 1;
   constexpr int ROW = HD + 4;  // floats per head of a state
   constexpr int RING = NST * SP * BLK;
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[kWarps][NST], empty[kWarps][NST];
+  __shared__ uint32_t s_got[kWarps][NST];  // the pages of a stage that are there
   __shared__ float s_ml[2][kWarps][8][2];
   __shared__ int s_state[kWarps];  // 1: state A, 2: and it ends its pair, 4: state B
-  __shared__ int s_pair[2][kWarps];
-  __shared__ int C[kMaxLanes + 1];
-  __shared__ int plan[2];
+  __shared__ int s_pair[2][kWarps], s_first[kWarps];  // of the states; the first stage of a B's pair
+  __shared__ PairWalk<HD> s_start[kWarps];
+  __shared__ int s_g[kWarps][2];
   __shared__ int ctx[kMaxLanes];
-  griddep_launch();
-  griddep_wait();  // q, the pages, tables and lengths come from earlier kernels
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hkv = p.num_kv_heads, G = p.num_heads / hkv;
+  if (warp < kWarps && lane == 0) {
+    for (int i = 0; i < NST; ++i) {
+      mbar_init(&full[warp][i], 1);
+      mbar_init(&empty[warp][i], 1);
+    }
+    fence_mbar_init();
+    s_state[warp] = 0;
+  }
+  griddep_launch();
+  griddep_wait();  // q, the pages, tables and lengths come from earlier kernels
   uint8_t* ring = smem + (size_t)warp * RING;
   float* state_a = reinterpret_cast<float*>(smem + (size_t)kWarps * RING);  // [warps][G][ROW]
-  if (warp == 0) stage_plan<HD>(p, C, ctx, plan);
-  if (lane == 0) s_state[warp] = 0;
+  PairWalk<HD> use;
+  int g0 = 0, g1 = 0, Q = 1;
+  float v[HD / 32][8];
+  if (warp < kWarps) {
+    Q = find_share<HD>(p, blockIdx.x * kWarps + warp, ctx, use, g0, g1);
+    if (use.lid >= 0) load_q<HD>(p, use.lid, use.kvh, G, lane, v);
+    if (lane == 0) {
+      s_start[warp] = use;
+      s_g[warp][0] = g0;
+      s_g[warp][1] = g1;
+    }
+  }
   __syncthreads();
-  const int total = plan[0], Q = plan[1];
-  // Lanes of context 0 get zeros.
-  for (int b = blockIdx.x; b < p.lanes; b += gridDim.x)
-    if (ctx[b] == 0)
-      for (int i = threadIdx.x; i < p.num_heads * HD; i += kWarps * 32) p.out[(size_t)b * p.ldo + i] = 0.f;
-  const int gw = blockIdx.x * kWarps + warp;
-  const int g0 = gw < (total + Q - 1) / Q ? gw * Q : total, g1 = min(total - g0, Q) + g0;
 
-  if (g0 < g1) {
-    PairWalk<HD> use;
-    use.seek(C, ctx, p.lanes, g0, g1);
-    PairWalk<HD> ld = use;
+  if (warp >= kWarps) {
+    // ---- loads ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
+    if (warp > kWarps) return;
+    bool more = lane < kWarps && s_start[lane < kWarps ? lane : 0].lid >= 0;
+    const int w = lane < kWarps ? lane : 0;
+    PairWalk<HD> ld = s_start[w];
+    const int a0 = s_g[w][0], a1 = s_g[w][1];
     const uint64_t pol = l2_evict_first_policy();
-    // ---- loads: the warp's stages in order, two of them ahead of the arithmetic ----
-    int ld_st = ld.sb, ld_at = 0;  // next stage; its place among the stages whose page ids `ids` holds
-    int32_t ids = 0;
-    const uint8_t* src0 = nullptr;  // this thread's 16 bytes of the head's block in page 0
-    auto fetch_ids = [&]() {  // page ids of the next 32 pages, one per thread
-      const int j = SP * ld_st + lane;
-      ids = j * kQ4Page < ctx[ld.lid] ? p.tables[(size_t)ld.lid * p.max_pages + j] : -2;  // -2: past the context
-      ld_at = 0;
-    };
-    auto enter = [&]() {
-      ld_st = ld.sb;
-      src0 = p.pool + ((size_t)p.layer * hkv + ld.kvh) * BLK + 16 * lane;
-      fetch_ids();
-    };
-    enter();
-    const uint32_t ring_at = smem_u32(ring) + 16 * lane;
-    uint32_t loaded = 0;  // SP bits per ring slot: the pages that are there
-    int slot_in = 0;
-    bool ld_more = true;
-    auto issue = [&]() {
-      if (ld_more && ld_st >= ld.se) {
-        ld_more = ld.next(ctx, p.lanes, hkv, g0, g1);
-        if (ld_more) enter();
+    int st = ld.sb, slot = 0;
+    uint32_t phase = 1;  // the first pass over the ring finds every slot free
+    int32_t ids[SP];
+    auto fetch = [&]() {  // page ids of stage st; -2: past the context
+#pragma unroll
+      for (int i = 0; i < SP; ++i) {
+        const int j = SP * st + i;
+        ids[i] = j * kQ4Page < ctx[ld.lid] ? p.tables[(size_t)ld.lid * p.max_pages + j] : -2;
       }
-      if (ld_more) {
-        if (ld_at == IDS) fetch_ids();
+    };
+    if (more) fetch();
+    long long idle_since = 0;
+    while (__any_sync(0xffffffffu, more)) {
+      const bool go = more && mbar_test_wait(&empty[w][slot], phase);
+      if (go) {
         uint32_t got = 0;
-        const uint8_t* src[SP];
-        int page[SP];
 #pragma unroll
-        for (int i = 0; i < SP; ++i) {
-          page[i] = __shfl_sync(0xffffffffu, ids, SP * ld_at + i);
-          got |= (unsigned)page[i] < (unsigned)p.num_pages ? 1u << i : 0u;
-          src[i] = src0 + (size_t)page[i] * p.page_bytes - i * BLK;
-        }
-        const uint32_t dst = ring_at + slot_in * (SP * BLK);
-        // A stage's pages follow one another in the ring: 288 chunks of 16 bytes, nine per thread.
-#pragma unroll
-        for (int i = 0; i < SP * BLK / 512; ++i) {
-          const int lo = 512 * i / BLK, cut = ((lo + 1) * BLK - 512 * i) / 16;  // threads from `cut` on: the next page
-          const int pg = cut < 32 && lane >= cut ? lo + 1 : lo;
-          const uint8_t* s = pg == lo ? src[lo] : src[lo + 1 < SP ? lo + 1 : lo];
-          if (got == ALL || (got >> pg & 1)) cp_async16(dst + 512 * i, s + 512 * i, pol);
-        }
-        if (got != ALL && lane == 0) {
+        for (int i = 0; i < SP; ++i) got |= (unsigned)ids[i] < (unsigned)p.num_pages ? 1u << i : 0u;
+        if (got != ALL) {
           bool bad = false;
 #pragma unroll
-          for (int i = 0; i < SP; ++i) bad |= !(got >> i & 1) && page[i] != -2;
+          for (int i = 0; i < SP; ++i) bad |= !(got >> i & 1) && ids[i] != -2;
           if (bad) atomicExch(p.bad, 1);
         }
-        loaded = (loaded & ~(ALL << (SP * slot_in))) | got << (SP * slot_in);
-        ++ld_st;
-        ++ld_at;
+        s_got[w][slot] = got;
+        mbar_arrive_expect_tx(&full[w][slot], BLK * __popc(got));
+        const uint8_t* src = p.pool + ((size_t)p.layer * hkv + ld.kvh) * BLK;
+        uint8_t* dst = smem + (size_t)w * RING + slot * (SP * BLK);
+#pragma unroll
+        for (int i = 0; i < SP; ++i)
+          if (got >> i & 1) bulk_load(dst + i * BLK, src + (size_t)ids[i] * p.page_bytes, BLK, &full[w][slot], pol);
+        if (++slot == NST) {
+          slot = 0;
+          phase ^= 1;
+        }
+        if (++st >= ld.se) {
+          more = ld.next(ctx, hkv, a0, a1);
+          st = ld.sb;
+        }
+        if (more) fetch();
       }
-      cp_async_commit();
-      slot_in = slot_in + 1 == NST ? 0 : slot_in + 1;
-    };
-#pragma unroll 1
-    for (int i = 0; i < NST - 1; ++i) issue();
-
+      if (__any_sync(0xffffffffu, go)) {
+        idle_since = 0;
+      } else {
+        // Every wait is bounded: about two seconds without a free slot, and the loader gives up.
+        const long long now = clock64();
+        if (idle_since == 0) idle_since = now;
+        if (now - idle_since > kSpinLimitCycles) {
+          if (lane == 0) atomicExch(p.err, kErrTimeout);
+          break;
+        }
+        __nanosleep(40);
+      }
+    }
+    return;
+  }
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMath));
+  auto math_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); };
+  if (use.lid >= 0) {
+    // ---- arithmetic ----
     int slot = 0;
-    bool more = true;
+    uint32_t phase = 0;
+    bool ok = true, more = true;
     const int h = lane >> 2, t = lane & 3;
     while (more) {
       QFrag<HD> q;
-      load_q<HD>(p, use.lid, use.kvh, G, lane, q);
+      split_q<HD>(p, v, q);
       float m = -INFINITY;
       float2 l2 = make_float2(0.f, 0.f);
       float o[HD / 16][4];
@@ -462,32 +513,37 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
       for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
-      for (int st = use.sb; st < use.se; ++st) {
-        cp_async_wait<NST - 2>();
-        __syncwarp();  // this stage is there for every thread, and nobody reads the slot before it any more
-        issue();
-        const int nvalid = min(SPOS, ctx[use.lid] - SPOS * st);
-        const uint32_t pages = (loaded >> (SP * slot)) & ALL;
+      int left = ctx[use.lid] - SPOS * use.sb;  // positions from this stage on
+      for (int st = use.sb; st < use.se && ok; ++st, left -= SPOS) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][slot], phase, p.err));
+        if (!ok) break;
+        const uint32_t pages = s_got[warp][slot];
         const uint8_t* buf = ring + slot * (SP * BLK);
-        if (nvalid == SPOS && pages == ALL)
-          stage_math<HD, false>(buf, q, m, l2, o, nvalid, pages, lane);
+        if (left >= SPOS && pages == ALL)
+          stage_math<HD, false>(buf, q, m, l2, o, left, pages, lane);
         else
-          stage_math<HD, true>(buf, q, m, l2, o, nvalid, pages, lane);
-        slot = slot + 1 == NST ? 0 : slot + 1;
+          stage_math<HD, true>(buf, q, m, l2, o, left, pages, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[warp][slot]);
+        if (++slot == NST) {
+          slot = 0;
+          phase ^= 1;
+        }
       }
+      const PairWalk<HD> done = use;
+      more = use.next(ctx, hkv, g0, g1);
+      if (more) load_q<HD>(p, use.lid, use.kvh, G, lane, v);
       float l = l2.x + l2.y;
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
-      const bool begins = use.sb == 0, ends = use.se == use.ns;
+      const bool begins = done.sb == 0, ends = done.se == done.ns;
       const int which = begins ? 1 : 0;
-      const int pair = use.lid * hkv + use.kvh;
       // A whole pair goes out; a piece to its state (B only at the share's end, over the idle ring).
-      float* d = begins && ends ? p.out + (size_t)use.lid * p.ldo + (size_t)use.kvh * G * HD
+      float* d = begins && ends ? p.out + (size_t)done.lid * p.ldo + (size_t)done.kvh * G * HD
                  : begins       ? reinterpret_cast<float*>(ring)
                                 : state_a + (size_t)warp * G * ROW;
       const int row = begins && ends ? HD : ROW;
       const float r = begins && ends ? (l == 0.f ? 0.f : 8.f / l) : 1.f;
-      __syncwarp();  // the last stage is read
       // This thread holds dims h hd/8 .. + hd/8 - 1 of heads 2t and 2t + 1.
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -506,88 +562,104 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
       }
       if (lane == 0 && !(begins && ends)) {
         s_state[warp] |= begins ? 4 : ends ? 3 : 1;
-        s_pair[which][warp] = pair;
+        if (begins) s_first[warp] = done.P;
+        s_pair[which][warp] = done.lid * hkv + done.kvh;
       }
-      more = use.next(ctx, p.lanes, hkv, g0, g1);
     }
   }
-  __syncthreads();
+  // Lanes of context 0 get zeros.
+  for (int b = blockIdx.x; b < p.lanes; b += gridDim.x)
+    if (ctx[b] == 0)
+      for (int i = threadIdx.x; i < p.num_heads * HD; i += kWarps * 32) p.out[(size_t)b * p.ldo + i] = 0.f;
+  math_sync();
 
-  // ---- pieces, in stage order: A of warp 0, B of warp 0, A of warp 1, ... ----
-  int open_pair = -1;  // a pair begun in this CTA that goes on in the next
-  if (threadIdx.x < G * (HD / 4)) {
-    const int g = threadIdx.x / (HD / 4), d = 4 * (threadIdx.x % (HD / 4));
-    float M = -INFINITY, L = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    int pair = -1;
-    bool begun = false, any = false;
-    auto add = [&](float4 v, float m, float l) {
-      const float Mn = fmaxf(M, m);
-      const float x = M == -INFINITY ? 0.f : ex2(M - Mn), y = m == -INFINITY ? 0.f : ex2(m - Mn);
-      M = Mn;
-      L = L * x + l * y;
-      a.x = a.x * x + v.x * y;
-      a.y = a.y * x + v.y * y;
-      a.z = a.z * x + v.z * y;
-      a.w = a.w * x + v.w * y;
-      any = true;
-    };
-    auto flush = [&](bool whole) {
-      if (whole) {
-        const float r = L == 0.f ? 0.f : 8.f / L;
-        *reinterpret_cast<float4*>(p.out + (size_t)(pair / hkv) * p.ldo + (size_t)((pair % hkv) * G + g) * HD + d) =
-            make_float4(a.x * r, a.y * r, a.z * r, a.w * r);
-      } else {
-        const size_t part = 2 * (size_t)blockIdx.x + (begun ? 1 : 0);
-        *reinterpret_cast<float4*>(p.part_o + (part * G + g) * HD + d) = a;
-        if (d == 0) {
-          p.part_ml[(part * G + g) * 2] = M;
-          p.part_ml[(part * G + g) * 2 + 1] = L;
+  // ---- pieces.  Chain 0 starts with A of warp 0, chain 1 + w with B of warp w; each goes on with
+  // the A's behind it until one ends its pair.  A warp takes a chain: thread w weighs the states of
+  // warp w, then the threads run over the dims. ----
+  static_assert(kWarps == 8, "eight threads hold the eight warps' states");
+  const int me = lane & 7;
+  const int st = s_state[me];
+  const uint32_t is_b = __ballot_sync(0xffffffffu, st & 4) & 0xffu, is_1 = __ballot_sync(0xffffffffu, (st & 3) == 1) & 0xffu,
+                 is_3 = __ballot_sync(0xffffffffu, (st & 3) == 3) & 0xffu;
+  const uint32_t chains = is_b << 1 | ((is_1 | is_3) & 1u);
+  if (chains == 0 && threadIdx.x == 0) p.meta[2 * blockIdx.x] = -1;
+  for (int chain = warp; chain <= kWarps; chain += kWarps) {
+    if (!(chains >> chain & 1)) continue;
+    const int first = chain ? chain - 1 : 0;         // warp of the chain's first state
+    const int from = chain ? first + 1 : 0;          // its first A
+    const int stop = __ffs(~is_1 >> from) - 1 + from;  // the first warp from there whose A does not go on
+    const bool ended = is_3 >> stop & 1;
+    const int end = ended ? stop + 1 : stop;  // states of warps [first, end), the first as B unless chain 0
+    const bool in = me >= first && me < end;
+    const int kind = chain && me == first ? 1 : 0;
+    float x[8], M[8], L[8];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      const float m = in && g < G ? s_ml[kind][me][g][0] : -INFINITY;
+      const float l = in && g < G ? s_ml[kind][me][g][1] : 0.f;
+      M[g] = m;
+#pragma unroll
+      for (int s = 1; s < 8; s <<= 1) M[g] = fmaxf(M[g], __shfl_xor_sync(0xffffffffu, M[g], s));
+      x[g] = m == -INFINITY ? 0.f : ex2(m - M[g]);
+      L[g] = l * x[g];
+#pragma unroll
+      for (int s = 1; s < 8; s <<= 1) L[g] += __shfl_xor_sync(0xffffffffu, L[g], s);
+    }
+    float4 a[8];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) a[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int d = 4 * (lane % (HD / 4));
+    for (int w = first; w < end; ++w) {
+      const float* src = (chain && w == first ? reinterpret_cast<const float*>(smem + (size_t)w * RING)
+                                              : state_a + (size_t)w * G * ROW) + d;
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        if (g < G) {
+          const float xw = __shfl_sync(0xffffffffu, x[g], w);
+          const float4 y = *reinterpret_cast<const float4*>(src + g * ROW);
+          a[g].x = fmaf(y.x, xw, a[g].x);
+          a[g].y = fmaf(y.y, xw, a[g].y);
+          a[g].z = fmaf(y.z, xw, a[g].z);
+          a[g].w = fmaf(y.w, xw, a[g].w);
         }
       }
-      M = -INFINITY;
-      L = 0.f;
-      a = make_float4(0.f, 0.f, 0.f, 0.f);
-      begun = any = false;
-    };
-#pragma unroll 4
-    for (int w = 0; w < kWarps; ++w) {
-      const int st = s_state[w];
-      const float4 va = *reinterpret_cast<const float4*>(state_a + ((size_t)w * G + g) * ROW + d);
-      const float4 vb = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + (size_t)w * RING) + g * ROW + d);
-      const float2 ma = *reinterpret_cast<const float2*>(s_ml[0][w][g]), mb = *reinterpret_cast<const float2*>(s_ml[1][w][g]);
-      if (st & 1) {
-        pair = s_pair[0][w];
-        add(va, ma.x, ma.y);
-        if (st & 2) flush(begun);
-      }
-      if (st & 4) {
-        pair = s_pair[1][w];
-        begun = true;
-        add(vb, mb.x, mb.y);
+    }
+    const int pair = s_pair[chain ? 1 : 0][first];
+    const bool whole = chain && ended;
+    const size_t part = (2 * (size_t)blockIdx.x + (chain ? 1 : 0)) * G;
+    float* dst = whole ? p.out + (size_t)(pair / hkv) * p.ldo + (size_t)(pair % hkv) * G * HD : p.part_o + part * HD;
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      if (g < G) {
+        const float r = whole ? (L[g] == 0.f ? 0.f : 8.f / L[g]) : 1.f;
+        if (lane < HD / 4)
+          *reinterpret_cast<float4*>(dst + g * HD + d) = make_float4(a[g].x * r, a[g].y * r, a[g].z * r, a[g].w * r);
+        if (!whole && lane == 0) {
+          p.part_ml[(part + g) * 2] = M[g];
+          p.part_ml[(part + g) * 2 + 1] = L[g];
+        }
       }
     }
-    if (any) {
-      if (begun) open_pair = pair;
-      flush(false);
-    }
-  }
-  if (threadIdx.x == 0) {
-    p.meta[2 * blockIdx.x] = open_pair;
-    if (open_pair >= 0) {
-      const int b = open_pair / hkv;
-      const int ns = (ctx[b] + SPOS - 1) / SPOS, P = C[b] + (open_pair % hkv) * ns;
-      p.meta[2 * blockIdx.x + 1] = (P + ns - 1) / (Q * kWarps) - P / (Q * kWarps) + 1;
+    if (chain == 31 - __clz(chains) && lane == 0) {
+      // A pair begun here that goes on in the next CTAs, and how many CTAs its stages fall into.
+      const bool open = chain && !ended;
+      p.meta[2 * blockIdx.x] = open ? pair : -1;
+      if (open) {
+        const int per = Q * kWarps, begin = s_first[first], ns = PairWalk<HD>::stages(ctx[pair / hkv]);
+        p.meta[2 * blockIdx.x + 1] = (begin + ns - 1) / per - begin / per + 1;
+      }
     }
   }
 }
 
-// Pairs that were cut: block c merges the pair whose first segment ends CTA c's share.  Its
-// segments are CTA c's last and the first ones of the CTAs behind it, merged in that order.
+// Pairs that were cut: block c merges the pair that CTA c began and left open.  Its segments
+// are CTA c's last and the first ones of the CTAs behind it, merged in that order.
 // 1024 threads: G hd / 4 columns by as many slices of the segments as fit.
 __global__ void __launch_bounds__(1024) attn_q4_combine_kernel(const AttnQ4Params p, int hd) {
   __shared__ float4 s_o[1024];
   __shared__ float s_l[1024];
+  extern __shared__ float2 s_ml[];  // [nseg][G], then the weights in place of the maxima
+  __shared__ float s_m[8];
   griddep_launch();
   griddep_wait();
   const int c = blockIdx.x, pair = p.meta[2 * c];
@@ -596,17 +668,27 @@ __global__ void __launch_bounds__(1024) attn_q4_combine_kernel(const AttnQ4Param
   const int cols = G * (hd / 4), slices = 1024 / cols;
   const int col = threadIdx.x % cols, slice = threadIdx.x / cols;
   const int g = col / (hd / 4), d = 4 * (col % (hd / 4));
-  auto part = [&](int s) { return (s == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + s)) * G + g; };
+  auto part = [&](int s) { return s == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + s); };
+  for (int i = threadIdx.x; i < nseg * G; i += 1024)
+    s_ml[i] = *reinterpret_cast<const float2*>(p.part_ml + (part(i / G) * G + i % G) * 2);
+  __syncthreads();
+  if (threadIdx.x < 32 * G) {
+    const int hg = threadIdx.x >> 5;
+    float M = -INFINITY;
+    for (int s = threadIdx.x & 31; s < nseg; s += 32) M = fmaxf(M, s_ml[s * G + hg].x);
+    M = warp_max(M);
+    if ((threadIdx.x & 31) == 0) s_m[hg] = M;
+  }
+  __syncthreads();
   float L = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   if (slice < slices) {
-    float M = -INFINITY;
-    for (int s = 0; s < nseg; ++s) M = fmaxf(M, p.part_ml[part(s) * 2]);
+    const float M = s_m[g];
     const int per = (nseg + slices - 1) / slices;
-#pragma unroll 4
+#pragma unroll 8
     for (int s = slice * per; s < min(nseg, (slice + 1) * per); ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part(s) * 2);
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + part(s) * hd + d);
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (part(s) * G + g) * hd + d);
+      const float2 ml = s_ml[s * G + g];
       const float x = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
       L = fmaf(ml.y, x, L);
       a.x = fmaf(v.x, x, a.x);
@@ -634,6 +716,16 @@ __global__ void __launch_bounds__(1024) attn_q4_combine_kernel(const AttnQ4Param
 }
 
 }  // namespace
+
+int attn_q4_device_error(int clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_attn_q4_error, sizeof(int)) != cudaSuccess) return -1;
+  if (clear && v) {
+    int z = 0;
+    cudaMemcpyToSymbol(g_attn_q4_error, &z, sizeof(int));
+  }
+  return v;
+}
 
 // Two partial segments per CTA (one that begins a pair, one that continues it), and the
 // descriptors of cut pairs.
@@ -681,13 +773,14 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
   p.num_kv_heads = (int)num_kv_heads;
   p.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   p.bad = ops_error_word();
-  GLC_REQUIRE(p.bad, "paged_attention_q4: device status word unavailable");
+  p.err = device_symbol_address(g_attn_q4_error);
+  GLC_REQUIRE(p.bad && p.err, "paged_attention_q4: device status word unavailable");
   auto kern = head_dim == 128 ? attn_q4_kernel<128> : attn_q4_kernel<64>;
   const size_t pages = head_dim == 128 ? kStagePages<128> : kStagePages<64>;
   const size_t smem = kWarps * (kStages * pages * q4_block_bytes(head_dim) + G * (head_dim + 4) * sizeof(float));
   if ((rc = allow_dynamic_smem((const void*)kern, (int)smem))) return rc;
-  if ((rc = launch_pdl(kern, dim3((unsigned)grid), dim3(kWarps * 32), smem, stream, 1, p))) return rc;
-  return launch_pdl(attn_q4_combine_kernel, dim3((unsigned)grid), dim3(1024), 0, stream, 1, p, (int)head_dim);
+  if ((rc = launch_pdl(kern, dim3((unsigned)grid), dim3(kThreads), smem, stream, 1, p))) return rc;
+  return launch_pdl(attn_q4_combine_kernel, dim3((unsigned)grid), dim3(1024), (size_t)grid * G * sizeof(float2), stream, 1, p, (int)head_dim);
 }
 
 }  // namespace glacier
