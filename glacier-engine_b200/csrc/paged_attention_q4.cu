@@ -26,16 +26,11 @@
 
 namespace glacier {
 
-__device__ int g_attn_q4_error;
-
 namespace {
 
 constexpr int kMaxLanes = 1024;
-constexpr int kWarps = 8;                     // warps that compute, two per SM partition
-constexpr int kThreads = 32 * (kWarps + 4);   // and a warpgroup whose first warp loads
-// Registers: 384 x 168 at launch = 256 x 232 + 128 x 40 after the split.
-constexpr int kRegsMath = 232, kRegsLoad = 40;
-constexpr int kStages = 5;  // stages in a warp's ring: 184 KB of K/V in flight per SM
+constexpr int kWarps = 8;   // two per SM partition
+constexpr int kStages = 4;  // stages in a warp's ring: 147 KB of K/V per SM, three quarters of it in flight
 // Pages per stage: 4608 bytes at either head size.
 template <int HD>
 constexpr int kStagePages = HD == 128 ? 2 : 4;
@@ -53,11 +48,10 @@ struct AttnQ4Params {
   int32_t* meta;   // [grid][2]: the pair that is cut at the end of CTA c's share (or -1), its segments
   float* part_ml;  // [2 grid][G][2] maximum (base 2) and sum of a segment
   float* part_o;   // [2 grid][G][hd]
-  size_t page_bytes;
+  uint32_t page_bytes;
   int lanes, max_pages, num_pages, layer, num_heads, num_kv_heads;
   float scale_log2;
   int* bad;
-  int* err;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -92,12 +86,14 @@ __device__ __forceinline__ uint32_t v_bits(uint32_t x) {
   return d;
 }
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
-          smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
-      : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 template <int N>
@@ -177,25 +173,20 @@ __device__ __forceinline__ void split_q(const AttnQ4Params& p, const float (&v)[
   }
 }
 
-// One stage of one warp: scores, online softmax, and the weighted V.  Weights are 2^(7 + s - m)
-// in base-2 scores s: m is a reference near the running maximum of head lane / 4, moved
-// (and everything rescaled) only when a score passes it by more than 2^8, so the weights stay
-// below 2^15 and their low parts normal fp16 numbers.  l: this thread's share of their
-// sum; o: sums of weight * v / 8.
-// nvalid: positions of the stage inside the context; pages: bit i set when page i was loaded.
-template <int HD, bool MASK>
-__device__ __forceinline__ void stage_math(const uint8_t* __restrict__ buf, const QFrag<HD>& q, float& m, float2& l,
-                                           float (&o)[HD / 16][4], int nvalid, uint32_t pages, int lane) {
-  constexpr int NG = HD / 32, NW = HD / 32;  // scale groups; words per thread and position (K) or pair (V)
-  constexpr int BLK = 18 * HD, SP = kStagePages<HD>;
+// Raw scores of one stage: sc[2 page + half] = the scores of head lane / 4 with the positions
+// 8 half + 2 (lane % 4) + {0, 1} of the page.
+template <int HD>
+__device__ __forceinline__ void stage_scores(const uint8_t* __restrict__ buf, const QFrag<HD>& q,
+                                             float2 (&sc)[2 * kStagePages<HD>], int lane) {
+  constexpr int NG = HD / 32;  // scale groups = words per thread and position
+  constexpr int BLK = 18 * HD;
   const int n = lane >> 2, t = lane & 3;
-  float2 sc[SP * 2];
 #pragma unroll
-  for (int pg = 0; pg < SP; ++pg) {
+  for (int pg = 0; pg < kStagePages<HD>; ++pg) {
     const uint8_t* K = buf + pg * BLK;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const Words<NW> w = lds<NW>(K + (8 * j + n) * (HD / 2) + t * (4 * NG));
+      const Words<NG> w = lds<NG>(K + (8 * j + n) * (HD / 2) + t * (4 * NG));
       const Words<NG> s = lds<NG>(K + 16 * HD + (4 * j + t) * (4 * NG));
       float2 r = make_float2(0.f, 0.f);
 #pragma unroll
@@ -208,13 +199,31 @@ __device__ __forceinline__ void stage_math(const uint8_t* __restrict__ buf, cons
         r = __ffma2_rn(f, make_float2(d[0], d[1]), r);
         r = __ffma2_rn(f, make_float2(d[2], d[3]), r);
       }
-      if constexpr (MASK) {
-        const int at = pg * kQ4Page + 8 * j + 2 * t;
-        const bool here = (pages >> pg) & 1;
-        if (!here || at >= nvalid) r.x = -INFINITY;
-        if (!here || at + 1 >= nvalid) r.y = -INFINITY;
-      }
       sc[2 * pg + j] = r;
+    }
+  }
+}
+
+// The online softmax of one stage's scores and its weighted V.  Weights are 2^(7 + s - m)
+// in base-2 scores s: m is a reference near the running maximum of head lane / 4, moved
+// (and everything rescaled) only when a score passes it by more than 2^8, so the weights stay
+// below 2^15 and their low parts normal fp16 numbers.  l: this thread's share of their
+// sum; o: sums of weight * v / 8.
+// nvalid: positions of the stage inside the context; pages: bit i set when page i was loaded.
+template <int HD, bool MASK>
+__device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, const QFrag<HD>& q,
+                                             float2 (&sc)[2 * kStagePages<HD>], float& m, float2& l,
+                                             float (&o)[HD / 16][4], int nvalid, uint32_t pages, int lane) {
+  constexpr int NG = HD / 32, NW = HD / 32;  // scale groups; words per thread and position pair
+  constexpr int BLK = 18 * HD, SP = kStagePages<HD>;
+  const int n = lane >> 2, t = lane & 3;
+  if constexpr (MASK) {
+#pragma unroll
+    for (int i = 0; i < 2 * SP; ++i) {
+      const int at = 8 * i + 2 * t;
+      const bool here = (pages >> (i / 2)) & 1;
+      if (!here || at >= nvalid) sc[i].x = -INFINITY;
+      if (!here || at + 1 >= nvalid) sc[i].y = -INFINITY;
     }
   }
   float mx = fmaxf(sc[0].x, sc[0].y);
@@ -384,128 +393,103 @@ __device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ct
 // begins a pair which goes on behind it (state B).  At the end of the CTA the pieces
 // merge in shared memory in stage order; what is cut at the CTA's own ends goes to the
 // combine kernel, at most two partial segments per CTA.
-// The last warp loads: its thread w keeps the ring of warp w filled by bulk copies, one per
-// page, so the arithmetic warps spend no instruction on page tables and addresses.
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 1) attn_q4_kernel(const AttnQ4Params p) {
+__global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Params p) {
   constexpr int BLK = 18 * HD, SP = kStagePages<HD>, SPOS = kStagePos<HD>;
-  constexpr int NST = kStages;
+  constexpr int NST = kStages, IDS = 32 / SP;
   constexpr uint32_t ALL = (1u << SP) - 1;
   constexpr int ROW = HD + 4;  // floats per head of a state
   constexpr int RING = NST * SP * BLK;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[kWarps][NST], empty[kWarps][NST];
-  __shared__ uint32_t s_got[kWarps][NST];  // the pages of a stage that are there
-  __shared__ float s_ml[2][kWarps][8][2];
+  __shared__ __align__(8) float s_ml[2][kWarps][8][2];
   __shared__ int s_state[kWarps];  // 1: state A, 2: and it ends its pair, 4: state B
   __shared__ int s_pair[2][kWarps], s_first[kWarps];  // of the states; the first stage of a B's pair
-  __shared__ PairWalk<HD> s_start[kWarps];
-  __shared__ int s_g[kWarps][2];
   __shared__ int ctx[kMaxLanes];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hkv = p.num_kv_heads, G = p.num_heads / hkv;
-  if (warp < kWarps && lane == 0) {
-    for (int i = 0; i < NST; ++i) {
-      mbar_init(&full[warp][i], 1);
-      mbar_init(&empty[warp][i], 1);
-    }
-    fence_mbar_init();
-    s_state[warp] = 0;
-  }
   griddep_launch();
   griddep_wait();  // q, the pages, tables and lengths come from earlier kernels
   uint8_t* ring = smem + (size_t)warp * RING;
   float* state_a = reinterpret_cast<float*>(smem + (size_t)kWarps * RING);  // [warps][G][ROW]
   PairWalk<HD> use;
-  int g0 = 0, g1 = 0, Q = 1;
-  float v[HD / 32][8];
-  if (warp < kWarps) {
-    Q = find_share<HD>(p, blockIdx.x * kWarps + warp, ctx, use, g0, g1);
-    if (use.lid >= 0) load_q<HD>(p, use.lid, use.kvh, G, lane, v);
-    if (lane == 0) {
-      s_start[warp] = use;
-      s_g[warp][0] = g0;
-      s_g[warp][1] = g1;
-    }
-  }
-  __syncthreads();
+  int g0 = 0, g1 = 0;
+  const int Q = find_share<HD>(p, blockIdx.x * kWarps + warp, ctx, use, g0, g1);
+  if (lane == 0) s_state[warp] = 0;
+  __syncwarp();  // ctx and the state word are this warp's own writes
 
-  if (warp >= kWarps) {
-    // ---- loads ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
-    if (warp > kWarps) return;
-    bool more = lane < kWarps && s_start[lane < kWarps ? lane : 0].lid >= 0;
-    const int w = lane < kWarps ? lane : 0;
-    PairWalk<HD> ld = s_start[w];
-    const int a0 = s_g[w][0], a1 = s_g[w][1];
+  if (use.lid >= 0) {
+    float v[HD / 32][8];
+    load_q<HD>(p, use.lid, use.kvh, G, lane, v);
+    // ---- loads: the warp's stages in order, NST - 1 of them ahead of the arithmetic ----
+    PairWalk<HD> ld = use;
     const uint64_t pol = l2_evict_first_policy();
-    int st = ld.sb, slot = 0;
-    uint32_t phase = 1;  // the first pass over the ring finds every slot free
-    int32_t ids[SP];
-    auto fetch = [&]() {  // page ids of stage st; -2: past the context
-#pragma unroll
-      for (int i = 0; i < SP; ++i) {
-        const int j = SP * st + i;
-        ids[i] = j * kQ4Page < ctx[ld.lid] ? p.tables[(size_t)ld.lid * p.max_pages + j] : -2;
-      }
+    int ld_st = 0, ld_at = 0;  // next stage; its place among the stages whose page ids `ids` holds
+    int32_t ids = 0;
+    uint32_t ids_ok = 0;             // bit i: page id i is one of the pool's
+    const uint8_t* src0 = nullptr;   // this thread's 16 bytes of the head's block in page 0
+    auto fetch_ids = [&]() {         // page ids of the next 32 pages, one per thread
+      const int j = SP * ld_st + lane;
+      const bool inside = j * kQ4Page < ctx[ld.lid];
+      ids = inside ? p.tables[(size_t)ld.lid * p.max_pages + j] : 0;
+      const bool ok = inside && (unsigned)ids < (unsigned)p.num_pages;
+      ids_ok = __ballot_sync(0xffffffffu, ok);
+      if (inside && !ok) atomicExch(p.bad, 1);
+      ld_at = 0;
     };
-    if (more) fetch();
-    long long idle_since = 0;
-    while (__any_sync(0xffffffffu, more)) {
-      const bool go = more && mbar_test_wait(&empty[w][slot], phase);
-      if (go) {
-        uint32_t got = 0;
-#pragma unroll
-        for (int i = 0; i < SP; ++i) got |= (unsigned)ids[i] < (unsigned)p.num_pages ? 1u << i : 0u;
-        if (got != ALL) {
-          bool bad = false;
-#pragma unroll
-          for (int i = 0; i < SP; ++i) bad |= !(got >> i & 1) && ids[i] != -2;
-          if (bad) atomicExch(p.bad, 1);
-        }
-        s_got[w][slot] = got;
-        mbar_arrive_expect_tx(&full[w][slot], BLK * __popc(got));
-        const uint8_t* src = p.pool + ((size_t)p.layer * hkv + ld.kvh) * BLK;
-        uint8_t* dst = smem + (size_t)w * RING + slot * (SP * BLK);
+    auto enter = [&]() {
+      ld_st = ld.sb;
+      src0 = p.pool + ((size_t)p.layer * hkv + ld.kvh) * BLK + 16 * lane;
+      fetch_ids();
+    };
+    enter();
+    const uint32_t ring_at = smem_u32(ring) + 16 * lane;
+    uint32_t loaded = 0;  // SP bits per ring slot: the pages that are there
+    int slot_in = 0;
+    bool ld_more = true;
+    auto issue = [&]() {
+      if (ld_more && ld_st >= ld.se) {
+        ld_more = ld.next(ctx, hkv, g0, g1);
+        if (ld_more) enter();
+      }
+      if (ld_more) {
+        if (ld_at == IDS) fetch_ids();
+        const uint32_t got = (ids_ok >> (SP * ld_at)) & ALL;
+        const uint8_t* src[SP];
 #pragma unroll
         for (int i = 0; i < SP; ++i)
-          if (got >> i & 1) bulk_load(dst + i * BLK, src + (size_t)ids[i] * p.page_bytes, BLK, &full[w][slot], pol);
-        if (++slot == NST) {
-          slot = 0;
-          phase ^= 1;
-        }
-        if (++st >= ld.se) {
-          more = ld.next(ctx, hkv, a0, a1);
-          st = ld.sb;
-        }
-        if (more) fetch();
+          src[i] = src0 + (uint64_t)(uint32_t)__shfl_sync(0xffffffffu, ids, SP * ld_at + i) * p.page_bytes - i * BLK;
+        const uint32_t dst = ring_at + slot_in * (SP * BLK);
+        // A stage's pages follow one another in the ring: chunks of 16 bytes, one per thread and step.
+        auto chunks = [&](bool all) {
+#pragma unroll
+          for (int i = 0; i < SP * BLK / 512; ++i) {
+            const int lo = 512 * i / BLK, cut = ((lo + 1) * BLK - 512 * i) / 16;  // threads from `cut` on: the next page
+            const int pg = cut < 32 && lane >= cut ? lo + 1 : lo;
+            const uint8_t* s = pg == lo ? src[lo] : src[lo + 1 < SP ? lo + 1 : lo];
+            if (all || (got >> pg & 1)) cp_async16(dst + 512 * i, s + 512 * i, pol);
+          }
+        };
+        if (got == ALL) chunks(true); else chunks(false);
+        loaded = (loaded & ~(ALL << (SP * slot_in))) | got << (SP * slot_in);
+        ++ld_st;
+        ++ld_at;
       }
-      if (__any_sync(0xffffffffu, go)) {
-        idle_since = 0;
-      } else {
-        // Every wait is bounded: about two seconds without a free slot, and the loader gives up.
-        const long long now = clock64();
-        if (idle_since == 0) idle_since = now;
-        if (now - idle_since > kSpinLimitCycles) {
-          if (lane == 0) atomicExch(p.err, kErrTimeout);
-          break;
-        }
-        __nanosleep(40);
-      }
-    }
-    return;
-  }
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMath));
-  auto math_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); };
-  if (use.lid >= 0) {
+      cp_async_commit();
+      slot_in = slot_in + 1 == NST ? 0 : slot_in + 1;
+    };
+#pragma unroll 1
+    for (int i = 0; i < NST - 1; ++i) issue();
+
     // ---- arithmetic ----
     int slot = 0;
-    uint32_t phase = 0;
-    bool ok = true, more = true;
+    bool more = true;
     const int h = lane >> 2, t = lane & 3;
     while (more) {
       QFrag<HD> q;
       split_q<HD>(p, v, q);
+      const PairWalk<HD> done = use;
+      more = use.next(ctx, hkv, g0, g1);
+      if (more) load_q<HD>(p, use.lid, use.kvh, G, lane, v);  // arrives while this pair is worked on
       float m = -INFINITY;
       float2 l2 = make_float2(0.f, 0.f);
       float o[HD / 16][4];
@@ -513,26 +497,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_q4_kernel(const AttnQ4Params
       for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
-      int left = ctx[use.lid] - SPOS * use.sb;  // positions from this stage on
-      for (int st = use.sb; st < use.se && ok; ++st, left -= SPOS) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][slot], phase, p.err));
-        if (!ok) break;
-        const uint32_t pages = s_got[warp][slot];
+      int left = ctx[done.lid] - SPOS * done.sb;  // positions from this stage on
+      for (int st = done.sb; st < done.se; ++st, left -= SPOS) {
+        cp_async_wait<NST - 2>();
+        __syncwarp();  // this stage is there for every thread, and nobody reads the slot before it any more
+        issue();
+        const uint32_t pages = (loaded >> (SP * slot)) & ALL;
         const uint8_t* buf = ring + slot * (SP * BLK);
+        float2 sc[2 * SP];
+        stage_scores<HD>(buf, q, sc, lane);
         if (left >= SPOS && pages == ALL)
-          stage_math<HD, false>(buf, q, m, l2, o, left, pages, lane);
+          stage_values<HD, false>(buf, q, sc, m, l2, o, SPOS, ALL, lane);
         else
-          stage_math<HD, true>(buf, q, m, l2, o, left, pages, lane);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[warp][slot]);
-        if (++slot == NST) {
-          slot = 0;
-          phase ^= 1;
-        }
+          stage_values<HD, true>(buf, q, sc, m, l2, o, left, pages, lane);
+        slot = slot + 1 == NST ? 0 : slot + 1;
       }
-      const PairWalk<HD> done = use;
-      more = use.next(ctx, hkv, g0, g1);
-      if (more) load_q<HD>(p, use.lid, use.kvh, G, lane, v);
+      __syncwarp();  // the last stage is read
       float l = l2.x + l2.y;
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -571,56 +551,54 @@ __global__ void __launch_bounds__(kThreads, 1) attn_q4_kernel(const AttnQ4Params
   for (int b = blockIdx.x; b < p.lanes; b += gridDim.x)
     if (ctx[b] == 0)
       for (int i = threadIdx.x; i < p.num_heads * HD; i += kWarps * 32) p.out[(size_t)b * p.ldo + i] = 0.f;
-  math_sync();
+  __syncthreads();
 
   // ---- pieces.  Chain 0 starts with A of warp 0, chain 1 + w with B of warp w; each goes on with
-  // the A's behind it until one ends its pair.  A warp takes a chain: thread w weighs the states of
-  // warp w, then the threads run over the dims. ----
-  static_assert(kWarps == 8, "eight threads hold the eight warps' states");
-  const int me = lane & 7;
-  const int st = s_state[me];
-  const uint32_t is_b = __ballot_sync(0xffffffffu, st & 4) & 0xffu, is_1 = __ballot_sync(0xffffffffu, (st & 3) == 1) & 0xffu,
-                 is_3 = __ballot_sync(0xffffffffu, (st & 3) == 3) & 0xffu;
+  // the A's behind it until one ends its pair.  A warp takes a chain, its threads the dims. ----
+  constexpr uint32_t WARPS = (1u << kWarps) - 1;
+  const int st = lane < kWarps ? s_state[lane] : 0;
+  const uint32_t is_b = __ballot_sync(0xffffffffu, st & 4) & WARPS,
+                 is_1 = __ballot_sync(0xffffffffu, (st & 3) == 1) & WARPS,
+                 is_3 = __ballot_sync(0xffffffffu, (st & 3) == 3) & WARPS;
   const uint32_t chains = is_b << 1 | ((is_1 | is_3) & 1u);
   if (chains == 0 && threadIdx.x == 0) p.meta[2 * blockIdx.x] = -1;
   for (int chain = warp; chain <= kWarps; chain += kWarps) {
     if (!(chains >> chain & 1)) continue;
-    const int first = chain ? chain - 1 : 0;         // warp of the chain's first state
-    const int from = chain ? first + 1 : 0;          // its first A
+    const int first = chain ? chain - 1 : 0;           // warp of the chain's first state
+    const int from = chain ? first + 1 : 0;            // its first A
     const int stop = __ffs(~is_1 >> from) - 1 + from;  // the first warp from there whose A does not go on
     const bool ended = is_3 >> stop & 1;
     const int end = ended ? stop + 1 : stop;  // states of warps [first, end), the first as B unless chain 0
-    const bool in = me >= first && me < end;
-    const int kind = chain && me == first ? 1 : 0;
-    float x[8], M[8], L[8];
-#pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      const float m = in && g < G ? s_ml[kind][me][g][0] : -INFINITY;
-      const float l = in && g < G ? s_ml[kind][me][g][1] : 0.f;
-      M[g] = m;
-#pragma unroll
-      for (int s = 1; s < 8; s <<= 1) M[g] = fmaxf(M[g], __shfl_xor_sync(0xffffffffu, M[g], s));
-      x[g] = m == -INFINITY ? 0.f : ex2(m - M[g]);
-      L[g] = l * x[g];
-#pragma unroll
-      for (int s = 1; s < 8; s <<= 1) L[g] += __shfl_xor_sync(0xffffffffu, L[g], s);
-    }
+    float M[8], L[8];
     float4 a[8];
 #pragma unroll
-    for (int g = 0; g < 8; ++g) a[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int g = 0; g < 8; ++g) {
+      M[g] = -INFINITY;
+      L[g] = 0.f;
+      a[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int w = first; w < end; ++w) {
+      const float(*ml)[2] = s_ml[chain && w == first ? 1 : 0][w];
+#pragma unroll
+      for (int g = 0; g < 8; ++g)
+        if (g < G) M[g] = fmaxf(M[g], ml[g][0]);
+    }
     const int d = 4 * (lane % (HD / 4));
     for (int w = first; w < end; ++w) {
-      const float* src = (chain && w == first ? reinterpret_cast<const float*>(smem + (size_t)w * RING)
-                                              : state_a + (size_t)w * G * ROW) + d;
+      const bool b = chain && w == first;
+      const float(*ml)[2] = s_ml[b ? 1 : 0][w];
+      const float* src = (b ? reinterpret_cast<const float*>(smem + (size_t)w * RING) : state_a + (size_t)w * G * ROW) + d;
 #pragma unroll
       for (int g = 0; g < 8; ++g) {
         if (g < G) {
-          const float xw = __shfl_sync(0xffffffffu, x[g], w);
+          const float2 r = *reinterpret_cast<const float2*>(ml[g]);
           const float4 y = *reinterpret_cast<const float4*>(src + g * ROW);
-          a[g].x = fmaf(y.x, xw, a[g].x);
-          a[g].y = fmaf(y.y, xw, a[g].y);
-          a[g].z = fmaf(y.z, xw, a[g].z);
-          a[g].w = fmaf(y.w, xw, a[g].w);
+          const float x = r.x == -INFINITY ? 0.f : ex2(r.x - M[g]);
+          L[g] = fmaf(r.y, x, L[g]);
+          a[g].x = fmaf(y.x, x, a[g].x);
+          a[g].y = fmaf(y.y, x, a[g].y);
+          a[g].z = fmaf(y.z, x, a[g].z);
+          a[g].w = fmaf(y.w, x, a[g].w);
         }
       }
     }
@@ -652,80 +630,59 @@ __global__ void __launch_bounds__(kThreads, 1) attn_q4_kernel(const AttnQ4Params
   }
 }
 
-// Pairs that were cut: block c merges the pair that CTA c began and left open.  Its segments
-// are CTA c's last and the first ones of the CTAs behind it, merged in that order.
-// 1024 threads: G hd / 4 columns by as many slices of the segments as fit.
-__global__ void __launch_bounds__(1024) attn_q4_combine_kernel(const AttnQ4Params p, int hd) {
-  __shared__ float4 s_o[1024];
-  __shared__ float s_l[1024];
-  extern __shared__ float2 s_ml[];  // [nseg][G], then the weights in place of the maxima
-  __shared__ float s_m[8];
+// Pairs that were cut: block (c, g) merges head g of the pair that CTA c began and left open.  Its
+// segments are CTA c's last and the first ones of the CTAs behind it; eight slices of
+// them in order, then the slices in order.
+constexpr int kSlices = 8;
+template <int HD>
+__global__ void __launch_bounds__(kSlices * HD / 4) attn_q4_combine_kernel(const AttnQ4Params p) {
+  __shared__ float4 s_o[kSlices][HD / 4];
+  __shared__ float s_l[kSlices];
   griddep_launch();
   griddep_wait();
-  const int c = blockIdx.x, pair = p.meta[2 * c];
-  if (pair < 0) return;
-  const int nseg = p.meta[2 * c + 1], G = p.num_heads / p.num_kv_heads;
-  const int cols = G * (hd / 4), slices = 1024 / cols;
-  const int col = threadIdx.x % cols, slice = threadIdx.x / cols;
-  const int g = col / (hd / 4), d = 4 * (col % (hd / 4));
-  auto part = [&](int s) { return s == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + s); };
-  for (int i = threadIdx.x; i < nseg * G; i += 1024)
-    s_ml[i] = *reinterpret_cast<const float2*>(p.part_ml + (part(i / G) * G + i % G) * 2);
-  __syncthreads();
-  if (threadIdx.x < 32 * G) {
-    const int hg = threadIdx.x >> 5;
-    float M = -INFINITY;
-    for (int s = threadIdx.x & 31; s < nseg; s += 32) M = fmaxf(M, s_ml[s * G + hg].x);
-    M = warp_max(M);
-    if ((threadIdx.x & 31) == 0) s_m[hg] = M;
-  }
-  __syncthreads();
+  const int c = blockIdx.x, g = blockIdx.y, G = gridDim.y;
+  const int2 meta = *reinterpret_cast<const int2*>(p.meta + 2 * c);
+  if (meta.x < 0) return;
+  const int nseg = meta.y, lane = threadIdx.x & 31;
+  const int col = threadIdx.x % (HD / 4), slice = threadIdx.x / (HD / 4);
+  auto part = [&](int s) { return (s == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + s)) * G + g; };
+  float M = -INFINITY;
+  for (int s = lane; s < nseg; s += 32) M = fmaxf(M, p.part_ml[part(s) * 2]);
+  M = warp_max(M);
   float L = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (slice < slices) {
-    const float M = s_m[g];
-    const int per = (nseg + slices - 1) / slices;
-#pragma unroll 8
-    for (int s = slice * per; s < min(nseg, (slice + 1) * per); ++s) {
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (part(s) * G + g) * hd + d);
-      const float2 ml = s_ml[s * G + g];
-      const float x = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-      L = fmaf(ml.y, x, L);
-      a.x = fmaf(v.x, x, a.x);
-      a.y = fmaf(v.y, x, a.y);
-      a.z = fmaf(v.z, x, a.z);
-      a.w = fmaf(v.w, x, a.w);
-    }
+  const int per = (nseg + kSlices - 1) / kSlices;
+#pragma unroll 4
+  for (int s = slice * per; s < min(nseg, (slice + 1) * per); ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + part(s) * HD + 4 * col);
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part(s) * 2);
+    const float x = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+    L = fmaf(ml.y, x, L);
+    a.x = fmaf(v.x, x, a.x);
+    a.y = fmaf(v.y, x, a.y);
+    a.z = fmaf(v.z, x, a.z);
+    a.w = fmaf(v.w, x, a.w);
   }
-  s_o[threadIdx.x] = a;
-  s_l[threadIdx.x] = L;
+  s_o[slice][col] = a;
+  if (col == 0) s_l[slice] = L;
   __syncthreads();
   if (slice != 0) return;
-  for (int s = 1; s < slices; ++s) {
-    const float4 v = s_o[s * cols + col];
-    L += s_l[s * cols + col];
+#pragma unroll
+  for (int s = 1; s < kSlices; ++s) {
+    const float4 v = s_o[s][col];
+    L += s_l[s];
     a.x += v.x;
     a.y += v.y;
     a.z += v.z;
     a.w += v.w;
   }
   const float r = L == 0.f ? 0.f : 8.f / L;
-  *reinterpret_cast<float4*>(p.out + (size_t)(pair / p.num_kv_heads) * p.ldo +
-                             (size_t)((pair % p.num_kv_heads) * G + g) * hd + d) =
+  *reinterpret_cast<float4*>(p.out + (size_t)(meta.x / p.num_kv_heads) * p.ldo +
+                             (size_t)((meta.x % p.num_kv_heads) * G + g) * HD + 4 * col) =
       make_float4(a.x * r, a.y * r, a.z * r, a.w * r);
 }
 
 }  // namespace
-
-int attn_q4_device_error(int clear) {
-  int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_attn_q4_error, sizeof(int)) != cudaSuccess) return -1;
-  if (clear && v) {
-    int z = 0;
-    cudaMemcpyToSymbol(g_attn_q4_error, &z, sizeof(int));
-  }
-  return v;
-}
 
 // Two partial segments per CTA (one that begins a pair, one that continues it), and the
 // descriptors of cut pairs.
@@ -751,6 +708,8 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
               "paged_attention_q4: q, out and workspace must be 16-byte aligned");
   const size_t need = attention_q4_workspace_floats(num_heads, num_kv_heads, head_dim);
   GLC_REQUIRE(workspace_floats >= need, "paged_attention_q4: workspace of %zu floats needed", need);
+  const size_t page_bytes = num_layers * num_kv_heads * q4_block_bytes(head_dim);
+  GLC_REQUIRE(page_bytes < ((size_t)1 << 32), "paged_attention_q4: pages of %zu bytes", page_bytes);
   const int grid = sm_count();
   const size_t G = num_heads / num_kv_heads;
   AttnQ4Params p;
@@ -764,7 +723,7 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
   p.meta = reinterpret_cast<int32_t*>(workspace);
   p.part_o = workspace + ceil_div(2 * (size_t)grid, (size_t)4) * 4;
   p.part_ml = p.part_o + 2 * (size_t)grid * G * head_dim;
-  p.page_bytes = num_layers * num_kv_heads * q4_block_bytes(head_dim);
+  p.page_bytes = (uint32_t)page_bytes;
   p.lanes = (int)lanes;
   p.max_pages = (int)max_pages;
   p.num_pages = (int)num_pages;
@@ -773,14 +732,14 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
   p.num_kv_heads = (int)num_kv_heads;
   p.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   p.bad = ops_error_word();
-  p.err = device_symbol_address(g_attn_q4_error);
-  GLC_REQUIRE(p.bad && p.err, "paged_attention_q4: device status word unavailable");
+  GLC_REQUIRE(p.bad, "paged_attention_q4: device status word unavailable");
   auto kern = head_dim == 128 ? attn_q4_kernel<128> : attn_q4_kernel<64>;
   const size_t pages = head_dim == 128 ? kStagePages<128> : kStagePages<64>;
   const size_t smem = kWarps * (kStages * pages * q4_block_bytes(head_dim) + G * (head_dim + 4) * sizeof(float));
   if ((rc = allow_dynamic_smem((const void*)kern, (int)smem))) return rc;
-  if ((rc = launch_pdl(kern, dim3((unsigned)grid), dim3(kThreads), smem, stream, 1, p))) return rc;
-  return launch_pdl(attn_q4_combine_kernel, dim3((unsigned)grid), dim3(1024), (size_t)grid * G * sizeof(float2), stream, 1, p, (int)head_dim);
+  if ((rc = launch_pdl(kern, dim3((unsigned)grid), dim3(kWarps * 32), smem, stream, 1, p))) return rc;
+  return launch_pdl(head_dim == 128 ? attn_q4_combine_kernel<128> : attn_q4_combine_kernel<64>,
+                    dim3((unsigned)grid, (unsigned)G), dim3((unsigned)(kSlices * head_dim / 4)), 0, stream, 1, p);
 }
 
 }  // namespace glacier
