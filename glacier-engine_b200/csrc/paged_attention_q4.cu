@@ -31,6 +31,7 @@ namespace {
 constexpr int kMaxLanes = 1024;
 constexpr int kWarps = 8;   // two per SM partition
 constexpr int kStages = 4;  // stages in a warp's ring: 147 KB of K/V per SM, three quarters of it in flight
+constexpr int kClusterCtas = 8;
 // Pages per stage: 4608 bytes at either head size.
 template <int HD>
 constexpr int kStagePages = HD == 128 ? 2 : 4;
@@ -388,12 +389,78 @@ __device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ct
   }
 }
 
+// The states of a cluster's warps to the pair's output: warp g merges head g over the CTA's
+// warps, then rank g merges it over the CTAs.  A pair of context 0 has no state and gets zeros.
+template <int HD>
+__device__ __forceinline__ void merge_cluster(const AttnQ4Params& p, uint8_t* smem, const float* state_a,
+                                              const float (*ml)[8][2], const int* s_state, int warp, int lane, int G) {
+  constexpr int ROW = HD + 4;
+  static_assert(kClusterCtas == 8 && kWarps == 8, "a warp and a CTA per query head");
+  __syncthreads();  // every state is written, every ring idle
+  float* part = reinterpret_cast<float*>(smem);  // [G][ROW]: o, maximum, sum
+  const int g = warp, d = 4 * (lane % (HD / 4));
+  if (g < G) {
+    float M = -INFINITY, L = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      if (s_state[w]) M = fmaxf(M, ml[w][g][0]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (!s_state[w]) continue;
+      const float x = ml[w][g][0] == -INFINITY ? 0.f : ex2(ml[w][g][0] - M);
+      const float4 y = *reinterpret_cast<const float4*>(state_a + ((size_t)w * G + g) * ROW + d);
+      L = fmaf(ml[w][g][1], x, L);
+      a.x = fmaf(y.x, x, a.x);
+      a.y = fmaf(y.y, x, a.y);
+      a.z = fmaf(y.z, x, a.z);
+      a.w = fmaf(y.w, x, a.w);
+    }
+    if (lane < HD / 4) *reinterpret_cast<float4*>(part + g * ROW + d) = a;
+    if (lane == 0) *reinterpret_cast<float2*>(part + g * ROW + HD) = make_float2(M, L);
+  }
+  cluster_sync_all();  // every CTA's states are visible to the cluster
+  const int rank = (int)cluster_ctarank();
+  if (warp == 0 && rank < G) {
+    const uint32_t local = smem_u32(part + rank * ROW);
+    float m[kClusterCtas], M = -INFINITY, L = 0.f;
+    float4 y[kClusterCtas], a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < kClusterCtas; ++c) {
+      const uint32_t at = mapa_shared(local, c);
+      m[c] = ld_dsmem_f32(at + 4 * HD);
+      y[c] = make_float4(ld_dsmem_f32(at + 4 * d), ld_dsmem_f32(at + 4 * d + 4), ld_dsmem_f32(at + 4 * d + 8),
+                         ld_dsmem_f32(at + 4 * d + 12));
+      M = fmaxf(M, m[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < kClusterCtas; ++c) {
+      const float x = m[c] == -INFINITY ? 0.f : ex2(m[c] - M);
+      L = fmaf(ld_dsmem_f32(mapa_shared(local, c) + 4 * HD + 4), x, L);
+      a.x = fmaf(y[c].x, x, a.x);
+      a.y = fmaf(y[c].y, x, a.y);
+      a.z = fmaf(y[c].z, x, a.z);
+      a.w = fmaf(y[c].w, x, a.w);
+    }
+    const float r = L == 0.f ? 0.f : 8.f / L;
+    const int pair = blockIdx.x / kClusterCtas, hkv = p.num_kv_heads;
+    if (lane < HD / 4)
+      *reinterpret_cast<float4*>(p.out + (size_t)(pair / hkv) * p.ldo + (size_t)((pair % hkv) * G + rank) * HD + d) =
+          make_float4(a.x * r, a.y * r, a.z * r, a.w * r);
+  }
+  cluster_sync_all();  // keep every CTA's shared memory until the ranks have read it
+}
+
 // A warp's share is one run of stages: whole pairs, which it finishes by itself, and at most
 // two pieces of pairs: one that continues a pair begun before it (state A), then one that
 // begins a pair which goes on behind it (state B).  At the end of the CTA the pieces
 // merge in shared memory in stage order; what is cut at the CTA's own ends goes to the
 // combine kernel, at most two partial segments per CTA.
-template <int HD>
+//
+// CLUSTER, for a few pairs of few pages: a cluster of eight CTAs per pair instead, its 64 warps
+// taking even pieces; every piece is a state, the CTAs' states merge over distributed shared memory
+// in rank order, and no combine kernel follows.
+template <int HD, bool CLUSTER>
 __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Params p) {
   constexpr int BLK = 18 * HD, SP = kStagePages<HD>, SPOS = kStagePos<HD>;
   constexpr int NST = kStages, IDS = 32 / SP;
@@ -413,7 +480,22 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
   float* state_a = reinterpret_cast<float*>(smem + (size_t)kWarps * RING);  // [warps][G][ROW]
   PairWalk<HD> use;
   int g0 = 0, g1 = 0;
-  const int Q = find_share<HD>(p, blockIdx.x * kWarps + warp, ctx, use, g0, g1);
+  int Q = 0;
+  if constexpr (CLUSTER) {
+    const int pair = blockIdx.x / kClusterCtas;
+    use.lid = pair / hkv;
+    use.kvh = pair - use.lid * hkv;
+    const int c = min(max(p.ctx_lens[use.lid], 0), p.max_pages * kQ4Page);
+    ctx[use.lid] = c;  // every warp writes the same value
+    use.ns = PairWalk<HD>::stages(c);
+    use.P = 0;
+    const int w = (int)cluster_ctarank() * kWarps + warp;
+    use.sb = g0 = (int)((long long)use.ns * w / (kClusterCtas * kWarps));
+    use.se = g1 = (int)((long long)use.ns * (w + 1) / (kClusterCtas * kWarps));
+    if (use.sb == use.se) use.lid = -1;
+  } else {
+    Q = find_share<HD>(p, blockIdx.x * kWarps + warp, ctx, use, g0, g1);
+  }
   if (lane == 0) s_state[warp] = 0;
   __syncwarp();  // ctx and the state word are this warp's own writes
 
@@ -516,7 +598,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
       float l = l2.x + l2.y;
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
-      const bool begins = done.sb == 0, ends = done.se == done.ns;
+      const bool begins = !CLUSTER && done.sb == 0, ends = done.se == done.ns;
       const int which = begins ? 1 : 0;
       // A whole pair goes out; a piece to its state (B only at the share's end, over the idle ring).
       float* d = begins && ends ? p.out + (size_t)done.lid * p.ldo + (size_t)done.kvh * G * HD
@@ -546,6 +628,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
         s_pair[which][warp] = done.lid * hkv + done.kvh;
       }
     }
+  }
+  if constexpr (CLUSTER) {
+    merge_cluster<HD>(p, smem, state_a, s_ml[0], s_state, warp, lane, G);
+    return;
   }
   // Lanes of context 0 get zeros.
   for (int b = blockIdx.x; b < p.lanes; b += gridDim.x)
@@ -682,6 +768,10 @@ __global__ void __launch_bounds__(kSlices * HD / 4) attn_q4_combine_kernel(const
       make_float4(a.x * r, a.y * r, a.z * r, a.w * r);
 }
 
+// The cluster form: at most one cluster per pair at a time on the SMs, and contexts that give a warp
+// few stages.
+constexpr size_t kClusterPairs = 16, kClusterPages = 512;
+
 }  // namespace
 
 // Two partial segments per CTA (one that begins a pair, one that continues it), and the
@@ -733,10 +823,15 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
   p.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   p.bad = ops_error_word();
   GLC_REQUIRE(p.bad, "paged_attention_q4: device status word unavailable");
-  auto kern = head_dim == 128 ? attn_q4_kernel<128> : attn_q4_kernel<64>;
+  const size_t pairs = lanes * num_kv_heads;
+  const bool cluster = pairs <= kClusterPairs && max_pages <= kClusterPages;
+  auto kern = head_dim == 128 ? (cluster ? attn_q4_kernel<128, true> : attn_q4_kernel<128, false>)
+                              : (cluster ? attn_q4_kernel<64, true> : attn_q4_kernel<64, false>);
   const size_t pages = head_dim == 128 ? kStagePages<128> : kStagePages<64>;
   const size_t smem = kWarps * (kStages * pages * q4_block_bytes(head_dim) + G * (head_dim + 4) * sizeof(float));
   if ((rc = allow_dynamic_smem((const void*)kern, (int)smem))) return rc;
+  if (cluster)
+    return launch_pdl(kern, dim3((unsigned)(pairs * kClusterCtas)), dim3(kWarps * 32), smem, stream, kClusterCtas, p);
   if ((rc = launch_pdl(kern, dim3((unsigned)grid), dim3(kWarps * 32), smem, stream, 1, p))) return rc;
   return launch_pdl(head_dim == 128 ? attn_q4_combine_kernel<128> : attn_q4_combine_kernel<64>,
                     dim3((unsigned)grid, (unsigned)G), dim3((unsigned)(kSlices * head_dim / 4)), 0, stream, 1, p);

@@ -200,7 +200,8 @@ def check(rc: int) -> int:
 
 
 def call(name: str, *args) -> int:
-    return check(getattr(lib(), name)(*args))
+    rc = getattr(_lib or lib(), name)(*args)
+    return check(rc) if rc else rc
 
 
 def handle(ptr):
