@@ -29,6 +29,7 @@
 #include <thread>
 #include <vector>
 
+#include "kv_q4.cuh"
 #include "persistent.cuh"
 
 namespace glacier {
@@ -54,6 +55,16 @@ int paged_attention(const float* q, size_t ldq, const float* pool, size_t page_f
                     size_t num_heads, size_t num_kv_heads, size_t head_dim, float* out, size_t ldo, float* workspace,
                     size_t workspace_floats, int chunk, cudaStream_t stream, SplitOut so = SplitOut(),
                     StepProfiler* prof = nullptr, int combine_kind = -1);
+int qkv_rope_append_q4(const float* qkv, size_t ld, size_t split_stride, int nsplit, const float* bias,
+                       const float* cos_t, const float* sin_t, size_t positions, const int32_t* pos,
+                       const int64_t* slots, size_t batch, size_t num_heads, size_t num_kv_heads, size_t head_dim,
+                       float* q_out, size_t ldq, void* pool, size_t num_pages, size_t num_layers, size_t layer,
+                       cudaStream_t stream);
+size_t attention_q4_workspace_floats(size_t num_heads, size_t num_kv_heads, size_t head_dim);
+int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_pages, size_t num_layers,
+                       const int32_t* block_tables, size_t max_pages, const int32_t* ctx_lens, size_t lanes,
+                       size_t layer, size_t num_heads, size_t num_kv_heads, size_t head_dim, float* out, size_t ldo,
+                       float* workspace, size_t workspace_floats, cudaStream_t stream);
 size_t argmax_workspace_bytes(size_t batch, size_t n);
 int argmax_rows(const float* logits, size_t ld, size_t batch, size_t n, const uint64_t* words, size_t word_count,
                 glacier_argmax_result* out, int32_t* tokens, int32_t* status, void* workspace, size_t ws_bytes,
@@ -149,6 +160,23 @@ __global__ void ctx_from_pos_kernel(const int32_t* __restrict__ pos, int32_t* __
     return;
   }
   ctx[i] = (i % groups == index) ? p + 1 : 0;
+}
+
+// The same for a 4-bit pool, with the cache position (page * 16 + row) that every layer's append
+// writes for the lane: -1 for an idle lane (position -1), -2 for a position that nothing can be
+// written for (the append raises the bad-input word).
+__global__ void ctx_slots_from_pos_kernel(const int32_t* __restrict__ pos, const int32_t* __restrict__ tables,
+                                          int max_pages, int32_t* __restrict__ ctx, int64_t* __restrict__ slots, int n,
+                                          int groups, int index, int limit) {
+  griddep_launch();
+  griddep_wait();
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int p = pos[i];
+  const bool in = p >= 0 && p < limit;
+  const int page = in ? tables[(size_t)i * max_pages + p / kQ4Page] : -1;
+  ctx[i] = in && i % groups == index ? p + 1 : 0;
+  slots[i] = p == -1 ? -1 : page < 0 ? -2 : (int64_t)page * kQ4Page + p % kQ4Page;
 }
 
 struct DevBuf {
@@ -441,7 +469,7 @@ struct glacier_cuda_model {
   bool emb_loaded = false, emb_f32 = false, final_loaded = false, finalized = false;
   // Reserved step workspace.
   size_t max_lanes = 0, max_pages = 0;
-  DevBuf x, hn, qkv, q, attn, proj, gu, act, down, logits, ctx, att_ws, arg_ws, status;
+  DevBuf x, hn, qkv, q, attn, proj, gu, act, down, logits, ctx, slots, att_ws, arg_ws, status;
   // GEMV-mode LM head with the eligible argmax in its epilogue: per-tile winners.
   DevBuf lm_arg;
   size_t att_floats = 0, arg_bytes = 0;
@@ -469,7 +497,8 @@ struct glacier_cuda_model {
 };
 
 struct glacier_cuda_kv {
-  size_t num_pages = 0, page_floats = 0;
+  size_t num_pages = 0, page_floats = 0, page_bytes = 0;
+  bool q4 = false;  // 4-bit pages (kv_q4.cuh); page_floats is 0
   DevBuf pool;
 };
 
@@ -764,14 +793,16 @@ int glacier_cuda_model_reserve(glacier_cuda_model* m, size_t max_lanes, size_t m
   const size_t L = max_lanes;
   m->att_segs = attention_segments(L, c.num_heads, c.head_dim, max_pages * 16);
   const size_t nsplit = (size_t)m->att_segs;
-  m->att_floats = attention_workspace_floats(L, c.num_heads, c.head_dim, nsplit);
+  // A step may run on a pool of either form.
+  m->att_floats = std::max(attention_workspace_floats(L, c.num_heads, c.head_dim, nsplit),
+                           attention_q4_workspace_floats(c.num_heads, c.num_kv_heads, c.head_dim));
   m->arg_bytes = argmax_workspace_bytes(L, c.vocab);
   if ((rc = m->x.alloc(L * c.dim * 4)) || (rc = m->hn.alloc(L * c.dim * 4)) ||
       (rc = m->qkv.alloc(L * m->qkv_dim * 4)) || (rc = m->q.alloc(L * m->q_dim * 4)) ||
       (rc = m->attn.alloc(L * m->q_dim * 4)) || (rc = m->proj.alloc(L * c.dim * 4)) ||
       (rc = m->gu.alloc(L * 2 * (size_t)c.hidden * 4)) || (rc = m->act.alloc(L * (size_t)c.hidden * 4)) ||
       (rc = m->down.alloc(L * c.dim * 4)) || (rc = m->logits.alloc(L * (size_t)c.vocab * 4)) ||
-      (rc = m->ctx.alloc(L * 4)) || (rc = m->att_ws.alloc(m->att_floats * 4)) ||
+      (rc = m->ctx.alloc(L * 4)) || (rc = m->slots.alloc(L * 8)) || (rc = m->att_ws.alloc(m->att_floats * 4)) ||
       (rc = m->arg_ws.alloc(m->arg_bytes)) || (rc = m->status.alloc(L * 4)) || (rc = m->pf_pos.alloc(L * 4)) ||
       (rc = m->pf_bt.alloc(L * max_pages * 4)) || (rc = m->lm_arg.alloc(argmax_records_bytes(L, c.vocab))))
     return rc;
@@ -842,7 +873,8 @@ glacier_cuda_kv* glacier_cuda_kv_create(const glacier_cuda_model* m, size_t num_
   kv->num_pages = num_pages;
   // One page = 16 positions of K and V for every layer (paged_kv_cache.zig:1-16).
   kv->page_floats = (size_t)m->cfg.num_layers * 2 * 16 * m->kv_dim;
-  if (kv->pool.alloc(num_pages * kv->page_floats * 4)) return nullptr;
+  kv->page_bytes = kv->page_floats * 4;
+  if (kv->pool.alloc(num_pages * kv->page_bytes)) return nullptr;
   if (cudaMemset(kv->pool.p, 0, kv->pool.bytes) != cudaSuccess) {
     set_error(GLACIER_CUDA_ECUDA, "kv_create: memset failed");
     return nullptr;
@@ -850,9 +882,36 @@ glacier_cuda_kv* glacier_cuda_kv_create(const glacier_cuda_model* m, size_t num_
   return kv.release();
 }
 
+glacier_cuda_kv* glacier_cuda_kv_create_q4(const glacier_cuda_model* m, size_t num_pages) {
+  if (!m || num_pages == 0) {
+    set_error(GLACIER_CUDA_EINVAL, "kv_create_q4: null model or zero pages");
+    return nullptr;
+  }
+  const auto& c = m->cfg;
+  // 16 stands for the pool's address, which is not there yet.
+  if (q4_check_pool("kv_create_q4", (const void*)16, num_pages, c.num_layers, 0, c.num_heads, c.num_kv_heads,
+                    c.head_dim) ||
+      bind_device(m))
+    return nullptr;
+  auto kv = std::make_unique<glacier_cuda_kv>();
+  kv->num_pages = num_pages;
+  kv->q4 = true;
+  kv->page_bytes = (size_t)c.num_layers * c.num_kv_heads * q4_block_bytes(c.head_dim);
+  if (kv->pool.alloc(num_pages * kv->page_bytes)) return nullptr;
+  if (cudaMemset(kv->pool.p, 0, kv->pool.bytes) != cudaSuccess) {
+    set_error(GLACIER_CUDA_ECUDA, "kv_create_q4: memset failed");
+    return nullptr;
+  }
+  return kv.release();
+}
+
 void glacier_cuda_kv_destroy(glacier_cuda_kv* kv) { delete kv; }
 
-float* glacier_cuda_kv_pages(glacier_cuda_kv* kv) { return kv ? kv->pool.as<float>() : nullptr; }
+float* glacier_cuda_kv_pages(glacier_cuda_kv* kv) { return kv && !kv->q4 ? kv->pool.as<float>() : nullptr; }
+
+void* glacier_cuda_kv_q4_pages(glacier_cuda_kv* kv) { return kv && kv->q4 ? kv->pool.p : nullptr; }
+
+size_t glacier_cuda_kv_page_bytes(const glacier_cuda_kv* kv) { return kv ? kv->page_bytes : 0; }
 
 size_t glacier_cuda_kv_page_floats(const glacier_cuda_kv* kv) { return kv ? kv->page_floats : 0; }
 
@@ -871,7 +930,7 @@ static int step_impl(glacier_cuda_model* m, glacier_cuda_kv* kv, size_t lanes, c
   const size_t max_ctx = max_pages * 16;
   int rc;
   // One lane, greedy step, one GPU: the persistent kernel runs the whole step.
-  if (m->ps && m->persistent && head == kHeadAllRows && lanes == 1 && !m->tp_comm)
+  if (m->ps && m->persistent && head == kHeadAllRows && lanes == 1 && !m->tp_comm && !kv->q4)
     return persist_step(m->ps, lanes, tokens, positions, block_tables, max_pages, kv->pool.as<float>(),
                         kv->page_floats, m->prof.on, eligible, eligible_words, tokens_out,
                         status_out ? status_out : m->status.as<int32_t>(), logits_out, st);
@@ -883,10 +942,14 @@ static int step_impl(glacier_cuda_model* m, glacier_cuda_kv* kv, size_t lanes, c
   };
   mark(GLACIER_CUDA_STEP_EMBED);
   const int pos_limit = (int)std::min<size_t>(max_ctx, c.max_positions);
-  if ((rc = launch_pdl(ctx_from_pos_kernel, dim3((unsigned)ceil_div(B, 128)), dim3(128), 0, st, 1, positions,
-                       m->ctx.as<int32_t>(), (int)B, m->tp_lane_groups, m->tp_lane_index, pos_limit,
-                       ops_error_word())))
-    return rc;
+  if (kv->q4)
+    rc = launch_pdl(ctx_slots_from_pos_kernel, dim3((unsigned)ceil_div(B, 128)), dim3(128), 0, st, 1, positions,
+                    block_tables, (int)max_pages, m->ctx.as<int32_t>(), m->slots.as<int64_t>(), (int)B,
+                    m->tp_lane_groups, m->tp_lane_index, pos_limit);
+  else
+    rc = launch_pdl(ctx_from_pos_kernel, dim3((unsigned)ceil_div(B, 128)), dim3(128), 0, st, 1, positions,
+                    m->ctx.as<int32_t>(), (int)B, m->tp_lane_groups, m->tp_lane_index, pos_limit, ops_error_word());
+  if (rc) return rc;
   int32_t* st_out = status_out ? status_out : m->status.as<int32_t>();
   // The LM head's epilogue picks the tokens (no argmax pass over the logits,
   // which are written only when the caller asks for them).
@@ -940,17 +1003,35 @@ static int step_impl(glacier_cuda_model* m, glacier_cuda_kv* kv, size_t lanes, c
     mark(GLACIER_CUDA_STEP_PROJ_QKV);
     if ((rc = project(L.qkv.w, hn, D, so_d, m->map_d, m->qkv.as<float>(), m->qkv_dim, sq))) return rc;
     mark(GLACIER_CUDA_STEP_ROPE_APPEND);
-    if ((rc = qkv_rope_append(m->qkv.as<float>(), m->qkv_dim, B * m->qkv_dim, sq, L.bqkv.as<float>(),
-                              m->rope_cos.as<float>(), m->rope_sin.as<float>(), c.max_positions, positions, B,
-                              c.num_heads, c.num_kv_heads, c.head_dim, m->q.as<float>(), m->q_dim,
-                              kv->pool.as<float>(), kv->page_floats, block_tables, max_pages, l, st)))
-      return rc;
-    mark(GLACIER_CUDA_STEP_ATTENTION);
-    if ((rc = paged_attention(m->q.as<float>(), m->q_dim, kv->pool.as<float>(), kv->page_floats, block_tables,
-                              max_pages, m->ctx.as<int32_t>(), max_ctx, B, l, c.num_heads, c.num_kv_heads, c.head_dim,
-                              m->gemm ? nullptr : m->attn.as<float>(), m->q_dim, m->att_ws.as<float>(), m->att_floats,
-                              m->att_segs, st, so_q, prof, GLACIER_CUDA_STEP_ATTN_COMBINE)))
-      return rc;
+    if (kv->q4) {
+      if ((rc = qkv_rope_append_q4(m->qkv.as<float>(), m->qkv_dim, B * m->qkv_dim, sq, L.bqkv.as<float>(),
+                                   m->rope_cos.as<float>(), m->rope_sin.as<float>(), c.max_positions, positions,
+                                   m->slots.as<int64_t>(), B, c.num_heads, c.num_kv_heads, c.head_dim,
+                                   m->q.as<float>(), m->q_dim, kv->pool.p, kv->num_pages, c.num_layers, l, st)))
+        return rc;
+      mark(GLACIER_CUDA_STEP_ATTENTION);
+      if ((rc = paged_attention_q4(m->q.as<float>(), m->q_dim, kv->pool.p, kv->num_pages, c.num_layers, block_tables,
+                                   max_pages, m->ctx.as<int32_t>(), B, l, c.num_heads, c.num_kv_heads, c.head_dim,
+                                   m->attn.as<float>(), m->q_dim, m->att_ws.as<float>(), m->att_floats, st)))
+        return rc;
+      if (m->gemm) {
+        mark(GLACIER_CUDA_STEP_ATTN_COMBINE);
+        if ((rc = split_activation(m->attn.as<float>(), m->q_dim, B, m->q_dim, m->np, so_q.xs, so_q.xscale, st)))
+          return rc;
+      }
+    } else {
+      if ((rc = qkv_rope_append(m->qkv.as<float>(), m->qkv_dim, B * m->qkv_dim, sq, L.bqkv.as<float>(),
+                                m->rope_cos.as<float>(), m->rope_sin.as<float>(), c.max_positions, positions, B,
+                                c.num_heads, c.num_kv_heads, c.head_dim, m->q.as<float>(), m->q_dim,
+                                kv->pool.as<float>(), kv->page_floats, block_tables, max_pages, l, st)))
+        return rc;
+      mark(GLACIER_CUDA_STEP_ATTENTION);
+      if ((rc = paged_attention(m->q.as<float>(), m->q_dim, kv->pool.as<float>(), kv->page_floats, block_tables,
+                                max_pages, m->ctx.as<int32_t>(), max_ctx, B, l, c.num_heads, c.num_kv_heads,
+                                c.head_dim, m->gemm ? nullptr : m->attn.as<float>(), m->q_dim, m->att_ws.as<float>(),
+                                m->att_floats, m->att_segs, st, so_q, prof, GLACIER_CUDA_STEP_ATTN_COMBINE)))
+        return rc;
+    }
     mark(GLACIER_CUDA_STEP_PROJ_O);
     if ((rc = project(L.o.w, m->attn.as<float>(), m->q_dim, so_q, m->map_q, m->proj.as<float>(), D, so_gemm)))
       return rc;

@@ -247,8 +247,9 @@ int kv_resize(int32_t* lens, const int32_t* targets, size_t lanes, int32_t* bloc
   if (!given)  // pages only, and how many is known on the device alone: threads for all that there can be
     return launch_pdl(kv_resize_kernel<true, true>, dim3(1),
                       dim3(std::max(lane_threads, lanes * max_pages > 1024 ? 1024u : 256u)), 0, stream, 1, p);
-  // One CTA's threads at four rows each: more are worth a second launch (64 lanes: 2.9 against 5.0 us
-  // at 4096 rows, 18 against 6.5 at 65536).
+  // One CTA's threads at four rows each: from there on a second launch pays (64 lanes grown from
+  // nothing and released again: 8.4 us in one CTA against 10.0 in two launches at 2048 rows, 10.0 and 9.9
+  // at 4096, 12.8 and 10.0 at 8192, 48 and 12.5 at 65536).
   if (rows <= 4 * kMaxLanes) {
     const unsigned threads = std::max({128u, lane_threads, std::min(1024u, (unsigned)ceil_div(rows, (size_t)128) * 32)});
     return launch_pdl(kv_resize_kernel<true, true>, dim3(1), dim3(threads), 0, stream, 1, p);

@@ -103,7 +103,10 @@ SIGNATURES = {
     "glacier_cuda_model_finalize": ([vp], i32),
     "glacier_cuda_model_reserve": ([vp, sz, sz], i32),
     "glacier_cuda_kv_create": ([vp, sz], vp),
+    "glacier_cuda_kv_create_q4": ([vp, sz], vp),
     "glacier_cuda_kv_destroy": ([vp], None),
+    "glacier_cuda_kv_q4_pages": ([vp], vp),
+    "glacier_cuda_kv_page_bytes": ([vp], sz),
     "glacier_cuda_kv_pages": ([vp], vp),
     "glacier_cuda_kv_page_floats": ([vp], sz),
     "glacier_cuda_decode_step": ([vp, vp, sz, vp, vp, vp, sz, vp, sz, vp, vp, vp, vp], i32),

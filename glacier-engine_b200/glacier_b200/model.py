@@ -312,37 +312,95 @@ class DecodeSession:
     Lane b owns pages [b*max_pages, (b+1)*max_pages) of one KV pool (the
     reference's per-request page table, paged_kv_cache.zig:44-48); torch only
     provides device memory and the stream.
+
+    ``kv_format`` "q4" holds the cache in 4 bits (glacier_cuda_kv_create_q4), in 9/64 of the bytes.
+
+    ``pool_pages`` makes the lanes share a pool of that many pages instead: block tables, lengths and
+    the free list live on the device, and glacier_cuda_kv_resize moves pages between them.  ``step``
+    then grows every active lane by one position and takes the positions from there (a lane that
+    gets no page has position -1 and ``grow_status`` GLACIER_CUDA_ENOMEM), ``prefill`` appends to a
+    lane, and ``resize`` sets lengths (0 ends a request).
     """
 
-    def __init__(self, dm: DeviceModel, lanes: int, max_pages: int, reserve_lanes: int | None = None):
+    def __init__(self, dm: DeviceModel, lanes: int, max_pages: int, reserve_lanes: int | None = None,
+                 kv_format: str = "f32", pool_pages: int | None = None):
         import torch
         self.torch = torch
         self.dm, self.lanes, self.max_pages = dm, lanes, max_pages
+        if kv_format not in ("f32", "q4"):
+            raise ValueError(f"kv_format {kv_format!r}: 'f32' or 'q4'")
+        self.kv_format = kv_format
+        self.num_pages = lanes * max_pages if pool_pages is None else pool_pages
         L = _lib.lib()
         _lib.call("glacier_cuda_model_reserve", dm.h, reserve_lanes or lanes, max_pages)
-        self.kv = _lib.handle(L.glacier_cuda_kv_create(dm.h, lanes * max_pages))
+        create = L.glacier_cuda_kv_create_q4 if kv_format == "q4" else L.glacier_cuda_kv_create
+        self.kv = _lib.handle(create(dm.h, self.num_pages))
         self.page_floats = L.glacier_cuda_kv_page_floats(self.kv)
+        self.page_bytes = L.glacier_cuda_kv_page_bytes(self.kv)
         dev = torch.device("cuda", torch.cuda.current_device())
-        self.block_tables = torch.arange(lanes * max_pages, dtype=torch.int32, device=dev).reshape(lanes, max_pages)
-        self.tokens = torch.zeros(lanes, dtype=torch.int32, device=dev)
-        self.positions = torch.zeros(lanes, dtype=torch.int32, device=dev)
-        self.out = torch.zeros(lanes, dtype=torch.int32, device=dev)
-        self.status = torch.zeros(lanes, dtype=torch.int32, device=dev)
+        i32 = dict(dtype=torch.int32, device=dev)
+        self.shared = pool_pages is not None
+        if self.shared:
+            self.block_tables = torch.full((lanes, max_pages), -1, **i32)
+            self.lens = torch.zeros(lanes, **i32)
+            self.targets = torch.zeros(lanes, **i32)
+            self.active = torch.ones(lanes, **i32)  # lanes that step() grows
+            self.free_pages = torch.arange(self.num_pages - 1, -1, -1, **i32)  # page 0 comes off first
+            self.free_count = torch.full((1,), self.num_pages, **i32)
+            self.grow_status = torch.zeros(lanes, **i32)
+            self._row_lanes = torch.empty(lanes, **i32)
+            self._slots = torch.empty(lanes, dtype=torch.int64, device=dev)
+        else:
+            self.block_tables = torch.arange(lanes * max_pages, **i32).reshape(lanes, max_pages)
+        self.tokens = torch.zeros(lanes, **i32)
+        self.positions = torch.zeros(lanes, **i32)
+        self.out = torch.zeros(lanes, **i32)
+        self.status = torch.zeros(lanes, **i32)
 
     def pages(self):
-        """The KV pool as a torch view [num_pages, page_floats] (device memory of the library)."""
-        ptr = _lib.lib().glacier_cuda_kv_pages(self.kv)
-        n = self.lanes * self.max_pages * self.page_floats
-        return _ptr_tensor(self.torch, ptr, n).view(self.lanes * self.max_pages, self.page_floats)
+        """The KV pool as a torch view (device memory of the library): float32 [num_pages, page_floats],
+        or uint8 [num_pages, page_bytes] of a 4-bit pool."""
+        L = _lib.lib()
+        if self.kv_format == "q4":
+            n = self.num_pages * self.page_bytes
+            return _ptr_tensor(self.torch, L.glacier_cuda_kv_q4_pages(self.kv), n, "|u1").view(self.num_pages, -1)
+        n = self.num_pages * self.page_floats
+        return _ptr_tensor(self.torch, L.glacier_cuda_kv_pages(self.kv), n).view(self.num_pages, self.page_floats)
+
+    def resize(self, targets, stream=None):
+        """Shared pool: brings the lanes to `targets` positions (host sequence or device int32 tensor); returns
+        the device statuses (0, or why a lane was left as it was)."""
+        from . import ops
+        if not self.shared:
+            raise ValueError("resize needs a session with pool_pages")
+        s = stream if stream is not None else self.torch.cuda.current_stream()
+        with self.torch.cuda.stream(s):
+            self.targets.copy_(self.torch.as_tensor(targets, dtype=self.torch.int32))
+        ops.kv_resize(self.lens, self.targets, self.block_tables, self.free_pages, self.free_count, self.grow_status,
+                      stream=stream)
+        return self.grow_status
+
+    def _grow(self, s):
+        """Shared pool: one position more for every active lane; their positions, -1 for the others."""
+        from . import ops
+        with self.torch.cuda.stream(s):
+            self.torch.add(self.lens, self.active, out=self.targets)
+        ops.kv_resize(self.lens, self.targets, self.block_tables, self.free_pages, self.free_count, self.grow_status,
+                      positions=self.positions, row_lanes=self._row_lanes, slots=self._slots, row_stride=1, stream=s)
 
     def step(self, tokens=None, positions=None, eligible=None, logits=None, stream=None):
-        """One decode step on device tensors already in self.tokens / self.positions."""
+        """One decode step on device tensors already in self.tokens / self.positions (with a shared pool the
+        positions come from the lanes' lengths)."""
         torch = self.torch
         if tokens is not None:
             self.tokens.copy_(torch.as_tensor(tokens, dtype=torch.int32))
         if positions is not None:
+            if self.shared:
+                raise ValueError("a session with pool_pages keeps its own positions")
             self.positions.copy_(torch.as_tensor(positions, dtype=torch.int32))
         s = stream if stream is not None else torch.cuda.current_stream()
+        if self.shared:
+            self._grow(s)
         words = 0 if eligible is None else eligible.shape[-1]
         _lib.call("glacier_cuda_decode_step", self.dm.h, self.kv, self.lanes, self.tokens.data_ptr(),
                   self.positions.data_ptr(), self.block_tables.data_ptr(), self.max_pages,
@@ -361,7 +419,8 @@ class DecodeSession:
         with torch.cuda.graph(self._graph, stream=s):
             out = self.step(stream=s)
             self.tokens.copy_(out)
-            self.positions.add_(1)
+            if not self.shared:
+                self.positions.add_(1)
         return self._graph
 
     def replay_greedy_step(self):
@@ -372,10 +431,20 @@ class DecodeSession:
     def prefill(self, prompt, lane: int = 0, start: int = 0, eligible=None, logits=None, stream=None):
         """Feeds prompt tokens (host sequence or device int32 tensor) of one request at positions
         start.. through lane `lane`'s block table; returns the device int32 tensor [1] holding
-        the greedy token that follows (generate.zig prompt loop, batched)."""
+        the greedy token that follows (generate.zig prompt loop, batched).  With a shared pool the prompt goes
+        behind the lane's positions, whose pages it takes first (MemoryError when there are not enough)."""
         torch = self.torch
         dev = self.tokens.device
         toks = torch.as_tensor(prompt, dtype=torch.int32).to(dev).contiguous()
+        if self.shared:
+            lens = self.lens.tolist()
+            start = lens[lane]
+            lens[lane] += toks.numel()
+            status = self.resize(lens, stream=stream)
+            if stream is not None:
+                stream.synchronize()
+            if int(status[lane]) != 0:
+                raise MemoryError(f"no pages for {toks.numel()} more positions of lane {lane}")
         out = torch.empty(1, dtype=torch.int32, device=dev)
         status = torch.empty(1, dtype=torch.int32, device=dev)
         s = stream if stream is not None else torch.cuda.current_stream()
@@ -400,13 +469,13 @@ class DecodeSession:
             pass
 
 
-def _ptr_tensor(torch, ptr: int, numel: int):
-    """A float32 torch view of library-owned device memory (no copy, no ownership)."""
+def _ptr_tensor(torch, ptr: int, numel: int, typestr: str = "<f4"):
+    """A torch view (float32 by default) of library-owned device memory (no copy, no ownership)."""
 
     class _Holder:
         pass
 
     h = _Holder()
-    h.__cuda_array_interface__ = {"shape": (numel,), "typestr": "<f4", "data": (ptr, False), "version": 3,
+    h.__cuda_array_interface__ = {"shape": (numel,), "typestr": typestr, "data": (ptr, False), "version": 3,
                                   "strides": None}
     return torch.as_tensor(h, device="cuda")

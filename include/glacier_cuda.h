@@ -346,9 +346,14 @@ int glacier_cuda_model_reserve(glacier_cuda_model *model, size_t max_lanes, size
 /* FP32 paged KV pool: num_pages pages of [num_layers][K|V][16][kv_dim] floats
  * (src/paged_kv_cache.zig:1421-1442), so host checkpoint / restore copies pages verbatim. */
 glacier_cuda_kv *glacier_cuda_kv_create(const glacier_cuda_model *model, size_t num_pages);
+/* A pool of 4-bit pages (section (f)), for the same steps: a page takes 9/64 of the FP32 bytes.
+ * NULL for a head geometry outside the 4-bit kernels' contract. */
+glacier_cuda_kv *glacier_cuda_kv_create_q4(const glacier_cuda_model *model, size_t num_pages);
 void glacier_cuda_kv_destroy(glacier_cuda_kv *kv);
-float *glacier_cuda_kv_pages(glacier_cuda_kv *kv);
-size_t glacier_cuda_kv_page_floats(const glacier_cuda_kv *kv);
+float *glacier_cuda_kv_pages(glacier_cuda_kv *kv);                /* NULL for a 4-bit pool */
+void *glacier_cuda_kv_q4_pages(glacier_cuda_kv *kv);              /* NULL for an FP32 pool */
+size_t glacier_cuda_kv_page_floats(const glacier_cuda_kv *kv);    /* 0 for a 4-bit pool */
+size_t glacier_cuda_kv_page_bytes(const glacier_cuda_kv *kv);     /* of either */
 
 /* One greedy decode step for `lanes` independent requests (device buffers): lane b feeds
  * tokens[b] at position positions[b] (its K/V row is written there; context = positions[b]+1)
@@ -358,7 +363,8 @@ size_t glacier_cuda_kv_page_floats(const glacier_cuda_kv *kv);
  * With 4 lanes or fewer the eligible argmax runs in the LM head's epilogue (logitless greedy,
  * int4_neon.c:1075-1254): logits are written only to a given logits_out.  A position outside
  * the RoPE table or past the block table gives that lane context 0, writes no K/V and raises
- * the bad-input device status (glacier_cuda_device_status = 2). */
+ * the bad-input device status (glacier_cuda_device_status = 2).  With a 4-bit pool, position -1 is
+ * an idle lane: context 0 and no K/V without the status, and its token means nothing. */
 int glacier_cuda_decode_step(glacier_cuda_model *model, glacier_cuda_kv *kv, size_t lanes,
                              const int32_t *tokens, const int32_t *positions, const int32_t *block_tables,
                              size_t max_pages, const uint64_t *eligible, size_t eligible_words,

@@ -1,0 +1,227 @@
+"""Decoding with the KV cache held in 4 bits: the model's steps over a 4-bit pool, its own pages or a
+pool shared through kv_resize.
+
+The twin computes each token with the CPU oracle's operators, in float32, but attends the K and V rows
+that the GPU holds (read back with kv_q4_read), in 64 bits.  So a code that rounds the other way
+because a projection's last bit differs moves both sides, and the logits are held to the decode steps' own
+tolerance.  The held rows themselves are held to the rows that the twin computes: half a quantisation step,
+and 2 % of one for the projections' rounding (1e-4 of a row's largest value, whose step is a seventh)."""
+import numpy as np
+import pytest
+
+import oracle
+from helpers import DECODE_LOGIT_TOL, max_err_vs_row_max
+from test_kv_q4 import attend64, scale_of, status_word
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def held_rows(sess, layer, lane, n):
+    from glacier_b200 import ops
+    c = sess.dm.cfg
+    p = torch.arange(n, device="cuda")
+    slots = sess.block_tables[lane].long()[p // 16] * 16 + p % 16
+    k, v = ops.kv_q4_read(sess.pages(), slots, c["num_layers"], layer, c["num_kv_heads"], c["head_dim"])
+    return k.cpu().numpy().astype(np.float64), v.cpu().numpy().astype(np.float64)
+
+
+def check_held(held, row):
+    for h, x in zip(held.reshape(-1, 32), np.asarray(row, np.float64).reshape(-1, 32)):
+        assert np.abs(h - x).max() <= 0.52 * scale_of(np.abs(x).max()) + 1e-12
+
+
+def twin(m, sess, lane, token, pos, cos, sin):
+    """Logits of `token` at `pos`, attending the rows that the session holds for the lane."""
+    c = m.cfg
+    D, F, H, Hkv, hd = c["dim"], c["hidden"], c["num_heads"], c["num_kv_heads"], c["head_dim"]
+    qd, kvd, eps, G = H * hd, Hkv * hd, c["eps"], c["num_heads"] // c["num_kv_heads"]
+    x = m.embedding[token].astype(np.float32)
+    for i, L in enumerate(m.layers):
+        h = oracle.rmsnorm(x, L["input_norm"], eps)
+        q = oracle.linear_int4(h, *L["wq"], qd, D, 32)[0] + L["bq"]
+        k = oracle.linear_int4(h, *L["wk"], kvd, D, 32)[0] + L["bk"]
+        v = oracle.linear_int4(h, *L["wv"], kvd, D, 32)[0] + L["bv"]
+        q = oracle.rope_apply(cos, sin, q, pos, H, hd)
+        k = oracle.rope_apply(cos, sin, k, pos, Hkv, hd)
+        ks, vs = held_rows(sess, i, lane, pos + 1)
+        check_held(ks[pos], k)
+        check_held(vs[pos], v)
+        a = np.concatenate([attend64(q.reshape(H, hd)[j * G:(j + 1) * G], ks[:, j * hd:(j + 1) * hd],
+                                     vs[:, j * hd:(j + 1) * hd]).ravel() for j in range(Hkv)]).astype(np.float32)
+        x = x + oracle.linear_int4(a, *L["wo"], D, qd, 32)[0]
+        h2 = oracle.rmsnorm(x, L["post_attn_norm"], eps)
+        g = oracle.linear_int4(h2, *L["wg"], F, D, 32)[0]
+        u = oracle.linear_int4(h2, *L["wu"], F, D, 32)[0]
+        x = x + oracle.linear_int4(oracle.silu_mul(g, u), *L["wd"], D, F, 32)[0]
+    return oracle.linear_int4(oracle.rmsnorm(x, m.final_norm, eps), *m.lm_head, c["vocab"], D, 32)[0]
+
+
+def make(heads, kv_heads, hd, lanes, max_pages, dim=512, hidden=1024, **session):
+    from glacier_b200.model import DecodeSession, DeviceModel, ModelConfig, SyntheticModel
+    cfg = ModelConfig(num_layers=2, dim=dim, hidden=hidden, num_heads=heads, num_kv_heads=kv_heads, head_dim=hd,
+                      vocab=1000)
+    m = SyntheticModel(cfg, seed=5)
+    dm = DeviceModel(m, max_positions=16 * max_pages)
+    cos, sin = oracle.rope_table(16 * max_pages, hd, cfg.theta)
+    return m, dm, DecodeSession(dm, lanes, max_pages, kv_format="q4", **session), cos, sin
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,lanes", [(8, 2, 64, 3), (28, 4, 128, 2), (28, 4, 128, 6)])
+def test_decode_over_a_4_bit_pool(heads, kv_heads, hd, lanes):
+    """Few lanes (GEMV, the cluster attention) and tensor-core mode (split activations)."""
+    m, dm, sess, cos, sin = make(heads, kv_heads, hd, lanes, 3)
+    logits = torch.empty((lanes, 1000), dtype=torch.float32, device="cuda")
+    cur = np.array([(37 * b + 11) % 1000 for b in range(lanes)], np.int32)
+    for pos in range(19):
+        out = sess.step(tokens=cur, positions=[pos] * lanes, logits=logits).cpu().numpy()
+        if pos in (0, 1, 15, 16, 18):
+            gl = logits.cpu().numpy()
+            for b in range(lanes):
+                assert max_err_vs_row_max(gl[b], twin(m, sess, b, int(cur[b]), pos, cos, sin)) <= DECODE_LOGIT_TOL
+        cur = out.astype(np.int32)
+    assert status_word() == 0
+    sess.close()
+    dm.close()
+
+
+def test_prefill_then_decode():
+    """A prompt in chunks, then steps behind it."""
+    m, dm, sess, cos, sin = make(8, 2, 64, 5, 4, reserve_lanes=8)
+    rng = np.random.default_rng(3)
+    prompts = [rng.integers(0, 1000, n).tolist() for n in (1, 8, 20, 33, 16)]
+    logits = torch.empty(1000, dtype=torch.float32, device="cuda")
+    first = []
+    for b, p in enumerate(prompts):
+        first.append(int(sess.prefill(p, lane=b, logits=logits)[0]))
+        assert max_err_vs_row_max(logits.cpu().numpy(), twin(m, sess, b, p[-1], len(p) - 1, cos, sin)) <= DECODE_LOGIT_TOL
+    step = torch.empty((5, 1000), dtype=torch.float32, device="cuda")
+    pos = [len(p) for p in prompts]
+    sess.step(tokens=first, positions=pos, logits=step)
+    for b in range(5):
+        assert max_err_vs_row_max(step[b].cpu().numpy(), twin(m, sess, b, first[b], pos[b], cos, sin)) <= DECODE_LOGIT_TOL
+    assert status_word() == 0
+    sess.close()
+    dm.close()
+
+
+def test_shared_pool_serves_requests_of_different_lengths():
+    """Lanes grow, end and are admitted again from one pool of pages smaller than lanes * max_pages."""
+    m, dm, sess, cos, sin = make(8, 2, 64, 3, 4, pool_pages=6)
+    rng = np.random.default_rng(4)
+    prompts = [rng.integers(0, 1000, n).tolist() for n in (15, 31, 2)]  # 1 + 2 + 1 pages
+    cur = [int(sess.prefill(p, lane=b)[0]) for b, p in enumerate(prompts)]
+    logits = torch.empty((3, 1000), dtype=torch.float32, device="cuda")
+    for k in range(3):  # lanes 0 and 1 cross a page border: all six pages are out
+        out = sess.step(tokens=cur, logits=logits).cpu().numpy()
+        assert sess.grow_status.tolist() == [0, 0, 0]
+        assert sess.positions.tolist() == [len(p) + k for p in prompts]
+        for b in range(3):
+            ref = twin(m, sess, b, int(cur[b]), len(prompts[b]) + k, cos, sin)
+            assert max_err_vs_row_max(logits[b].cpu().numpy(), ref) <= DECODE_LOGIT_TOL
+        cur = out.tolist()
+    assert int(sess.free_count) == 0
+    with pytest.raises(MemoryError):
+        sess.prefill([1] * 20, lane=2)
+    assert sess.lens.tolist() == [18, 34, 5]
+    sess.resize([18, 0, 5])  # request 1 ends
+    assert int(sess.free_count) == 3
+    new = rng.integers(0, 1000, 33).tolist()
+    cur[1] = int(sess.prefill(new, lane=1)[0])
+    sess.active.copy_(torch.tensor([1, 1, 0]))  # lane 2 waits
+    sess.step(tokens=cur, logits=logits)
+    assert sess.positions.tolist() == [18, 33, -1] and sess.lens.tolist() == [19, 34, 5]
+    for b, pos in ((0, 18), (1, 33)):
+        ref = twin(m, sess, b, int(cur[b]), pos, cos, sin)
+        assert max_err_vs_row_max(logits[b].cpu().numpy(), ref) <= DECODE_LOGIT_TOL
+    tables = sess.block_tables.cpu().numpy()
+    used = [t for b, n in enumerate((19, 34, 5)) for t in tables[b, :-(-n // 16)]]
+    assert len(set(used)) == len(used) == 6
+    assert status_word() == 0  # an idle lane is no error
+    sess.close()
+    dm.close()
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_captured_steps_equal_eager_ones(shared):
+    runs = []
+    for captured in (False, True):
+        more = dict(pool_pages=7) if shared else {}
+        m, dm, sess, cos, sin = make(8, 2, 64, 2, 3, **more)
+        for b in range(2):
+            sess.tokens[b] = int(sess.prefill([3 + b, 9, 27], lane=b)[0])
+        if not shared:
+            sess.positions.fill_(3)
+        toks = []
+        if captured:
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                sess.capture_greedy_step(stream=s)
+                for _ in range(20):
+                    toks.append(sess.replay_greedy_step().clone())
+            s.synchronize()
+        else:
+            for _ in range(20):
+                out = sess.step()
+                toks.append(out.clone())
+                sess.tokens.copy_(out)
+                if not shared:
+                    sess.positions.add_(1)
+        runs.append(torch.stack(toks).cpu().numpy())
+        assert status_word() == 0
+        sess.close()
+        dm.close()
+    np.testing.assert_array_equal(runs[0], runs[1])
+
+
+def test_an_fp32_pool_can_be_shared_too():
+    """kv_resize under FP32 pages: the tokens of a session with its own pages."""
+    from glacier_b200.model import DecodeSession, DeviceModel, ModelConfig, SyntheticModel
+    cfg = ModelConfig(num_layers=2, dim=256, hidden=512, num_heads=8, num_kv_heads=2, head_dim=64, vocab=1000)
+    dm = DeviceModel(SyntheticModel(cfg, seed=7), max_positions=64)
+    got = []
+    for more in ({}, dict(pool_pages=5)):
+        sess = DecodeSession(dm, 2, 4, **more)
+        cur, toks = [int(sess.prefill([5, 6 + b], lane=b)[0]) for b in range(2)], []
+        for k in range(18):
+            cur = sess.step(tokens=cur, positions=None if more else [2 + k] * 2).tolist()
+            toks.append(cur)
+        got.append(toks)
+        sess.close()
+    assert got[0] == got[1]
+    dm.close()
+
+
+def test_refusals():
+    from glacier_b200 import _lib
+    from glacier_b200.model import DecodeSession, DeviceModel, ModelConfig, SyntheticModel
+    cfg = ModelConfig(num_layers=1, dim=256, hidden=512, num_heads=8, num_kv_heads=2, head_dim=32, vocab=100)
+    dm = DeviceModel(SyntheticModel(cfg, seed=7), max_positions=64)
+    with pytest.raises(_lib.GlacierCudaError):
+        DecodeSession(dm, 2, 4, kv_format="q4")  # 32-dim heads
+    with pytest.raises(ValueError):
+        DecodeSession(dm, 2, 4, kv_format="q8")
+    sess = DecodeSession(dm, 2, 4)
+    with pytest.raises(ValueError):
+        sess.resize([1, 1])
+    L = _lib.lib()
+    assert not L.glacier_cuda_kv_create_q4(dm.h, 0) and not L.glacier_cuda_kv_create_q4(None, 4)
+    assert not L.glacier_cuda_kv_q4_pages(sess.kv) and L.glacier_cuda_kv_page_bytes(sess.kv) == 4 * sess.page_floats
+    sess.close()
+    dm.close()
+
+
+def test_a_position_or_page_out_of_range_is_reported():
+    m, dm, sess, cos, sin = make(8, 2, 64, 3, 2)
+    logits = torch.empty((3, 1000), dtype=torch.float32, device="cuda")
+    sess.step(tokens=[1, 2, 3], positions=[0, 32, 0], logits=logits)  # past the table
+    assert status_word() == 2
+    sess.block_tables[2, 0] = -1
+    sess.step(tokens=[1, 2, 3], positions=[1, 0, 0], logits=logits)  # no page
+    assert status_word() == 2
+    for b, pos in ((0, 1), (1, 0)):
+        ref = twin(m, sess, b, b + 1, pos, cos, sin)
+        assert max_err_vs_row_max(logits[b].cpu().numpy(), ref) <= DECODE_LOGIT_TOL
+    sess.close()
+    dm.close()
