@@ -22,6 +22,10 @@
 //     are fp16 numbers (scales have 7 significant bits), so one half FMA is exact.
 // The cache's orders put every operand register's codes in one word of one thread: K's words
 // (t, g) and V's 16-bit units by position pair are the fragments of these instructions.
+#include <algorithm>
+#include <atomic>
+#include <chrono>
+
 #include "kv_q4.cuh"
 
 namespace glacier {
@@ -31,7 +35,7 @@ namespace {
 constexpr int kMaxLanes = 1024;
 constexpr int kWarps = 8;   // two per SM partition
 constexpr int kStages = 4;  // stages in a warp's ring: 147 KB of K/V per SM, three quarters of it in flight
-constexpr int kClusterCtas = 8;
+constexpr int kClusterCtas = 4;
 // Pages per stage: 4608 bytes at either head size.
 template <int HD>
 constexpr int kStagePages = HD == 128 ? 2 : 4;
@@ -46,11 +50,13 @@ struct AttnQ4Params {
   const int32_t* ctx_lens;
   float* out;
   size_t ldo;
-  int32_t* meta;   // [grid][2]: the pair that is cut at the end of CTA c's share (or -1), its segments
+  unsigned long long* tickets;  // [grid]: segments written of the pair that CTA c began and left open
+  unsigned long long nonce;     // marks this launch's tickets: whatever else a ticket holds counts as none
   float* part_ml;  // [2 grid][G][2] maximum (base 2) and sum of a segment
   float* part_o;   // [2 grid][G][hd]
   uint32_t page_bytes;
   int lanes, max_pages, num_pages, layer, num_heads, num_kv_heads;
+  int clusters;  // cluster form: clusters per pair
   float scale_log2;
   int* bad;
 };
@@ -296,34 +302,36 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
   }
 }
 
-// A walk over the pairs of a warp's share [g0, g1) and its segment [sb, se) of each.  The
-// stages of all (lane, kv head) pairs are laid end to end, lane-major, and warp w of the
-// grid takes [w Q, (w + 1) Q): every warp reads the same number of bytes.
+// A walk over the pairs of a warp's share [g0, g1) and its segment [sb, se) of each.  All (lane,
+// kv head) pairs are laid end to end, lane-major, each with a unit for every stage and one in front
+// for the change of pair (it takes about a stage's time), and warp w of the grid takes units
+// [w Q, (w + 1) Q): every warp does the same work.
 template <int HD>
 struct PairWalk {
   int lid, kvh, ns, sb, se;
-  int P;  // the pair's first stage
+  int P;  // the pair's first unit
   __device__ __forceinline__ static int stages(int ctx) { return (ctx + kStagePos<HD> - 1) / kStagePos<HD>; }
+  __device__ __forceinline__ static int units(int ctx) { return ctx > 0 ? stages(ctx) + 1 : 0; }
   __device__ __forceinline__ void set(const int* ctx, int g0, int g1) {
     ns = stages(ctx[lid]);
-    sb = max(0, g0 - P);
-    se = min(ns, g1 - P);
+    sb = max(0, g0 - P - 1);
+    se = min(ns, g1 - P - 1);
   }
-  // False when the share is at its end.
+  // False when the share holds no further stage.
   __device__ __forceinline__ bool next(const int* ctx, int hkv, int g0, int g1) {
-    P += ns;
-    if (P >= g1) return false;
+    P += ns + 1;
+    if (P + 1 >= g1) return false;
     if (++kvh == hkv) {
       kvh = 0;
       do ++lid;
-      while (ctx[lid] == 0);  // a stage before g1 is some lane's
+      while (ctx[lid] == 0);  // a unit before g1 is some lane's
     }
     set(ctx, g0, g1);
     return true;
   }
 };
 
-// Shares of the warps, found by every warp for itself: the sum of all stages, then the lane that
+// Shares of the warps, found by every warp for itself: the sum of all units, then the lane that
 // holds the share's first one.  ctx: clamped contexts, for the block.  Returns Q; start.lid = -1 when
 // the share is empty.  A chunk of 128 lanes is four consecutive ones per thread; the first chunk
 // stays in registers.
@@ -333,14 +341,15 @@ __device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ct
   const int lane = threadIdx.x & 31;
   const int cap = p.max_pages * kQ4Page;
   int ns[4], incl = 0;
-  auto chunk = [&](int b0) {  // stages of lanes b0 + 4 lane ..; incl: running sum over the threads
+  auto chunk = [&](int b0) {  // units of lanes b0 + 4 lane ..; incl: running sum over the threads
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int b = b0 + 4 * lane + i;
       const int c = b < p.lanes ? min(max(p.ctx_lens[b], 0), cap) : 0;
-      if (b < p.lanes) ctx[b] = c;  // every warp writes the same values
-      ns[i] = PairWalk<HD>::stages(c);
+      if (b < p.lanes) ctx[b] = c;  // every warp writes the same values, and reads its own
+      ns[i] = PairWalk<HD>::units(c);
     }
+    __syncwarp();
     incl = ns[0] + ns[1] + ns[2] + ns[3];
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
@@ -377,11 +386,11 @@ __device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ct
         }
       first = __shfl_sync(0xffffffffu, first, src) * p.num_kv_heads;
       start.lid = b0 + 4 * src + __shfl_sync(0xffffffffu, i, src);
-      start.ns = __shfl_sync(0xffffffffu, n, src);
-      start.kvh = (unsigned)(g0 - first) / (unsigned)start.ns;
-      start.P = first + start.kvh * start.ns;
-      start.sb = g0 - start.P;
-      start.se = min(start.ns, g1 - start.P);
+      n = __shfl_sync(0xffffffffu, n, src);
+      start.kvh = (unsigned)(g0 - first) / (unsigned)n;
+      start.P = first + start.kvh * n;
+      start.set(ctx, g0, g1);
+      if (start.se <= start.sb) start.lid = -1;  // the change of pair alone: the next warp begins it
       return Q;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
@@ -389,13 +398,64 @@ __device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ct
   }
 }
 
+// Counts one of `n` arrivals at a ticket; true for the last, which clears it.  A ticket that another
+// launch did not write (any contents of a new workspace) counts as none: 48 bits tell them apart.
+// Only the first arrival needs the compare-and-swap: one per arrival, retried, took 14 us more
+// where 37 CTAs share a pair.
+__device__ __forceinline__ bool last_of(unsigned long long* ticket, unsigned long long nonce, int n) {
+  unsigned long long old = *reinterpret_cast<volatile unsigned long long*>(ticket);
+  bool first = false;
+  if (old >> 16 != nonce) {
+    const unsigned long long was = atomicCAS(ticket, old, nonce << 16 | 1u);
+    first = was == old;
+    old = 0;
+  }
+  if (!first) old = atomicAdd(ticket, 1ull) & 0xffffu;
+  if ((int)old + 1 != n) return false;
+  atomicExch(ticket, 0ull);
+  return true;
+}
+
+// One head of a pair from its n partial segments in order: rows at(s) of part_o and part_ml.
+template <int HD, typename At>
+__device__ __forceinline__ void merge_segments(const AttnQ4Params& p, int pair, int g, int n, int lane, int G, At at) {
+  const int d = 4 * (lane % (HD / 4));
+  float M = -INFINITY, L = 0.f;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = lane; s < n; s += 32) M = fmaxf(M, __ldcg(p.part_ml + at(s) * 2));
+  M = warp_max(M);
+#pragma unroll 8
+  for (int s = 0; s < n; ++s) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + at(s) * HD + d));
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + at(s) * 2));
+    const float x = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+    L = fmaf(ml.y, x, L);
+    a.x = fmaf(v.x, x, a.x);
+    a.y = fmaf(v.y, x, a.y);
+    a.z = fmaf(v.z, x, a.z);
+    a.w = fmaf(v.w, x, a.w);
+  }
+  const float r = L == 0.f ? 0.f : 8.f / L;
+  if (lane < HD / 4)
+    *reinterpret_cast<float4*>(p.out + (size_t)(pair / p.num_kv_heads) * p.ldo +
+                               (size_t)((pair % p.num_kv_heads) * G + g) * HD + d) =
+        make_float4(a.x * r, a.y * r, a.z * r, a.w * r);
+}
+
+// Clusters that a pair of `ns` stages is cut into: two stages per warp at least.
+__device__ __forceinline__ int pair_clusters(int ns, int most) {
+  return min(most, max(1, (ns + 2 * kClusterCtas * kWarps - 1) / (2 * kClusterCtas * kWarps)));
+}
+
 // The states of a cluster's warps to the pair's output: warp g merges head g over the CTA's
-// warps, then rank g merges it over the CTAs.  A pair of context 0 has no state and gets zeros.
+// warps, then one rank merges it over the CTAs, and the last of the pair's clusters to come to
+// head g's ticket merges it over the clusters.  A pair of context 0 has no state and gets zeros.
 template <int HD>
 __device__ __forceinline__ void merge_cluster(const AttnQ4Params& p, uint8_t* smem, const float* state_a,
-                                              const float (*ml)[8][2], const int* s_state, int warp, int lane, int G) {
+                                              const float (*ml)[8][2], const int* s_state, int warp, int lane, int G,
+                                              int pair, int nclusters) {
   constexpr int ROW = HD + 4;
-  static_assert(kClusterCtas == 8 && kWarps == 8, "a warp and a CTA per query head");
+  static_assert(kWarps == 8, "a warp per query head");
   __syncthreads();  // every state is written, every ring idle
   float* part = reinterpret_cast<float*>(smem);  // [G][ROW]: o, maximum, sum
   const int g = warp, d = 4 * (lane % (HD / 4));
@@ -421,8 +481,9 @@ __device__ __forceinline__ void merge_cluster(const AttnQ4Params& p, uint8_t* sm
   }
   cluster_sync_all();  // every CTA's states are visible to the cluster
   const int rank = (int)cluster_ctarank();
-  if (warp == 0 && rank < G) {
-    const uint32_t local = smem_u32(part + rank * ROW);
+  const int head = warp * kClusterCtas + rank;  // heads go to the ranks in turn
+  if (head < G) {
+    const uint32_t local = smem_u32(part + head * ROW);
     float m[kClusterCtas], M = -INFINITY, L = 0.f;
     float4 y[kClusterCtas], a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -442,24 +503,39 @@ __device__ __forceinline__ void merge_cluster(const AttnQ4Params& p, uint8_t* sm
       a.z = fmaf(y[c].z, x, a.z);
       a.w = fmaf(y[c].w, x, a.w);
     }
-    const float r = L == 0.f ? 0.f : 8.f / L;
-    const int pair = blockIdx.x / kClusterCtas, hkv = p.num_kv_heads;
-    if (lane < HD / 4)
-      *reinterpret_cast<float4*>(p.out + (size_t)(pair / hkv) * p.ldo + (size_t)((pair % hkv) * G + rank) * HD + d) =
-          make_float4(a.x * r, a.y * r, a.z * r, a.w * r);
+    const bool whole = nclusters == 1;
+    const int hkv = p.num_kv_heads;
+    const size_t at = (size_t)(blockIdx.x / kClusterCtas) * G + head;
+    const float r = !whole ? 1.f : L == 0.f ? 0.f : 8.f / L;
+    float* dst = whole ? p.out + (size_t)(pair / hkv) * p.ldo + (size_t)((pair % hkv) * G + head) * HD : p.part_o + at * HD;
+    if (lane < HD / 4) *reinterpret_cast<float4*>(dst + d) = make_float4(a.x * r, a.y * r, a.z * r, a.w * r);
+    if (!whole && lane == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
   }
   cluster_sync_all();  // keep every CTA's shared memory until the ranks have read it
+  if (nclusters > 1 && head < G) {
+    __syncwarp();
+    bool last = false;
+    if (lane == 0) {
+      __threadfence();
+      last = last_of(p.tickets + pair * G + head, p.nonce, nclusters);
+      __threadfence();
+    }
+    if (__shfl_sync(0xffffffffu, last, 0))
+      merge_segments<HD>(p, pair, head, nclusters, lane, G,
+                         [&](int s) { return ((size_t)pair * p.clusters + s) * G + head; });
+  }
 }
 
 // A warp's share is one run of stages: whole pairs, which it finishes by itself, and at most
 // two pieces of pairs: one that continues a pair begun before it (state A), then one that
 // begins a pair which goes on behind it (state B).  At the end of the CTA the pieces
-// merge in shared memory in stage order; what is cut at the CTA's own ends goes to the
-// combine kernel, at most two partial segments per CTA.
+// merge in shared memory in stage order.  What is cut at the CTA's own ends is written out, at
+// most two partial segments per CTA, and the CTA that finds itself to be the last of a pair's takes
+// them all together, in order: no second launch, and the result does not depend on which it was.
 //
-// CLUSTER, for a few pairs of few pages: a cluster of eight CTAs per pair instead, its 64 warps
-// taking even pieces; every piece is a state, the CTAs' states merge over distributed shared memory
-// in rank order, and no combine kernel follows.
+// CLUSTER, for few pairs: clusters of four CTAs per pair instead, as many as its context wants and
+// the SMs hold, whose warps take even pieces.  Every piece is a state, and the CTAs' states merge over
+// distributed shared memory in rank order.
 template <int HD, bool CLUSTER>
 __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Params p) {
   constexpr int BLK = 18 * HD, SP = kStagePages<HD>, SPOS = kStagePos<HD>;
@@ -470,7 +546,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) float s_ml[2][kWarps][8][2];
   __shared__ int s_state[kWarps];  // 1: state A, 2: and it ends its pair, 4: state B
-  __shared__ int s_pair[2][kWarps], s_first[kWarps];  // of the states; the first stage of a B's pair
+  __shared__ int s_pair[2][kWarps], s_first[2][kWarps];  // of the states; the unit of the pair's first stage
+  __shared__ int s_cut[2][3];  // pairs that are cut at the CTA's front and end: pair, first CTA, CTAs
+  __shared__ bool s_last[2];
   __shared__ int ctx[kMaxLanes];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hkv = p.num_kv_heads, G = p.num_heads / hkv;
@@ -480,18 +558,23 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
   float* state_a = reinterpret_cast<float*>(smem + (size_t)kWarps * RING);  // [warps][G][ROW]
   PairWalk<HD> use;
   int g0 = 0, g1 = 0;
-  int Q = 0;
+  int Q = 0, pair = 0, nclusters = 1;  // cluster form: the CTA's pair and its clusters
   if constexpr (CLUSTER) {
-    const int pair = blockIdx.x / kClusterCtas;
+    const int cluster = blockIdx.x / kClusterCtas;
+    pair = cluster / p.clusters;
     use.lid = pair / hkv;
     use.kvh = pair - use.lid * hkv;
     const int c = min(max(p.ctx_lens[use.lid], 0), p.max_pages * kQ4Page);
     ctx[use.lid] = c;  // every warp writes the same value
     use.ns = PairWalk<HD>::stages(c);
     use.P = 0;
-    const int w = (int)cluster_ctarank() * kWarps + warp;
-    use.sb = g0 = (int)((long long)use.ns * w / (kClusterCtas * kWarps));
-    use.se = g1 = (int)((long long)use.ns * (w + 1) / (kClusterCtas * kWarps));
+    nclusters = pair_clusters(use.ns, p.clusters);
+    const int part = cluster - pair * p.clusters;
+    if (part >= nclusters) return;  // the whole cluster
+    constexpr long long W = kClusterCtas * kWarps;
+    const long long w = part * W + (int)cluster_ctarank() * kWarps + warp, all = nclusters * W;
+    use.sb = g0 = (int)(use.ns * w / all);
+    use.se = g1 = (int)(use.ns * (w + 1) / all);
     if (use.sb == use.se) use.lid = -1;
   } else {
     Q = find_share<HD>(p, blockIdx.x * kWarps + warp, ctx, use, g0, g1);
@@ -624,162 +707,129 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
       }
       if (lane == 0 && !(begins && ends)) {
         s_state[warp] |= begins ? 4 : ends ? 3 : 1;
-        if (begins) s_first[warp] = done.P;
+        if (begins || warp == 0) s_first[which][warp] = done.P + 1;
         s_pair[which][warp] = done.lid * hkv + done.kvh;
       }
     }
   }
   if constexpr (CLUSTER) {
-    merge_cluster<HD>(p, smem, state_a, s_ml[0], s_state, warp, lane, G);
-    return;
-  }
-  // Lanes of context 0 get zeros.
-  for (int b = blockIdx.x; b < p.lanes; b += gridDim.x)
-    if (ctx[b] == 0)
-      for (int i = threadIdx.x; i < p.num_heads * HD; i += kWarps * 32) p.out[(size_t)b * p.ldo + i] = 0.f;
-  __syncthreads();
+    merge_cluster<HD>(p, smem, state_a, s_ml[0], s_state, warp, lane, G, pair, nclusters);
+  } else {
+    // Lanes of context 0 get zeros.
+    for (int b = blockIdx.x; b < p.lanes; b += gridDim.x)
+      if (ctx[b] == 0)
+        for (int i = threadIdx.x; i < p.num_heads * HD; i += kWarps * 32) p.out[(size_t)b * p.ldo + i] = 0.f;
+    __syncthreads();
 
-  // ---- pieces.  Chain 0 starts with A of warp 0, chain 1 + w with B of warp w; each goes on with
-  // the A's behind it until one ends its pair.  A warp takes a chain, its threads the dims. ----
-  constexpr uint32_t WARPS = (1u << kWarps) - 1;
-  const int st = lane < kWarps ? s_state[lane] : 0;
-  const uint32_t is_b = __ballot_sync(0xffffffffu, st & 4) & WARPS,
-                 is_1 = __ballot_sync(0xffffffffu, (st & 3) == 1) & WARPS,
-                 is_3 = __ballot_sync(0xffffffffu, (st & 3) == 3) & WARPS;
-  const uint32_t chains = is_b << 1 | ((is_1 | is_3) & 1u);
-  if (chains == 0 && threadIdx.x == 0) p.meta[2 * blockIdx.x] = -1;
-  for (int chain = warp; chain <= kWarps; chain += kWarps) {
-    if (!(chains >> chain & 1)) continue;
-    const int first = chain ? chain - 1 : 0;           // warp of the chain's first state
-    const int from = chain ? first + 1 : 0;            // its first A
-    const int stop = __ffs(~is_1 >> from) - 1 + from;  // the first warp from there whose A does not go on
-    const bool ended = is_3 >> stop & 1;
-    const int end = ended ? stop + 1 : stop;  // states of warps [first, end), the first as B unless chain 0
-    float M[8], L[8];
-    float4 a[8];
+    // ---- pieces.  Chain 0 starts with A of warp 0, chain 1 + w with B of warp w; each goes on with
+    // the A's behind it until one ends its pair.  A warp takes a chain, its threads the dims. ----
+    constexpr uint32_t WARPS = (1u << kWarps) - 1;
+    const int st = lane < kWarps ? s_state[lane] : 0;
+    const uint32_t is_b = __ballot_sync(0xffffffffu, st & 4) & WARPS,
+                   is_1 = __ballot_sync(0xffffffffu, (st & 3) == 1) & WARPS,
+                   is_3 = __ballot_sync(0xffffffffu, (st & 3) == 3) & WARPS;
+    const uint32_t chains = is_b << 1 | ((is_1 | is_3) & 1u);
+    if (threadIdx.x < 2) s_cut[threadIdx.x][0] = -1;
+    __syncthreads();
+    for (int chain = warp; chain <= kWarps; chain += kWarps) {
+      if (!(chains >> chain & 1)) continue;
+      const int first = chain ? chain - 1 : 0;           // warp of the chain's first state
+      const int from = chain ? first + 1 : 0;            // its first A
+      const int stop = __ffs(~is_1 >> from) - 1 + from;  // the first warp from there whose A does not go on
+      const bool ended = is_3 >> stop & 1;
+      const int end = ended ? stop + 1 : stop;  // states of warps [first, end), the first as B unless chain 0
+      float M[8], L[8];
+      float4 a[8];
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      M[g] = -INFINITY;
-      L[g] = 0.f;
-      a[g] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    for (int w = first; w < end; ++w) {
-      const float(*ml)[2] = s_ml[chain && w == first ? 1 : 0][w];
+      for (int g = 0; g < 8; ++g) {
+        M[g] = -INFINITY;
+        L[g] = 0.f;
+        a[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      for (int w = first; w < end; ++w) {
+        const float(*ml)[2] = s_ml[chain && w == first ? 1 : 0][w];
 #pragma unroll
-      for (int g = 0; g < 8; ++g)
-        if (g < G) M[g] = fmaxf(M[g], ml[g][0]);
-    }
-    const int d = 4 * (lane % (HD / 4));
-    for (int w = first; w < end; ++w) {
-      const bool b = chain && w == first;
-      const float(*ml)[2] = s_ml[b ? 1 : 0][w];
-      const float* src = (b ? reinterpret_cast<const float*>(smem + (size_t)w * RING) : state_a + (size_t)w * G * ROW) + d;
+        for (int g = 0; g < 8; ++g)
+          if (g < G) M[g] = fmaxf(M[g], ml[g][0]);
+      }
+      const int d = 4 * (lane % (HD / 4));
+      for (int w = first; w < end; ++w) {
+        const bool b = chain && w == first;
+        const float(*ml)[2] = s_ml[b ? 1 : 0][w];
+        const float* src = (b ? reinterpret_cast<const float*>(smem + (size_t)w * RING) : state_a + (size_t)w * G * ROW) + d;
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          if (g < G) {
+            const float2 r = *reinterpret_cast<const float2*>(ml[g]);
+            const float4 y = *reinterpret_cast<const float4*>(src + g * ROW);
+            const float x = r.x == -INFINITY ? 0.f : ex2(r.x - M[g]);
+            L[g] = fmaf(r.y, x, L[g]);
+            a[g].x = fmaf(y.x, x, a[g].x);
+            a[g].y = fmaf(y.y, x, a[g].y);
+            a[g].z = fmaf(y.z, x, a[g].z);
+            a[g].w = fmaf(y.w, x, a[g].w);
+          }
+        }
+      }
+      const int pair = s_pair[chain ? 1 : 0][first];
+      const bool whole = chain && ended;
+      const size_t part = (2 * (size_t)blockIdx.x + (chain ? 1 : 0)) * G;
+      float* dst = whole ? p.out + (size_t)(pair / hkv) * p.ldo + (size_t)(pair % hkv) * G * HD : p.part_o + part * HD;
 #pragma unroll
       for (int g = 0; g < 8; ++g) {
         if (g < G) {
-          const float2 r = *reinterpret_cast<const float2*>(ml[g]);
-          const float4 y = *reinterpret_cast<const float4*>(src + g * ROW);
-          const float x = r.x == -INFINITY ? 0.f : ex2(r.x - M[g]);
-          L[g] = fmaf(r.y, x, L[g]);
-          a[g].x = fmaf(y.x, x, a[g].x);
-          a[g].y = fmaf(y.y, x, a[g].y);
-          a[g].z = fmaf(y.z, x, a[g].z);
-          a[g].w = fmaf(y.w, x, a[g].w);
+          const float r = whole ? (L[g] == 0.f ? 0.f : 8.f / L[g]) : 1.f;
+          if (lane < HD / 4)
+            *reinterpret_cast<float4*>(dst + g * HD + d) = make_float4(a[g].x * r, a[g].y * r, a[g].z * r, a[g].w * r);
+          if (!whole && lane == 0) {
+            p.part_ml[(part + g) * 2] = M[g];
+            p.part_ml[(part + g) * 2 + 1] = L[g];
+          }
         }
       }
-    }
-    const int pair = s_pair[chain ? 1 : 0][first];
-    const bool whole = chain && ended;
-    const size_t part = (2 * (size_t)blockIdx.x + (chain ? 1 : 0)) * G;
-    float* dst = whole ? p.out + (size_t)(pair / hkv) * p.ldo + (size_t)(pair % hkv) * G * HD : p.part_o + part * HD;
-#pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      if (g < G) {
-        const float r = whole ? (L[g] == 0.f ? 0.f : 8.f / L[g]) : 1.f;
-        if (lane < HD / 4)
-          *reinterpret_cast<float4*>(dst + g * HD + d) = make_float4(a[g].x * r, a[g].y * r, a[g].z * r, a[g].w * r);
-        if (!whole && lane == 0) {
-          p.part_ml[(part + g) * 2] = M[g];
-          p.part_ml[(part + g) * 2 + 1] = L[g];
-        }
+      if (!whole && lane == 0) {
+        const int per = Q * kWarps, begin = s_first[chain ? 1 : 0][first], ns = PairWalk<HD>::stages(ctx[pair / hkv]);
+        int* cut = s_cut[chain ? 1 : 0];
+        cut[0] = pair;
+        cut[1] = begin / per;
+        cut[2] = (begin + ns - 1) / per - begin / per + 1;
       }
     }
-    if (chain == 31 - __clz(chains) && lane == 0) {
-      // A pair begun here that goes on in the next CTAs, and how many CTAs its stages fall into.
-      const bool open = chain && !ended;
-      p.meta[2 * blockIdx.x] = open ? pair : -1;
-      if (open) {
-        const int per = Q * kWarps, begin = s_first[first], ns = PairWalk<HD>::stages(ctx[pair / hkv]);
-        p.meta[2 * blockIdx.x + 1] = (begin + ns - 1) / per - begin / per + 1;
-      }
+    __syncthreads();  // the partial segments are written
+    if (s_cut[0][0] < 0 && s_cut[1][0] < 0) return;
+    if (threadIdx.x == 0) {
+      __threadfence();
+      for (int i = 0; i < 2; ++i)
+        s_last[i] = s_cut[i][0] >= 0 && last_of(p.tickets + s_cut[i][1], p.nonce, s_cut[i][2]);
+      __threadfence();
     }
+    __syncthreads();
+    for (int i = 0; i < 2; ++i)
+      if (s_last[i] && warp < G) {
+        const int c0 = s_cut[i][1];
+        merge_segments<HD>(p, s_cut[i][0], warp, s_cut[i][2], lane, G, [&](int s) {
+          return (s == 0 ? 2 * (size_t)c0 + 1 : 2 * (size_t)(c0 + s)) * G + warp;
+        });
+      }
   }
 }
 
-// Pairs that were cut: block (c, g) merges head g of the pair that CTA c began and left open.  Its
-// segments are CTA c's last and the first ones of the CTAs behind it; eight slices of
-// them in order, then the slices in order.
-constexpr int kSlices = 8;
-template <int HD>
-__global__ void __launch_bounds__(kSlices * HD / 4) attn_q4_combine_kernel(const AttnQ4Params p) {
-  __shared__ float4 s_o[kSlices][HD / 4];
-  __shared__ float s_l[kSlices];
-  griddep_launch();
-  griddep_wait();
-  const int c = blockIdx.x, g = blockIdx.y, G = gridDim.y;
-  const int2 meta = *reinterpret_cast<const int2*>(p.meta + 2 * c);
-  if (meta.x < 0) return;
-  const int nseg = meta.y, lane = threadIdx.x & 31;
-  const int col = threadIdx.x % (HD / 4), slice = threadIdx.x / (HD / 4);
-  auto part = [&](int s) { return (s == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + s)) * G + g; };
-  float M = -INFINITY;
-  for (int s = lane; s < nseg; s += 32) M = fmaxf(M, p.part_ml[part(s) * 2]);
-  M = warp_max(M);
-  float L = 0.f;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int per = (nseg + kSlices - 1) / kSlices;
-#pragma unroll 4
-  for (int s = slice * per; s < min(nseg, (slice + 1) * per); ++s) {
-    const float4 v = *reinterpret_cast<const float4*>(p.part_o + part(s) * HD + 4 * col);
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part(s) * 2);
-    const float x = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-    L = fmaf(ml.y, x, L);
-    a.x = fmaf(v.x, x, a.x);
-    a.y = fmaf(v.y, x, a.y);
-    a.z = fmaf(v.z, x, a.z);
-    a.w = fmaf(v.w, x, a.w);
-  }
-  s_o[slice][col] = a;
-  if (col == 0) s_l[slice] = L;
-  __syncthreads();
-  if (slice != 0) return;
-#pragma unroll
-  for (int s = 1; s < kSlices; ++s) {
-    const float4 v = s_o[s][col];
-    L += s_l[s];
-    a.x += v.x;
-    a.y += v.y;
-    a.z += v.z;
-    a.w += v.w;
-  }
-  const float r = L == 0.f ? 0.f : 8.f / L;
-  *reinterpret_cast<float4*>(p.out + (size_t)(meta.x / p.num_kv_heads) * p.ldo +
-                             (size_t)((meta.x % p.num_kv_heads) * G + g) * HD + 4 * col) =
-      make_float4(a.x * r, a.y * r, a.z * r, a.w * r);
-}
-
-// The cluster form: at most one cluster per pair at a time on the SMs, and contexts that give a warp
-// few stages.
-constexpr size_t kClusterPairs = 16, kClusterPages = 512;
+// The cluster form: about as many clusters of four CTAs as fit on the SMs at once (33 of eight GPCs,
+// while clusters of eight leave 28 of the 148 SMs out).
+constexpr size_t kClusters = 32;
 
 }  // namespace
 
-// Two partial segments per CTA (one that begins a pair, one that continues it), and the
-// descriptors of cut pairs.
+// Tickets: one per CTA, or per head of the cluster form's pairs.
+static size_t ticket_floats() {
+  return 2 * std::max(ceil_div((size_t)sm_count(), (size_t)2) * 2, kClusters * 8);
+}
+
+// The tickets and two partial segments per CTA (one that begins a pair, one that continues it).
 size_t attention_q4_workspace_floats(size_t num_heads, size_t num_kv_heads, size_t head_dim) {
   if (!num_kv_heads) return 0;
   const size_t ctas = (size_t)sm_count();
-  return ceil_div(2 * ctas, (size_t)4) * 4 + 2 * ctas * (num_heads / num_kv_heads) * (head_dim + 2);
+  return ticket_floats() + 2 * ctas * (num_heads / num_kv_heads) * (head_dim + 2);
 }
 
 int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_pages, size_t num_layers,
@@ -810,8 +860,13 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
   p.ctx_lens = ctx_lens;
   p.out = out;
   p.ldo = ldo;
-  p.meta = reinterpret_cast<int32_t*>(workspace);
-  p.part_o = workspace + ceil_div(2 * (size_t)grid, (size_t)4) * 4;
+  // Every launch marks its tickets with a number of its own; a captured one keeps its, and finds the
+  // tickets cleared by the replay before.
+  static std::atomic<unsigned long long> launches{(unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
+  do p.nonce = launches.fetch_add(1, std::memory_order_relaxed) & 0xffffffffffffull;
+  while (p.nonce == 0);
+  p.tickets = reinterpret_cast<unsigned long long*>(workspace);
+  p.part_o = workspace + ticket_floats();
   p.part_ml = p.part_o + 2 * (size_t)grid * G * head_dim;
   p.page_bytes = (uint32_t)page_bytes;
   p.lanes = (int)lanes;
@@ -824,17 +879,16 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
   p.bad = ops_error_word();
   GLC_REQUIRE(p.bad, "paged_attention_q4: device status word unavailable");
   const size_t pairs = lanes * num_kv_heads;
-  const bool cluster = pairs <= kClusterPairs && max_pages <= kClusterPages;
+  const bool cluster = pairs <= kClusters;
+  p.clusters = cluster ? (int)(kClusters / pairs) : 0;
   auto kern = head_dim == 128 ? (cluster ? attn_q4_kernel<128, true> : attn_q4_kernel<128, false>)
                               : (cluster ? attn_q4_kernel<64, true> : attn_q4_kernel<64, false>);
   const size_t pages = head_dim == 128 ? kStagePages<128> : kStagePages<64>;
   const size_t smem = kWarps * (kStages * pages * q4_block_bytes(head_dim) + G * (head_dim + 4) * sizeof(float));
   if ((rc = allow_dynamic_smem((const void*)kern, (int)smem))) return rc;
   if (cluster)
-    return launch_pdl(kern, dim3((unsigned)(pairs * kClusterCtas)), dim3(kWarps * 32), smem, stream, kClusterCtas, p);
-  if ((rc = launch_pdl(kern, dim3((unsigned)grid), dim3(kWarps * 32), smem, stream, 1, p))) return rc;
-  return launch_pdl(head_dim == 128 ? attn_q4_combine_kernel<128> : attn_q4_combine_kernel<64>,
-                    dim3((unsigned)grid, (unsigned)G), dim3((unsigned)(kSlices * head_dim / 4)), 0, stream, 1, p);
+    return launch_pdl(kern, dim3((unsigned)(pairs * p.clusters * kClusterCtas)), dim3(kWarps * 32), smem, stream, kClusterCtas, p);
+  return launch_pdl(kern, dim3((unsigned)grid), dim3(kWarps * 32), smem, stream, 1, p);
 }
 
 }  // namespace glacier
