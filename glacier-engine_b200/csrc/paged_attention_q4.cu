@@ -10,11 +10,13 @@
 // bits together; the held values are exact.  (A tcgen05.mma needs 64 or 128 rows and its
 // operands in shared memory as fp16: the codes would be unpacked, written and read once more.)
 //   * q K^T: M is the query heads, and eight of them would leave half of the sixteen rows
-//     idle: rows 0-7 hold q's high and rows 8-15 its low parts.  A code c is used as the fp16
-//     number whose bits are the code, c * 2^-24, or c * 2^-20 one nibble higher (q's dims there
-//     carry 2^-4): one shift and four ANDs make four operand registers of eight codes.  The zero
-//     point is the accumulator's initial value, -7 sum q of the group, and the group's scale
-//     multiplies the fp32 result.
+//     idle: rows 0-7 hold q's high and rows 8-15 its low parts.  A code c at bits 4-7 is used as
+//     the subnormal fp16 number that these bits are, c * 2^-20: three shifts and four ANDs make
+//     four operand registers of eight codes.  (At bits 0-3, c * 2^-24, one shift would do, but the
+//     tensor core aligns a subnormal's products as if it had the smallest normal exponent, and
+//     its sums were 2^-20 off; at bits 4-7 they are within 2^-25.)  The zero point is the
+//     accumulator's initial value, -7 sum q of the group, and the group's scale multiplies the
+//     fp32 result.
 //   * (P V)^T = V^T P^T: M is sixteen dims, N the heads, so that no accumulator is idle, and the
 //     score accumulators are the weights' operand as they stand.  The scale belongs to the summed
 //     index, so it has to be in the operand: (c - 7) s / 8 = (72 - h) s / 8 for the fp16 number
@@ -158,25 +160,28 @@ __device__ __forceinline__ void split_q(const AttnQ4Params& p, const float (&v)[
   // A power of two that brings the head's largest |q| into [2^14, 2^15), from the exponent bits.
   const int e = top > 0.f && top <= 3.4028235e38f ? min(max((int)(__float_as_uint(top) >> 23) - 127 - 14, -100), 100) : 0;
   const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-  q.f = __uint_as_float((uint32_t)(127 + e) << 23) * 0x1p24f * p.scale_log2;
+  q.f = __uint_as_float((uint32_t)(127 + e) << 23) * 0x1p20f * p.scale_log2;
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    float sum = 0.f;
-    // The word's nibbles pair dims (i, i + 4); pairs 1 and 3 are used 2^4 higher.
+    // High and low parts keep sums of their own: the high row then adds numbers of few bits, which the
+    // tensor core's sums hold whole.
+    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float m = (i & 1) ? inv * 0.0625f : inv;
+    for (int i = 0; i < 4; ++i) {  // the word's nibbles pair dims (i, i + 4)
       uint32_t hi, lo;
-      split2(make_float2(v[g][i] * m, v[g][i + 4] * m), hi, lo);
+      split2(make_float2(v[g][i] * inv, v[g][i + 4] * inv), hi, lo);
       q.a[2 * g + (i >> 1)][(i & 1) * 2] = hi;
       q.a[2 * g + (i >> 1)][(i & 1) * 2 + 1] = lo;
-      const float2 f = __fadd2_rn(__half22float2(bits_h2(hi)), __half22float2(bits_h2(lo)));
-      sum = fmaf((i & 1) ? 16.f : 1.f, f.x + f.y, sum);
+      const float2 h = __half22float2(bits_h2(hi)), l = __half22float2(bits_h2(lo));
+      sum = __fadd2_rn(sum, make_float2(h.x + h.y, l.x + l.y));
     }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    q.c[g][0] = q.c[g][1] = -7.f * 0x1p-24f * sum;
-    q.c[g][2] = q.c[g][3] = 0.f;  // the low rows' sum is in the high rows'
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
+      sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
+    }
+    q.c[g][0] = q.c[g][1] = -7.f * 0x1p-20f * sum.x;
+    q.c[g][2] = q.c[g][3] = -7.f * 0x1p-20f * sum.y;
   }
 }
 
@@ -200,8 +205,8 @@ __device__ __forceinline__ void stage_scores(const uint8_t* __restrict__ buf, co
       for (int g = 0; g < NG; ++g) {
         float d[4];
         const uint32_t x = w.w[g], y = x >> 8;
-        mma_f16(d, q.a[2 * g], x & 0x000F000Fu, x & 0x00F000F0u, q.c[g]);
-        mma_f16(d, q.a[2 * g + 1], y & 0x000F000Fu, y & 0x00F000F0u, d);
+        mma_f16(d, q.a[2 * g], x * 16u & 0x00F000F0u, x & 0x00F000F0u, q.c[g]);
+        mma_f16(d, q.a[2 * g + 1], y * 16u & 0x00F000F0u, y & 0x00F000F0u, d);
         const float2 f = __half22float2(bits_h2(s.w[g]));
         r = __ffma2_rn(f, make_float2(d[0], d[1]), r);
         r = __ffma2_rn(f, make_float2(d[2], d[3]), r);
@@ -211,8 +216,8 @@ __device__ __forceinline__ void stage_scores(const uint8_t* __restrict__ buf, co
   }
 }
 
-// The online softmax of one stage's scores and its weighted V.  Weights are 2^(7 + s - m)
-// in base-2 scores s: m is a reference near the running maximum of head lane / 4, moved
+// The online softmax of one stage's scores and its weighted V.  Weights are 2^7 2^(s - m) in
+// base-2 scores s: m is a reference near the running maximum of head lane / 4, moved
 // (and everything rescaled) only when a score passes it by more than 2^8, so the weights stay
 // below 2^15 and their low parts normal fp16 numbers.  l: this thread's share of their
 // sum; o: sums of weight * v / 8.
@@ -254,7 +259,14 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
       o[i][3] *= a1;
     }
   }
-  const float base = m == -INFINITY ? 7.f : fmaf(-m, q.f, 7.f);
+  const float base = m == -INFINITY ? 0.f : -(m * q.f);
+  // The stage's sums start from zero and are added with rounding: a tensor core's sums cut, always
+  // towards zero, and over ten stages that was 1e-6 of the result (with this, 3e-7; 1.5 % of the time).
+  float sum[HD / 16][4];
+#pragma unroll
+  for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sum[i][c] = 0.f;
 #pragma unroll
   for (int pg = 0; pg < SP; ++pg) {
     uint32_t hi[2], lo[2];
@@ -263,6 +275,7 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
       float2 e = __ffma2_rn(sc[2 * pg + j], make_float2(q.f, q.f), make_float2(base, base));
       e.x = ex2(e.x);
       e.y = ex2(e.y);
+      e = __fmul2_rn(e, make_float2(128.f, 128.f));
       l = __fadd2_rn(l, e);
       split2(e, hi[j], lo[j]);
     }
@@ -295,11 +308,19 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
           a[2 * j] = h2_bits(__hfma2(bits_h2(v_bits(i == 0 ? x * 16u : x >> 4)), s8[j], s9[j]));
           a[2 * j + 1] = h2_bits(__hfma2(bits_h2(v_bits(i == 0 ? x : x >> 8)), s8[j], s9[j]));
         }
-        mma_f16(o[2 * k + i / 2], a, hi[0], hi[1], o[2 * k + i / 2]);
-        mma_f16(o[2 * k + i / 2], a, lo[0], lo[1], o[2 * k + i / 2]);
+        mma_f16(sum[2 * k + i / 2], a, hi[0], hi[1], sum[2 * k + i / 2]);
+        mma_f16(sum[2 * k + i / 2], a, lo[0], lo[1], sum[2 * k + i / 2]);
       }
     }
   }
+#pragma unroll
+  for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; c += 2) {
+      const float2 r = __fadd2_rn(make_float2(o[i][c], o[i][c + 1]), make_float2(sum[i][c], sum[i][c + 1]));
+      o[i][c] = r.x;
+      o[i][c + 1] = r.y;
+    }
 }
 
 // A walk over the pairs of a warp's share [g0, g1) and its segment [sb, se) of each.  All (lane,
@@ -398,20 +419,27 @@ __device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ct
   }
 }
 
-// Counts one of `n` arrivals at a ticket; true for the last, which clears it.  A ticket that another
-// launch did not write (any contents of a new workspace) counts as none: 48 bits tell them apart.
-// Only the first arrival needs the compare-and-swap: one per arrival, retried, took 14 us more
-// where 37 CTAs share a pair.
-__device__ __forceinline__ bool last_of(unsigned long long* ticket, unsigned long long nonce, int n) {
+// Tickets count the arrivals of a pair's segments; the last arrival clears its ticket.  A launch
+// marks its tickets with a number of its own, so whatever else one holds (any contents of a new
+// workspace) counts as none: 48 bits tell them apart.  open_ticket() is called early by whoever owns the
+// ticket, so that an arrival is one atomic addition as a rule; it does not rely on it.
+__device__ __forceinline__ void open_ticket(unsigned long long* ticket, unsigned long long nonce) {
   unsigned long long old = *reinterpret_cast<volatile unsigned long long*>(ticket);
-  bool first = false;
-  if (old >> 16 != nonce) {
-    const unsigned long long was = atomicCAS(ticket, old, nonce << 16 | 1u);
-    first = was == old;
-    old = 0;
+  while (old >> 16 != nonce) {
+    const unsigned long long was = atomicCAS(ticket, old, nonce << 16);
+    if (was == old) return;
+    old = was;
   }
-  if (!first) old = atomicAdd(ticket, 1ull) & 0xffffu;
-  if ((int)old + 1 != n) return false;
+}
+
+// One of `n` arrivals; true for the last.
+__device__ __forceinline__ bool last_of(unsigned long long* ticket, unsigned long long nonce, int n) {
+  unsigned long long old = atomicAdd(ticket, 1ull);
+  if (old >> 16 != nonce) {  // not open yet: the addition went to something that does not count
+    open_ticket(ticket, nonce);
+    old = atomicAdd(ticket, 1ull);
+  }
+  if ((int)(old & 0xffffu) + 1 != n) return false;
   atomicExch(ticket, 0ull);
   return true;
 }
@@ -547,8 +575,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
   __shared__ __align__(8) float s_ml[2][kWarps][8][2];
   __shared__ int s_state[kWarps];  // 1: state A, 2: and it ends its pair, 4: state B
   __shared__ int s_pair[2][kWarps], s_first[2][kWarps];  // of the states; the unit of the pair's first stage
-  __shared__ int s_cut[2][3];  // pairs that are cut at the CTA's front and end: pair, first CTA, CTAs
-  __shared__ bool s_last[2];
   __shared__ int ctx[kMaxLanes];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hkv = p.num_kv_heads, G = p.num_heads / hkv;
@@ -571,12 +597,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
     nclusters = pair_clusters(use.ns, p.clusters);
     const int part = cluster - pair * p.clusters;
     if (part >= nclusters) return;  // the whole cluster
+    if (part == 0 && nclusters > 1 && cluster_ctarank() == 0 && threadIdx.x < G)
+      open_ticket(p.tickets + pair * G + threadIdx.x, p.nonce);
     constexpr long long W = kClusterCtas * kWarps;
     const long long w = part * W + (int)cluster_ctarank() * kWarps + warp, all = nclusters * W;
     use.sb = g0 = (int)(use.ns * w / all);
     use.se = g1 = (int)(use.ns * (w + 1) / all);
     if (use.sb == use.se) use.lid = -1;
   } else {
+    if (threadIdx.x == 0) open_ticket(p.tickets + blockIdx.x, p.nonce);
     Q = find_share<HD>(p, blockIdx.x * kWarps + warp, ctx, use, g0, g1);
   }
   if (lane == 0) s_state[warp] = 0;
@@ -722,17 +751,18 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
     __syncthreads();
 
     // ---- pieces.  Chain 0 starts with A of warp 0, chain 1 + w with B of warp w; each goes on with
-    // the A's behind it until one ends its pair.  A warp takes a chain, its threads the dims. ----
+    // the A's behind it until one ends its pair.  Warp w takes the chain that it began, and the first
+    // warp that began none takes chain 0 (warp 0 both, when all did); its threads take the dims. ----
     constexpr uint32_t WARPS = (1u << kWarps) - 1;
     const int st = lane < kWarps ? s_state[lane] : 0;
     const uint32_t is_b = __ballot_sync(0xffffffffu, st & 4) & WARPS,
                    is_1 = __ballot_sync(0xffffffffu, (st & 3) == 1) & WARPS,
                    is_3 = __ballot_sync(0xffffffffu, (st & 3) == 3) & WARPS;
-    const uint32_t chains = is_b << 1 | ((is_1 | is_3) & 1u);
-    if (threadIdx.x < 2) s_cut[threadIdx.x][0] = -1;
-    __syncthreads();
-    for (int chain = warp; chain <= kWarps; chain += kWarps) {
-      if (!(chains >> chain & 1)) continue;
+    const int zero_by = (is_b & WARPS) == WARPS ? 0 : __ffs(~is_b) - 1;
+    const int d = 4 * (lane % (HD / 4));
+    for (int round = 0; round < 2; ++round) {
+      const int chain = round == 0 ? 1 + warp : 0;
+      if (round == 0 ? !(is_b >> warp & 1) : warp != zero_by || !((is_1 | is_3) & 1)) continue;
       const int first = chain ? chain - 1 : 0;           // warp of the chain's first state
       const int from = chain ? first + 1 : 0;            // its first A
       const int stop = __ffs(~is_1 >> from) - 1 + from;  // the first warp from there whose A does not go on
@@ -746,71 +776,85 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
         L[g] = 0.f;
         a[g] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      for (int w = first; w < end; ++w) {
-        const float(*ml)[2] = s_ml[chain && w == first ? 1 : 0][w];
-#pragma unroll
-        for (int g = 0; g < 8; ++g)
-          if (g < G) M[g] = fmaxf(M[g], ml[g][0]);
-      }
-      const int d = 4 * (lane % (HD / 4));
+      // One more state of head g.
+      auto add = [&](int g, float2 ml, float4 y) {
+        const float Mn = fmaxf(M[g], ml.x);
+        const float x = M[g] == -INFINITY ? 0.f : ex2(M[g] - Mn), z = ml.x == -INFINITY ? 0.f : ex2(ml.x - Mn);
+        M[g] = Mn;
+        L[g] = L[g] * x + ml.y * z;
+        a[g].x = a[g].x * x + y.x * z;
+        a[g].y = a[g].y * x + y.y * z;
+        a[g].z = a[g].z * x + y.z * z;
+        a[g].w = a[g].w * x + y.w * z;
+      };
+#pragma unroll 1
       for (int w = first; w < end; ++w) {
         const bool b = chain && w == first;
         const float(*ml)[2] = s_ml[b ? 1 : 0][w];
-        const float* src = (b ? reinterpret_cast<const float*>(smem + (size_t)w * RING) : state_a + (size_t)w * G * ROW) + d;
+        const float* src =
+            (b ? reinterpret_cast<const float*>(smem + (size_t)w * RING) : state_a + (size_t)w * G * ROW) + d;
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
-          if (g < G) {
-            const float2 r = *reinterpret_cast<const float2*>(ml[g]);
-            const float4 y = *reinterpret_cast<const float4*>(src + g * ROW);
-            const float x = r.x == -INFINITY ? 0.f : ex2(r.x - M[g]);
-            L[g] = fmaf(r.y, x, L[g]);
-            a[g].x = fmaf(y.x, x, a[g].x);
-            a[g].y = fmaf(y.y, x, a[g].y);
-            a[g].z = fmaf(y.z, x, a[g].z);
-            a[g].w = fmaf(y.w, x, a[g].w);
-          }
-        }
+        for (int g = 0; g < 8; ++g)
+          if (g < G)
+            add(g, *reinterpret_cast<const float2*>(ml[g]), *reinterpret_cast<const float4*>(src + g * ROW));
       }
       const int pair = s_pair[chain ? 1 : 0][first];
-      const bool whole = chain && ended;
-      const size_t part = (2 * (size_t)blockIdx.x + (chain ? 1 : 0)) * G;
-      float* dst = whole ? p.out + (size_t)(pair / hkv) * p.ldo + (size_t)(pair % hkv) * G * HD : p.part_o + part * HD;
+      float* out = p.out + (size_t)(pair / hkv) * p.ldo + (size_t)(pair % hkv) * G * HD + d;
+      bool write = chain && ended;  // a whole pair
+      if (!write) {
+        // A segment of a pair that is cut at the CTA's front or end.
+        const size_t part = (2 * (size_t)blockIdx.x + (chain ? 1 : 0)) * G;
+        float2 mine = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        if (g < G) {
-          const float r = whole ? (L[g] == 0.f ? 0.f : 8.f / L[g]) : 1.f;
-          if (lane < HD / 4)
-            *reinterpret_cast<float4*>(dst + g * HD + d) = make_float4(a[g].x * r, a[g].y * r, a[g].z * r, a[g].w * r);
-          if (!whole && lane == 0) {
-            p.part_ml[(part + g) * 2] = M[g];
-            p.part_ml[(part + g) * 2 + 1] = L[g];
+        for (int g = 0; g < 8; ++g) {
+          if (g < G && lane < HD / 4) *reinterpret_cast<float4*>(p.part_o + (part + g) * HD + d) = a[g];
+          if (lane == g) mine = make_float2(M[g], L[g]);
+        }
+        if (lane < G) *reinterpret_cast<float2*>(p.part_ml + (part + lane) * 2) = mine;
+        const int per = Q * kWarps, begin = s_first[chain ? 1 : 0][first], ns = PairWalk<HD>::stages(ctx[pair / hkv]);
+        const int c0 = begin / per, n = (begin + ns - 1) / per - c0 + 1;  // its first CTA, its CTAs
+        __syncwarp();
+        if (lane == 0) {
+          __threadfence();
+          write = last_of(p.tickets + c0, p.nonce, n);
+          __threadfence();
+        }
+        write = __shfl_sync(0xffffffffu, write, 0);
+        if (write) {
+          // All are there: CTA c0's last segment, then the first ones of the CTAs behind it.
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            M[g] = -INFINITY;
+            L[g] = 0.f;
+            a[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll 1
+          for (int s = 0; s < n; ++s) {
+            const size_t at = (s == 0 ? 2 * (size_t)c0 + 1 : 2 * (size_t)(c0 + s)) * G;
+            float2 ml[8];
+            float4 y[8];
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+              if (g < G) {
+                ml[g] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (at + g) * 2));
+                y[g] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (at + g) * HD + d));
+              }
+            }
+#pragma unroll
+            for (int g = 0; g < 8; ++g)
+              if (g < G) add(g, ml[g], y[g]);
           }
         }
       }
-      if (!whole && lane == 0) {
-        const int per = Q * kWarps, begin = s_first[chain ? 1 : 0][first], ns = PairWalk<HD>::stages(ctx[pair / hkv]);
-        int* cut = s_cut[chain ? 1 : 0];
-        cut[0] = pair;
-        cut[1] = begin / per;
-        cut[2] = (begin + ns - 1) / per - begin / per + 1;
+      if (write) {
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          const float r = L[g] == 0.f ? 0.f : 8.f / L[g];
+          if (g < G && lane < HD / 4)
+            *reinterpret_cast<float4*>(out + g * HD) = make_float4(a[g].x * r, a[g].y * r, a[g].z * r, a[g].w * r);
+        }
       }
     }
-    __syncthreads();  // the partial segments are written
-    if (s_cut[0][0] < 0 && s_cut[1][0] < 0) return;
-    if (threadIdx.x == 0) {
-      __threadfence();
-      for (int i = 0; i < 2; ++i)
-        s_last[i] = s_cut[i][0] >= 0 && last_of(p.tickets + s_cut[i][1], p.nonce, s_cut[i][2]);
-      __threadfence();
-    }
-    __syncthreads();
-    for (int i = 0; i < 2; ++i)
-      if (s_last[i] && warp < G) {
-        const int c0 = s_cut[i][1];
-        merge_segments<HD>(p, s_cut[i][0], warp, s_cut[i][2], lane, G, [&](int s) {
-          return (s == 0 ? 2 * (size_t)c0 + 1 : 2 * (size_t)(c0 + s)) * G + warp;
-        });
-      }
   }
 }
 
