@@ -35,8 +35,14 @@ namespace glacier {
 namespace {
 
 constexpr int kMaxLanes = 1024;
-constexpr int kWarps = 8;   // two per SM partition
-constexpr int kStages = 4;  // stages in a warp's ring: 147 KB of K/V per SM, three quarters of it in flight
+// Warps per CTA (one CTA per SM) and stages in a warp's ring.  Three warps per SM partition cover each
+// other's latencies better than two, but at hd 128 they have to spill at 168 registers: the 64-lane 7B
+// layer takes 33.6 us with eight warps and 35.5 with twelve, 128 lanes of 1 to 1999 positions at hd 64
+// 31.4 and 29.8 (64 lanes of 2048, with 3 stages a warp: 16.6 and 17.9).  147 and 166 KB of K/V per SM.
+template <int HD>
+constexpr int kWarps = HD == 128 ? 8 : 12;
+template <int HD>
+constexpr int kStages = HD == 128 ? 4 : 3;
 constexpr int kClusterCtas = 4;
 // Pages per stage: 4608 bytes at either head size.
 template <int HD>
@@ -384,7 +390,7 @@ __device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ct
     total += __shfl_sync(0xffffffffu, incl, 31);
   }
   total *= p.num_kv_heads;
-  const int warps = gridDim.x * kWarps;
+  const int warps = gridDim.x * kWarps<HD>;
   const int Q = max(1, (int)(((unsigned)total + warps - 1) / (unsigned)warps));
   start.lid = -1;
   g0 = g1 = 0;
@@ -471,8 +477,9 @@ __device__ __forceinline__ void merge_segments(const AttnQ4Params& p, int pair, 
 }
 
 // Clusters that a pair of `ns` stages is cut into: two stages per warp at least.
+template <int HD>
 __device__ __forceinline__ int pair_clusters(int ns, int most) {
-  return min(most, max(1, (ns + 2 * kClusterCtas * kWarps - 1) / (2 * kClusterCtas * kWarps)));
+  return min(most, max(1, (ns + 2 * kClusterCtas * kWarps<HD> - 1) / (2 * kClusterCtas * kWarps<HD>)));
 }
 
 // The states of a cluster's warps to the pair's output: warp g merges head g over the CTA's
@@ -483,7 +490,7 @@ __device__ __forceinline__ void merge_cluster(const AttnQ4Params& p, uint8_t* sm
                                               const float (*ml)[8][2], const int* s_state, int warp, int lane, int G,
                                               int pair, int nclusters) {
   constexpr int ROW = HD + 4;
-  static_assert(kWarps == 8, "a warp per query head");
+  static_assert(kWarps<HD> >= 8, "a warp per query head");
   __syncthreads();  // every state is written, every ring idle
   float* part = reinterpret_cast<float*>(smem);  // [G][ROW]: o, maximum, sum
   const int g = warp, d = 4 * (lane % (HD / 4));
@@ -491,10 +498,10 @@ __device__ __forceinline__ void merge_cluster(const AttnQ4Params& p, uint8_t* sm
     float M = -INFINITY, L = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w)
+    for (int w = 0; w < kWarps<HD>; ++w)
       if (s_state[w]) M = fmaxf(M, ml[w][g][0]);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kWarps<HD>; ++w) {
       if (!s_state[w]) continue;
       const float x = ml[w][g][0] == -INFINITY ? 0.f : ex2(ml[w][g][0] - M);
       const float4 y = *reinterpret_cast<const float4*>(state_a + ((size_t)w * G + g) * ROW + d);
@@ -565,23 +572,23 @@ __device__ __forceinline__ void merge_cluster(const AttnQ4Params& p, uint8_t* sm
 // the SMs hold, whose warps take even pieces.  Every piece is a state, and the CTAs' states merge over
 // distributed shared memory in rank order.
 template <int HD, bool CLUSTER>
-__global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Params p) {
+__global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ4Params p) {
   constexpr int BLK = 18 * HD, SP = kStagePages<HD>, SPOS = kStagePos<HD>;
-  constexpr int NST = kStages, IDS = 32 / SP;
+  constexpr int NST = kStages<HD>, IDS = 32 / SP;
   constexpr uint32_t ALL = (1u << SP) - 1;
   constexpr int ROW = HD + 4;  // floats per head of a state
   constexpr int RING = NST * SP * BLK;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) float s_ml[2][kWarps][8][2];
-  __shared__ int s_state[kWarps];  // 1: state A, 2: and it ends its pair, 4: state B
-  __shared__ int s_pair[2][kWarps], s_first[2][kWarps];  // of the states; the unit of the pair's first stage
+  __shared__ __align__(8) float s_ml[2][kWarps<HD>][8][2];
+  __shared__ int s_state[kWarps<HD>];  // 1: state A, 2: and it ends its pair, 4: state B
+  __shared__ int s_pair[2][kWarps<HD>], s_first[2][kWarps<HD>];  // of the states; the unit of the pair's first stage
   __shared__ int ctx[kMaxLanes];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hkv = p.num_kv_heads, G = p.num_heads / hkv;
   griddep_launch();
   griddep_wait();  // q, the pages, tables and lengths come from earlier kernels
   uint8_t* ring = smem + (size_t)warp * RING;
-  float* state_a = reinterpret_cast<float*>(smem + (size_t)kWarps * RING);  // [warps][G][ROW]
+  float* state_a = reinterpret_cast<float*>(smem + (size_t)kWarps<HD> * RING);  // [warps][G][ROW]
   PairWalk<HD> use;
   int g0 = 0, g1 = 0;
   int Q = 0, pair = 0, nclusters = 1;  // cluster form: the CTA's pair and its clusters
@@ -594,19 +601,19 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
     ctx[use.lid] = c;  // every warp writes the same value
     use.ns = PairWalk<HD>::stages(c);
     use.P = 0;
-    nclusters = pair_clusters(use.ns, p.clusters);
+    nclusters = pair_clusters<HD>(use.ns, p.clusters);
     const int part = cluster - pair * p.clusters;
     if (part >= nclusters) return;  // the whole cluster
     if (part == 0 && nclusters > 1 && cluster_ctarank() == 0 && threadIdx.x < G)
       open_ticket(p.tickets + pair * G + threadIdx.x, p.nonce);
-    constexpr long long W = kClusterCtas * kWarps;
-    const long long w = part * W + (int)cluster_ctarank() * kWarps + warp, all = nclusters * W;
+    constexpr long long W = kClusterCtas * kWarps<HD>;
+    const long long w = part * W + (int)cluster_ctarank() * kWarps<HD> + warp, all = nclusters * W;
     use.sb = g0 = (int)(use.ns * w / all);
     use.se = g1 = (int)(use.ns * (w + 1) / all);
     if (use.sb == use.se) use.lid = -1;
   } else {
     if (threadIdx.x == 0) open_ticket(p.tickets + blockIdx.x, p.nonce);
-    Q = find_share<HD>(p, blockIdx.x * kWarps + warp, ctx, use, g0, g1);
+    Q = find_share<HD>(p, blockIdx.x * kWarps<HD> + warp, ctx, use, g0, g1);
   }
   if (lane == 0) s_state[warp] = 0;
   __syncwarp();  // ctx and the state word are this warp's own writes
@@ -747,14 +754,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
     // Lanes of context 0 get zeros.
     for (int b = blockIdx.x; b < p.lanes; b += gridDim.x)
       if (ctx[b] == 0)
-        for (int i = threadIdx.x; i < p.num_heads * HD; i += kWarps * 32) p.out[(size_t)b * p.ldo + i] = 0.f;
+        for (int i = threadIdx.x; i < p.num_heads * HD; i += kWarps<HD> * 32) p.out[(size_t)b * p.ldo + i] = 0.f;
     __syncthreads();
 
     // ---- pieces.  Chain 0 starts with A of warp 0, chain 1 + w with B of warp w; each goes on with
     // the A's behind it until one ends its pair.  Warp w takes the chain that it began, and the first
     // warp that began none takes chain 0 (warp 0 both, when all did); its threads take the dims. ----
-    constexpr uint32_t WARPS = (1u << kWarps) - 1;
-    const int st = lane < kWarps ? s_state[lane] : 0;
+    constexpr uint32_t WARPS = (1u << kWarps<HD>) - 1;
+    const int st = lane < kWarps<HD> ? s_state[lane] : 0;
     const uint32_t is_b = __ballot_sync(0xffffffffu, st & 4) & WARPS,
                    is_1 = __ballot_sync(0xffffffffu, (st & 3) == 1) & WARPS,
                    is_3 = __ballot_sync(0xffffffffu, (st & 3) == 3) & WARPS;
@@ -811,7 +818,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_q4_kernel(const AttnQ4Par
           if (lane == g) mine = make_float2(M[g], L[g]);
         }
         if (lane < G) *reinterpret_cast<float2*>(p.part_ml + (part + lane) * 2) = mine;
-        const int per = Q * kWarps, begin = s_first[chain ? 1 : 0][first], ns = PairWalk<HD>::stages(ctx[pair / hkv]);
+        const int per = Q * kWarps<HD>, begin = s_first[chain ? 1 : 0][first], ns = PairWalk<HD>::stages(ctx[pair / hkv]);
         const int c0 = begin / per, n = (begin + ns - 1) / per - c0 + 1;  // its first CTA, its CTAs
         __syncwarp();
         if (lane == 0) {
@@ -928,11 +935,14 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
   auto kern = head_dim == 128 ? (cluster ? attn_q4_kernel<128, true> : attn_q4_kernel<128, false>)
                               : (cluster ? attn_q4_kernel<64, true> : attn_q4_kernel<64, false>);
   const size_t pages = head_dim == 128 ? kStagePages<128> : kStagePages<64>;
-  const size_t smem = kWarps * (kStages * pages * q4_block_bytes(head_dim) + G * (head_dim + 4) * sizeof(float));
+  const size_t warps = head_dim == 128 ? kWarps<128> : kWarps<64>;
+  const size_t stages = head_dim == 128 ? kStages<128> : kStages<64>;
+  const size_t smem = warps * (stages * pages * q4_block_bytes(head_dim) + G * (head_dim + 4) * sizeof(float));
   if ((rc = allow_dynamic_smem((const void*)kern, (int)smem))) return rc;
   if (cluster)
-    return launch_pdl(kern, dim3((unsigned)(pairs * p.clusters * kClusterCtas)), dim3(kWarps * 32), smem, stream, kClusterCtas, p);
-  return launch_pdl(kern, dim3((unsigned)grid), dim3(kWarps * 32), smem, stream, 1, p);
+    return launch_pdl(kern, dim3((unsigned)(pairs * p.clusters * kClusterCtas)), dim3((unsigned)warps * 32), smem,
+                      stream, kClusterCtas, p);
+  return launch_pdl(kern, dim3((unsigned)grid), dim3((unsigned)warps * 32), smem, stream, 1, p);
 }
 
 }  // namespace glacier
