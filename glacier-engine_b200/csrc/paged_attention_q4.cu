@@ -22,6 +22,8 @@
 //     index, so it has to be in the operand: (c - 7) s / 8 = (72 - h) s / 8 for the fp16 number
 //     h = 64 + (15 - c), whose bits one LOP3 makes from a code at bits 4-7.  9 s and the result
 //     are fp16 numbers (scales have 7 significant bits), so one half FMA is exact.
+//     With four heads at most (PACK) the weights' high and low parts share the eight columns: score
+//     rows 4-7 repeat heads 0-3, columns 4-7 take the low parts, and one instruction does both.
 // The cache's orders put every operand register's codes in one word of one thread: K's words
 // (t, g) and V's 16-bit units by position pair are the fragments of these instructions.
 #include <algorithm>
@@ -137,11 +139,12 @@ struct QFrag {
   float f;                // raw score -> base-2 score
 };
 
-// This thread's dims of head lane / 4: 8 t .. 8 t + 7 of every group (zeros past the last head).
-template <int HD>
+// This thread's dims of head lane / 4 (PACK: lane / 4 % 4): 8 t .. 8 t + 7 of every group (zeros past
+// the last head).
+template <int HD, bool PACK>
 __device__ __forceinline__ void load_q(const AttnQ4Params& p, int lid, int kvh, int G, int lane,
                                        float (&v)[HD / 32][8]) {
-  const int h = lane >> 2, t = lane & 3;
+  const int h = PACK ? lane >> 2 & 3 : lane >> 2, t = lane & 3;
 #pragma unroll
   for (int g = 0; g < HD / 32; ++g) {
     if (h < G) {
@@ -228,7 +231,7 @@ __device__ __forceinline__ void stage_scores(const uint8_t* __restrict__ buf, co
 // below 2^15 and their low parts normal fp16 numbers.  l: this thread's share of their
 // sum; o: sums of weight * v / 8.
 // nvalid: positions of the stage inside the context; pages: bit i set when page i was loaded.
-template <int HD, bool MASK>
+template <int HD, bool MASK, bool PACK>
 __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, const QFrag<HD>& q,
                                              float2 (&sc)[2 * kStagePages<HD>], float& m, float2& l,
                                              float (&o)[HD / 16][4], int nvalid, uint32_t pages, int lane) {
@@ -284,6 +287,7 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
       e = __fmul2_rn(e, make_float2(128.f, 128.f));
       l = __fadd2_rn(l, e);
       split2(e, hi[j], lo[j]);
+      if (PACK && n >= 4) hi[j] = lo[j];
     }
     const uint8_t* V = buf + pg * BLK + 8 * HD;
     const uint8_t* S = buf + pg * BLK + 17 * HD + (n / (8 / NG)) * 4;
@@ -315,7 +319,7 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
           a[2 * j + 1] = h2_bits(__hfma2(bits_h2(v_bits(i == 0 ? x : x >> 8)), s8[j], s9[j]));
         }
         mma_f16(sum[2 * k + i / 2], a, hi[0], hi[1], sum[2 * k + i / 2]);
-        mma_f16(sum[2 * k + i / 2], a, lo[0], lo[1], sum[2 * k + i / 2]);
+        if constexpr (!PACK) mma_f16(sum[2 * k + i / 2], a, lo[0], lo[1], sum[2 * k + i / 2]);
       }
     }
   }
@@ -571,7 +575,7 @@ __device__ __forceinline__ void merge_cluster(const AttnQ4Params& p, uint8_t* sm
 // CLUSTER, for few pairs: clusters of four CTAs per pair instead, as many as its context wants and
 // the SMs hold, whose warps take even pieces.  Every piece is a state, and the CTAs' states merge over
 // distributed shared memory in rank order.
-template <int HD, bool CLUSTER>
+template <int HD, bool CLUSTER, bool PACK>
 __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ4Params p) {
   constexpr int BLK = 18 * HD, SP = kStagePages<HD>, SPOS = kStagePos<HD>;
   constexpr int NST = kStages<HD>, IDS = 32 / SP;
@@ -620,7 +624,7 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
 
   if (use.lid >= 0) {
     float v[HD / 32][8];
-    load_q<HD>(p, use.lid, use.kvh, G, lane, v);
+    load_q<HD, PACK>(p, use.lid, use.kvh, G, lane, v);
     // ---- loads: the warp's stages in order, NST - 1 of them ahead of the arithmetic ----
     PairWalk<HD> ld = use;
     const uint64_t pol = l2_evict_first_policy();
@@ -690,7 +694,7 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
       split_q<HD>(p, v, q);
       const PairWalk<HD> done = use;
       more = use.next(ctx, hkv, g0, g1);
-      if (more) load_q<HD>(p, use.lid, use.kvh, G, lane, v);  // arrives while this pair is worked on
+      if (more) load_q<HD, PACK>(p, use.lid, use.kvh, G, lane, v);  // arrives while this pair is worked on
       float m = -INFINITY;
       float2 l2 = make_float2(0.f, 0.f);
       float o[HD / 16][4];
@@ -708,15 +712,21 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
         float2 sc[2 * SP];
         stage_scores<HD>(buf, q, sc, lane);
         if (left >= SPOS && pages == ALL)
-          stage_values<HD, false>(buf, q, sc, m, l2, o, SPOS, ALL, lane);
+          stage_values<HD, false, PACK>(buf, q, sc, m, l2, o, SPOS, ALL, lane);
         else
-          stage_values<HD, true>(buf, q, sc, m, l2, o, left, pages, lane);
+          stage_values<HD, true, PACK>(buf, q, sc, m, l2, o, left, pages, lane);
         slot = slot + 1 == NST ? 0 : slot + 1;
       }
       __syncwarp();  // the last stage is read
       float l = l2.x + l2.y;
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if constexpr (PACK) {
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[i][c] += __shfl_xor_sync(0xffffffffu, o[i][c], 2);
+      }
       const bool begins = !CLUSTER && done.sb == 0, ends = done.se == done.ns;
       const int which = begins ? 1 : 0;
       // A whole pair goes out; a piece to its state (B only at the share's end, over the idle ring).
@@ -932,8 +942,12 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
   const size_t pairs = lanes * num_kv_heads;
   const bool cluster = pairs <= kClusters;
   p.clusters = cluster ? (int)(kClusters / pairs) : 0;
-  auto kern = head_dim == 128 ? (cluster ? attn_q4_kernel<128, true> : attn_q4_kernel<128, false>)
-                              : (cluster ? attn_q4_kernel<64, true> : attn_q4_kernel<64, false>);
+  using Kern = void (*)(AttnQ4Params);
+  static const Kern kerns[8] = {attn_q4_kernel<64, false, false>, attn_q4_kernel<64, false, true>,
+                                attn_q4_kernel<64, true, false>,  attn_q4_kernel<64, true, true>,
+                                attn_q4_kernel<128, false, false>, attn_q4_kernel<128, false, true>,
+                                attn_q4_kernel<128, true, false>,  attn_q4_kernel<128, true, true>};
+  const Kern kern = kerns[(head_dim == 128 ? 4 : 0) + (cluster ? 2 : 0) + (G <= 4 ? 1 : 0)];
   const size_t pages = head_dim == 128 ? kStagePages<128> : kStagePages<64>;
   const size_t warps = head_dim == 128 ? kWarps<128> : kWarps<64>;
   const size_t stages = head_dim == 128 ? kStages<128> : kStages<64>;
