@@ -131,11 +131,14 @@ def argmax_eligible(logits, words=None, stream=None):
 # only a refusal looks for the tensor to name.
 
 _F32, _I32, _I64, _U8 = torch.float32, torch.int32, torch.int64, torch.uint8
+_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _refuse(dev, **tensors):
     """Raises for the first (tensor, dtype, shape) that is not contiguous on `dev` with that type and shape."""
     for name, (t, dtype, shape) in tensors.items():
+        if t is None:
+            continue
         if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous() or tuple(t.shape) != tuple(shape):
             raise GlacierCudaError(EINVAL, f"{name}: {str(t.dtype)[6:]} {tuple(t.shape)} on {t.device}, expected a "
                                            f"contiguous {str(dtype)[6:]} {tuple(shape)} on the GPU of the first tensor")
@@ -150,6 +153,8 @@ class _On:
     """Makes another device, or a given stream, current around a call."""
 
     def __init__(self, dev, stream):
+        if dev < 0:
+            _refuse(dev)
         if stream is not None and stream.device.index != dev:
             raise GlacierCudaError(EINVAL, f"a stream of {stream.device} for tensors on GPU {dev}")
         self.ctx = torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(dev))
@@ -161,31 +166,9 @@ class _On:
         self.ctx.__exit__(*exc)
 
 
-def _run(op, dev, stream, args):
-    """op(*args, raw stream) on the tensors' device, with that stream current."""
-    if stream is None and dev == torch.cuda.current_device():
-        return op(*args, torch._C._cuda_getCurrentRawStream(dev))
-    with _On(dev, stream):
-        return op(*args, torch._C._cuda_getCurrentRawStream(dev))
-
-
 def kv_q4_page_bytes(num_layers: int, num_kv_heads: int, head_dim: int) -> int:
     """Bytes of one 16-position page of a 4-bit pool (all layers)."""
     return lib().glacier_cuda_kv_q4_page_bytes(num_layers, num_kv_heads, head_dim)
-
-
-def _page_shape(pages, num_layers, num_kv_heads, head_dim):
-    return (pages.shape[0], 18 * num_layers * num_kv_heads * head_dim)
-
-
-def _append(qkv, ld, bias, cos, sin, pos, slots, num_heads, num_kv_heads, head_dim, q_out, pages, num_layers, layer, s):
-    b, qd = qkv.shape[0], num_heads * head_dim
-    if q_out is None:
-        q_out = torch.empty((b, qd), dtype=_F32, device=qkv.device)
-    call("glacier_cuda_qkv_rope_append_q4", qkv.data_ptr(), ld, _ptr(bias), cos.data_ptr(), sin.data_ptr(),
-         cos.shape[0], pos.data_ptr(), slots.data_ptr(), b, num_heads, num_kv_heads, head_dim, q_out.data_ptr(), qd,
-         pages.data_ptr(), pages.shape[0], num_layers, layer, s)
-    return q_out
 
 
 def qkv_rope_append_q4(qkv, bias, cos, sin, pos, slots, num_heads, num_kv_heads, head_dim, pages, num_layers, layer,
@@ -193,42 +176,46 @@ def qkv_rope_append_q4(qkv, bias, cos, sin, pos, slots, num_heads, num_kv_heads,
     """qkv_rope_append into a 4-bit pool: ``pages`` uint8 [num_pages, kv_q4_page_bytes], row b's K and V
     quantised into position ``slots[b]`` (int64: page * 16 + row; -1: a padding row).  Returns the rotated q
     [batch, num_heads * head_dim].  ``qkv`` may be a view with a row stride."""
-    dev, b, qd = qkv.get_device(), qkv.shape[0], num_heads * head_dim
-    width, table = qd + 2 * num_kv_heads * head_dim, (cos.shape[0], head_dim // 2)
+    dev = qkv.get_device()
+    if stream is not None or dev < 0 or dev != _device():
+        with _On(dev, stream):
+            return qkv_rope_append_q4(qkv, bias, cos, sin, pos, slots, num_heads, num_kv_heads, head_dim, pages,
+                                      num_layers, layer, q_out)
+    qd, kvd = num_heads * head_dim, num_kv_heads * head_dim
+    width = qd + 2 * kvd
     if qkv.dtype is not _F32 or qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
         raise GlacierCudaError(EINVAL, f"qkv: {qkv.dtype} {tuple(qkv.shape)}, expected float32 rows of {width}")
-    page = _page_shape(pages, num_layers, num_kv_heads, head_dim)
-    if not (dev >= 0 and _fits(cos, _F32, table, dev) and _fits(sin, _F32, table, dev) and _fits(pos, _I32, (b,), dev)
-            and _fits(slots, _I64, (b,), dev) and _fits(pages, _U8, page, dev)
+    b, positions, num_pages = qkv.shape[0], cos.shape[0], pages.shape[0]
+    rows, table, page = (b,), (positions, head_dim // 2), (num_pages, 18 * num_layers * kvd)
+    if not (_fits(cos, _F32, table, dev) and _fits(sin, _F32, table, dev) and _fits(pos, _I32, rows, dev)
+            and _fits(slots, _I64, rows, dev) and _fits(pages, _U8, page, dev)
             and (bias is None or _fits(bias, _F32, (width,), dev))
             and (q_out is None or _fits(q_out, _F32, (b, qd), dev))):
-        named = dict(cos=(cos, _F32, table), sin=(sin, _F32, table), pos=(pos, _I32, (b,)), slots=(slots, _I64, (b,)),
-                     pages=(pages, _U8, page))
-        if bias is not None:
-            named["bias"] = (bias, _F32, (width,))
-        if q_out is not None:
-            named["q_out"] = (q_out, _F32, (b, qd))
-        _refuse(dev, **named)
-    ld = qkv.stride(0) if b > 1 else width
-    return _run(_append, dev, stream, (qkv, ld, bias, cos, sin, pos, slots, num_heads, num_kv_heads, head_dim, q_out,
-                                       pages, num_layers, layer))
-
-
-def _read(pages, slots, num_layers, layer, num_kv_heads, head_dim, s):
-    rows = slots.numel()
-    k = torch.empty((rows, num_kv_heads * head_dim), dtype=_F32, device=pages.device)
-    v = torch.empty_like(k)
-    call("glacier_cuda_kv_q4_read_f32", pages.data_ptr(), pages.shape[0], num_layers, layer, num_kv_heads, head_dim,
-         slots.data_ptr(), rows, k.data_ptr(), v.data_ptr(), s)
-    return k, v
+        _refuse(dev, cos=(cos, _F32, table), sin=(sin, _F32, table), pos=(pos, _I32, rows), slots=(slots, _I64, rows),
+                pages=(pages, _U8, page), bias=(bias, _F32, (width,)), q_out=(q_out, _F32, (b, qd)))
+    if q_out is None:
+        q_out = qkv.new_empty((b, qd))
+    call("glacier_cuda_qkv_rope_append_q4", qkv.data_ptr(), qkv.stride(0) if b > 1 else width, _ptr(bias),
+         cos.data_ptr(), sin.data_ptr(), positions, pos.data_ptr(), slots.data_ptr(), b, num_heads, num_kv_heads,
+         head_dim, q_out.data_ptr(), qd, pages.data_ptr(), num_pages, num_layers, layer, _raw_stream(dev))
+    return q_out
 
 
 def kv_q4_read(pages, slots, num_layers, layer, num_kv_heads, head_dim, stream=None):
     """The K and V values held at ``slots``: two float32 [rows, num_kv_heads * head_dim] (zeros for slot -1)."""
-    dev, rows, page = pages.get_device(), (slots.numel(),), _page_shape(pages, num_layers, num_kv_heads, head_dim)
-    if not (dev >= 0 and _fits(slots, _I64, rows, dev) and _fits(pages, _U8, page, dev)):
-        _refuse(dev, slots=(slots, _I64, rows), pages=(pages, _U8, page))
-    return _run(_read, dev, stream, (pages, slots, num_layers, layer, num_kv_heads, head_dim))
+    dev = pages.get_device()
+    if stream is not None or dev < 0 or dev != _device():
+        with _On(dev, stream):
+            return kv_q4_read(pages, slots, num_layers, layer, num_kv_heads, head_dim)
+    rows, num_pages, kvd = slots.numel(), pages.shape[0], num_kv_heads * head_dim
+    page = (num_pages, 18 * num_layers * kvd)
+    if not (_fits(slots, _I64, (rows,), dev) and _fits(pages, _U8, page, dev)):
+        _refuse(dev, slots=(slots, _I64, (rows,)), pages=(pages, _U8, page))
+    k = pages.new_empty((rows, kvd), dtype=_F32)
+    v = torch.empty_like(k)
+    call("glacier_cuda_kv_q4_read_f32", pages.data_ptr(), num_pages, num_layers, layer, num_kv_heads, head_dim,
+         slots.data_ptr(), rows, k.data_ptr(), v.data_ptr(), _raw_stream(dev))
+    return k, v
 
 
 def paged_attention_q4_workspace(num_heads, num_kv_heads, head_dim, device=None):
@@ -237,43 +224,32 @@ def paged_attention_q4_workspace(num_heads, num_kv_heads, head_dim, device=None)
     return torch.empty(n, dtype=_F32, device="cuda" if device is None else device)
 
 
-def _attend(q, pages, block_tables, ctx_lens, num_layers, layer, num_heads, num_kv_heads, head_dim, out, workspace, s):
-    if workspace is None:
-        workspace = paged_attention_q4_workspace(num_heads, num_kv_heads, head_dim, q.device)
-    if out is None:
-        out = torch.empty_like(q)
-    call("glacier_cuda_paged_attention_q4", q.data_ptr(), pages.data_ptr(), pages.shape[0], num_layers,
-         block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), q.shape[0], layer, num_heads,
-         num_kv_heads, head_dim, out.data_ptr(), workspace.data_ptr(), workspace.numel(), s)
-    return out
-
-
 def paged_attention_q4(q, pages, block_tables, ctx_lens, num_layers, layer, num_heads, num_kv_heads, head_dim,
                        out=None, workspace=None, stream=None):
     """paged_attention_f32 over a 4-bit pool, one query row per lane."""
-    dev, lanes = q.get_device(), q.shape[0]
-    rows, page = (lanes, num_heads * head_dim), _page_shape(pages, num_layers, num_kv_heads, head_dim)
-    table = (lanes, block_tables.shape[-1])
-    if not (dev >= 0 and _fits(q, _F32, rows, dev) and _fits(pages, _U8, page, dev)
-            and _fits(block_tables, _I32, table, dev) and _fits(ctx_lens, _I32, (lanes,), dev)
+    dev = q.get_device()
+    if stream is not None or dev < 0 or dev != _device():
+        with _On(dev, stream):
+            return paged_attention_q4(q, pages, block_tables, ctx_lens, num_layers, layer, num_heads, num_kv_heads,
+                                      head_dim, out, workspace)
+    lanes, num_pages, max_pages = q.shape[0], pages.shape[0], block_tables.shape[-1]
+    rows, page = (lanes, num_heads * head_dim), (num_pages, 18 * num_layers * num_kv_heads * head_dim)
+    floats = 0 if workspace is None else workspace.numel()
+    if not (_fits(q, _F32, rows, dev) and _fits(pages, _U8, page, dev)
+            and _fits(block_tables, _I32, (lanes, max_pages), dev) and _fits(ctx_lens, _I32, (lanes,), dev)
             and (out is None or _fits(out, _F32, rows, dev))
-            and (workspace is None or _fits(workspace, _F32, (workspace.numel(),), dev))):
-        named = dict(q=(q, _F32, rows), pages=(pages, _U8, page), block_tables=(block_tables, _I32, table),
-                     ctx_lens=(ctx_lens, _I32, (lanes,)))
-        if out is not None:
-            named["out"] = (out, _F32, rows)
-        if workspace is not None:
-            named["workspace"] = (workspace, _F32, (workspace.numel(),))
-        _refuse(dev, **named)
-    return _run(_attend, dev, stream, (q, pages, block_tables, ctx_lens, num_layers, layer, num_heads, num_kv_heads,
-                                       head_dim, out, workspace))
-
-
-def _resize(lens, targets, block_tables, free_pages, free_count, status, positions, row_lanes, slots, row_offsets,
-            row_stride, rows, s):
-    call("glacier_cuda_kv_resize", lens.data_ptr(), targets.data_ptr(), lens.shape[0], block_tables.data_ptr(),
-         block_tables.shape[1], free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), status.data_ptr(),
-         row_stride, rows, _ptr(positions), _ptr(row_lanes), _ptr(slots), _ptr(row_offsets), s)
+            and (workspace is None or _fits(workspace, _F32, (floats,), dev))):
+        _refuse(dev, q=(q, _F32, rows), pages=(pages, _U8, page), block_tables=(block_tables, _I32, (lanes, max_pages)),
+                ctx_lens=(ctx_lens, _I32, (lanes,)), out=(out, _F32, rows), workspace=(workspace, _F32, (floats,)))
+    if workspace is None:
+        workspace = paged_attention_q4_workspace(num_heads, num_kv_heads, head_dim, q.device)
+        floats = workspace.numel()
+    if out is None:
+        out = torch.empty_like(q)
+    call("glacier_cuda_paged_attention_q4", q.data_ptr(), pages.data_ptr(), num_pages, num_layers,
+         block_tables.data_ptr(), max_pages, ctx_lens.data_ptr(), lanes, layer, num_heads, num_kv_heads, head_dim,
+         out.data_ptr(), workspace.data_ptr(), floats, _raw_stream(dev))
+    return out
 
 
 def kv_resize(lens, targets, block_tables, free_pages, free_count, status, positions=None, row_lanes=None, slots=None,
@@ -282,26 +258,28 @@ def kv_resize(lens, targets, block_tables, free_pages, free_count, status, posit
     ``block_tables`` and the ``free_pages`` stack of ``free_count`` entries, and the new positions are written
     as rows (positions, row_lanes int32, slots int64; packed, or row_stride rows per lane).  All int32 but slots;
     see glacier_cuda_kv_resize for the order in which lanes are served and the statuses."""
-    dev, lanes = lens.get_device(), (lens.shape[0],)
-    table, pool = (lens.shape[0], block_tables.shape[-1]), (free_pages.numel(),)
-    if not (dev >= 0 and _fits(lens, _I32, lanes, dev) and _fits(targets, _I32, lanes, dev)
-            and _fits(block_tables, _I32, table, dev) and _fits(free_pages, _I32, pool, dev)
+    dev = lens.get_device()
+    if stream is not None or dev < 0 or dev != _device():
+        with _On(dev, stream):
+            return kv_resize(lens, targets, block_tables, free_pages, free_count, status, positions, row_lanes, slots,
+                             row_offsets, row_stride)
+    n, max_pages, capacity = lens.shape[0], block_tables.shape[-1], free_pages.numel()
+    lanes, rows = (n,), 0 if slots is None else slots.numel()
+    if not (_fits(lens, _I32, lanes, dev) and _fits(targets, _I32, lanes, dev)
+            and _fits(block_tables, _I32, (n, max_pages), dev) and _fits(free_pages, _I32, (capacity,), dev)
             and _fits(free_count, _I32, (1,), dev) and _fits(status, _I32, lanes, dev)
-            and (row_offsets is None or _fits(row_offsets, _I32, (lens.shape[0] + 1,), dev))):
-        named = dict(lens=(lens, _I32, lanes), targets=(targets, _I32, lanes), block_tables=(block_tables, _I32, table),
-                     free_pages=(free_pages, _I32, pool), free_count=(free_count, _I32, (1,)),
-                     status=(status, _I32, lanes))
-        if row_offsets is not None:
-            named["row_offsets"] = (row_offsets, _I32, (lens.shape[0] + 1,))
-        _refuse(dev, **named)
-    rows = 0
+            and (row_offsets is None or _fits(row_offsets, _I32, (n + 1,), dev))):
+        _refuse(dev, lens=(lens, _I32, lanes), targets=(targets, _I32, lanes),
+                block_tables=(block_tables, _I32, (n, max_pages)), free_pages=(free_pages, _I32, (capacity,)),
+                free_count=(free_count, _I32, (1,)), status=(status, _I32, lanes),
+                row_offsets=(row_offsets, _I32, (n + 1,)))
     if slots is not None and positions is not None and row_lanes is not None:
-        rows = slots.numel()
         if not (_fits(slots, _I64, (rows,), dev) and _fits(positions, _I32, (rows,), dev)
                 and _fits(row_lanes, _I32, (rows,), dev)):
             _refuse(dev, slots=(slots, _I64, (rows,)), positions=(positions, _I32, (rows,)),
                     row_lanes=(row_lanes, _I32, (rows,)))
     elif not (slots is positions is row_lanes is None):
         raise GlacierCudaError(EINVAL, "kv_resize: positions, row_lanes and slots go together")
-    _run(_resize, dev, stream, (lens, targets, block_tables, free_pages, free_count, status, positions, row_lanes,
-                                slots, row_offsets, row_stride, rows))
+    call("glacier_cuda_kv_resize", lens.data_ptr(), targets.data_ptr(), n, block_tables.data_ptr(), max_pages,
+         free_pages.data_ptr(), capacity, free_count.data_ptr(), status.data_ptr(), row_stride, rows, _ptr(positions),
+         _ptr(row_lanes), _ptr(slots), _ptr(row_offsets), _raw_stream(dev))
