@@ -230,23 +230,14 @@ __device__ __forceinline__ void stage_scores(const uint8_t* __restrict__ buf, co
 // (and everything rescaled) only when a score passes it by more than 2^8, so the weights stay
 // below 2^15 and their low parts normal fp16 numbers.  l: this thread's share of their
 // sum; o: sums of weight * v / 8.
-// nvalid: positions of the stage inside the context; pages: bit i set when page i was loaded.
-template <int HD, bool MASK, bool PACK>
+// keep: masks of the V scales, one per eight positions (two positions a word).
+template <int HD, bool PACK>
 __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, const QFrag<HD>& q,
-                                             float2 (&sc)[2 * kStagePages<HD>], float& m, float2& l,
-                                             float (&o)[HD / 16][4], int nvalid, uint32_t pages, int lane) {
+                                             float2 (&sc)[2 * kStagePages<HD>], const uint32_t (&keep)[2 * kStagePages<HD>],
+                                             float& m, float2& l, float (&o)[HD / 16][4], int lane) {
   constexpr int NG = HD / 32, NW = HD / 32;  // scale groups; words per thread and position pair
   constexpr int BLK = 18 * HD, SP = kStagePages<HD>;
   const int n = lane >> 2, t = lane & 3;
-  if constexpr (MASK) {
-#pragma unroll
-    for (int i = 0; i < 2 * SP; ++i) {
-      const int at = 8 * i + 2 * t;
-      const bool here = (pages >> (i / 2)) & 1;
-      if (!here || at >= nvalid) sc[i].x = -INFINITY;
-      if (!here || at + 1 >= nvalid) sc[i].y = -INFINITY;
-    }
-  }
   float mx = fmaxf(sc[0].x, sc[0].y);
 #pragma unroll
   for (int i = 1; i < 2 * SP; ++i) mx = fmaxf(mx, fmaxf(sc[i].x, sc[i].y));
@@ -296,13 +287,8 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       w[j] = lds<NW>(V + (t + 4 * j) * HD + n * (4 * NW));
-      uint32_t sb = *reinterpret_cast<const uint32_t*>(S + (t + 4 * j) * (4 * NG));
-      if constexpr (MASK) {  // left-over scales may be anything, and 0 * NaN is NaN
-        const int at = pg * kQ4Page + 8 * j + 2 * t;
-        const bool here = (pages >> pg) & 1;
-        if (!here || at >= nvalid) sb = 0;
-        else if (at + 1 >= nvalid) sb &= 0xffffu;
-      }
+      // Left-over scales may be anything, and 0 * NaN is NaN.
+      const uint32_t sb = *reinterpret_cast<const uint32_t*>(S + (t + 4 * j) * (4 * NG)) & keep[2 * pg + j];
       s9[j] = __hmul2(bits_h2(sb), __float2half2_rn(9.f));
       s8[j] = __hmul2(bits_h2(sb), __float2half2_rn(-0.125f));
     }
@@ -625,7 +611,7 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
   if (use.lid >= 0) {
     float v[HD / 32][8];
     load_q<HD, PACK>(p, use.lid, use.kvh, G, lane, v);
-    // ---- loads: the warp's stages in order, NST - 1 of them ahead of the arithmetic ----
+    // ---- loads: the warp's stages in order, the ring kept full ----
     PairWalk<HD> ld = use;
     const uint64_t pol = l2_evict_first_policy();
     int ld_st = 0, ld_at = 0;  // next stage; its place among the stages whose page ids `ids` holds
@@ -639,6 +625,7 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
       const bool ok = inside && (unsigned)ids < (unsigned)p.num_pages;
       ids_ok = __ballot_sync(0xffffffffu, ok);
       if (inside && !ok) atomicExch(p.bad, 1);
+      if (!ok) ids = 0;
       ld_at = 0;
     };
     auto enter = [&]() {
@@ -665,16 +652,13 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
           src[i] = src0 + (uint64_t)(uint32_t)__shfl_sync(0xffffffffu, ids, SP * ld_at + i) * p.page_bytes - i * BLK;
         const uint32_t dst = ring_at + slot_in * (SP * BLK);
         // A stage's pages follow one another in the ring: chunks of 16 bytes, one per thread and step.
-        auto chunks = [&](bool all) {
+        // A page that is not there reads page 0 in its place (one path, and no traffic to speak of).
 #pragma unroll
-          for (int i = 0; i < SP * BLK / 512; ++i) {
-            const int lo = 512 * i / BLK, cut = ((lo + 1) * BLK - 512 * i) / 16;  // threads from `cut` on: the next page
-            const int pg = cut < 32 && lane >= cut ? lo + 1 : lo;
-            const uint8_t* s = pg == lo ? src[lo] : src[lo + 1 < SP ? lo + 1 : lo];
-            if (all || (got >> pg & 1)) cp_async16(dst + 512 * i, s + 512 * i, pol);
-          }
-        };
-        if (got == ALL) chunks(true); else chunks(false);
+        for (int i = 0; i < SP * BLK / 512; ++i) {
+          const int lo = 512 * i / BLK, cut = ((lo + 1) * BLK - 512 * i) / 16;  // threads from `cut` on: the next page
+          const uint8_t* s = cut < 32 && lane >= cut ? src[lo + 1 < SP ? lo + 1 : lo] : src[lo];
+          cp_async16(dst + 512 * i, s + 512 * i, pol);
+        }
         loaded = (loaded & ~(ALL << (SP * slot_in))) | got << (SP * slot_in);
         ++ld_st;
         ++ld_at;
@@ -682,8 +666,7 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
       cp_async_commit();
       slot_in = slot_in + 1 == NST ? 0 : slot_in + 1;
     };
-#pragma unroll 1
-    for (int i = 0; i < NST - 1; ++i) issue();
+    int ahead = 0;  // stages in the ring, this one included
 
     // ---- arithmetic ----
     int slot = 0;
@@ -704,17 +687,30 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
         for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
       int left = ctx[done.lid] - SPOS * done.sb;  // positions from this stage on
       for (int st = done.sb; st < done.se; ++st, left -= SPOS) {
-        cp_async_wait<NST - 2>();
-        __syncwarp();  // this stage is there for every thread, and nobody reads the slot before it any more
-        issue();
+        __syncwarp();  // nobody reads the slot of the stage before any more
+#pragma unroll 1
+        for (; ahead < NST; ++ahead) issue();
+        --ahead;
+        cp_async_wait<NST - 1>();
+        __syncwarp();  // this stage is there for every thread
         const uint32_t pages = (loaded >> (SP * slot)) & ALL;
         const uint8_t* buf = ring + slot * (SP * BLK);
         float2 sc[2 * SP];
         stage_scores<HD>(buf, q, sc, lane);
-        if (left >= SPOS && pages == ALL)
-          stage_values<HD, false, PACK>(buf, q, sc, m, l2, o, SPOS, ALL, lane);
-        else
-          stage_values<HD, true, PACK>(buf, q, sc, m, l2, o, left, pages, lane);
+        uint32_t keep[2 * SP];
+#pragma unroll
+        for (int i = 0; i < 2 * SP; ++i) keep[i] = 0xffffffffu;
+        if (left < SPOS || pages != ALL) {
+          // Positions past the context, and of pages that are not there.
+#pragma unroll
+          for (int i = 0; i < 2 * SP; ++i) {
+            const int in = (pages >> (i / 2) & 1) ? left - 8 * i - 2 * t : 0;  // this thread's two positions
+            if (in < 1) sc[i].x = -INFINITY;
+            if (in < 2) sc[i].y = -INFINITY;
+            keep[i] = in < 1 ? 0u : in < 2 ? 0xffffu : 0xffffffffu;
+          }
+        }
+        stage_values<HD, PACK>(buf, q, sc, keep, m, l2, o, lane);
         slot = slot + 1 == NST ? 0 : slot + 1;
       }
       __syncwarp();  // the last stage is read
