@@ -46,6 +46,7 @@ constexpr int kWarps = HD == 128 ? 8 : 12;
 template <int HD>
 constexpr int kStages = HD == 128 ? 4 : 3;
 constexpr int kClusterCtas = 4;
+constexpr int kPart = 4;  // heads that a warp merges at once, at most
 // Pages per stage: 4608 bytes at either head size.
 template <int HD>
 constexpr int kStagePages = HD == 128 ? 2 : 4;
@@ -60,7 +61,7 @@ struct AttnQ4Params {
   const int32_t* ctx_lens;
   float* out;
   size_t ldo;
-  unsigned long long* tickets;  // [grid]: segments written of the pair that CTA c began and left open
+  unsigned long long* tickets;  // [grid][8]: segments written of the pair that CTA c began and left open, per head
   unsigned long long nonce;     // marks this launch's tickets: whatever else a ticket holds counts as none
   float* part_ml;  // [2 grid][G][2] maximum (base 2) and sum of a segment
   float* part_o;   // [2 grid][G][hd]
@@ -466,6 +467,12 @@ __device__ __forceinline__ void merge_segments(const AttnQ4Params& p, int pair, 
         make_float4(a.x * r, a.y * r, a.z * r, a.w * r);
 }
 
+// Position of the k-th set bit.
+__device__ __forceinline__ int nth_bit(uint32_t bits, int k) {
+  for (; k > 0; --k) bits &= bits - 1;
+  return __ffs(bits) - 1;
+}
+
 // Clusters that a pair of `ns` stages is cut into: two stages per warp at least.
 template <int HD>
 __device__ __forceinline__ int pair_clusters(int ns, int most) {
@@ -602,7 +609,7 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
     use.se = g1 = (int)(use.ns * (w + 1) / all);
     if (use.sb == use.se) use.lid = -1;
   } else {
-    if (threadIdx.x == 0) open_ticket(p.tickets + blockIdx.x, p.nonce);
+    if (threadIdx.x < G) open_ticket(p.tickets + 8 * blockIdx.x + threadIdx.x, p.nonce);
     Q = find_share<HD>(p, blockIdx.x * kWarps<HD> + warp, ctx, use, g0, g1);
   }
   if (lane == 0) s_state[warp] = 0;
@@ -764,27 +771,32 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
     __syncthreads();
 
     // ---- pieces.  Chain 0 starts with A of warp 0, chain 1 + w with B of warp w; each goes on with
-    // the A's behind it until one ends its pair.  Warp w takes the chain that it began, and the first
-    // warp that began none takes chain 0 (warp 0 both, when all did); its threads take the dims. ----
+    // the A's behind it until one ends its pair.  A warp takes one head of a chain when there are warps
+    // enough, up to four otherwise; its threads take the dims.  The first chain and the last come
+    // first: theirs are the pairs that are cut. ----
     constexpr uint32_t WARPS = (1u << kWarps<HD>) - 1;
     const int st = lane < kWarps<HD> ? s_state[lane] : 0;
     const uint32_t is_b = __ballot_sync(0xffffffffu, st & 4) & WARPS,
                    is_1 = __ballot_sync(0xffffffffu, (st & 3) == 1) & WARPS,
                    is_3 = __ballot_sync(0xffffffffu, (st & 3) == 3) & WARPS;
-    const int zero_by = (is_b & WARPS) == WARPS ? 0 : __ffs(~is_b) - 1;
-    const int d = 4 * (lane % (HD / 4));
-    for (int round = 0; round < 2; ++round) {
-      const int chain = round == 0 ? 1 + warp : 0;
-      if (round == 0 ? !(is_b >> warp & 1) : warp != zero_by || !((is_1 | is_3) & 1)) continue;
+    const uint32_t chains = is_b << 1 | ((is_1 | is_3) & 1u);
+    const int d = 4 * (lane % (HD / 4)), num_chains = __popc(chains);
+    int per = 1;  // heads per task
+    while (per < kPart && num_chains * ((G + per - 1) / per) > kWarps<HD>) ++per;
+    const int parts = (G + per - 1) / per;
+#pragma unroll 1
+    for (int task = warp; task < num_chains * parts; task += kWarps<HD>) {
+      const int k = task / parts, h0 = (task - k * parts) * per, heads = min(per, G - h0);
+      const int chain = k == 1 ? 31 - __clz(chains) : nth_bit(chains, max(k - 1, 0));
       const int first = chain ? chain - 1 : 0;           // warp of the chain's first state
       const int from = chain ? first + 1 : 0;            // its first A
       const int stop = __ffs(~is_1 >> from) - 1 + from;  // the first warp from there whose A does not go on
       const bool ended = is_3 >> stop & 1;
       const int end = ended ? stop + 1 : stop;  // states of warps [first, end), the first as B unless chain 0
-      float M[8], L[8];
-      float4 a[8];
+      float M[kPart], L[kPart];
+      float4 a[kPart];
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
+      for (int g = 0; g < kPart; ++g) {
         M[g] = -INFINITY;
         L[g] = 0.f;
         a[g] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -803,67 +815,69 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
 #pragma unroll 1
       for (int w = first; w < end; ++w) {
         const bool b = chain && w == first;
-        const float(*ml)[2] = s_ml[b ? 1 : 0][w];
+        const float(*ml)[2] = s_ml[b ? 1 : 0][w] + h0;
         const float* src =
-            (b ? reinterpret_cast<const float*>(smem + (size_t)w * RING) : state_a + (size_t)w * G * ROW) + d;
+            (b ? reinterpret_cast<const float*>(smem + (size_t)w * RING) : state_a + (size_t)w * G * ROW) + h0 * ROW + d;
 #pragma unroll
-        for (int g = 0; g < 8; ++g)
-          if (g < G)
+        for (int g = 0; g < kPart; ++g)
+          if (g < heads)
             add(g, *reinterpret_cast<const float2*>(ml[g]), *reinterpret_cast<const float4*>(src + g * ROW));
       }
       const int pair = s_pair[chain ? 1 : 0][first];
-      float* out = p.out + (size_t)(pair / hkv) * p.ldo + (size_t)(pair % hkv) * G * HD + d;
-      bool write = chain && ended;  // a whole pair
-      if (!write) {
+      float* out = p.out + (size_t)(pair / hkv) * p.ldo + (size_t)((pair % hkv) * G + h0) * HD + d;
+      uint32_t write = (1u << heads) - 1;  // a whole pair's heads
+      if (!(chain && ended)) {
         // A segment of a pair that is cut at the CTA's front or end.
-        const size_t part = (2 * (size_t)blockIdx.x + (chain ? 1 : 0)) * G;
+        const size_t part = (2 * (size_t)blockIdx.x + (chain ? 1 : 0)) * G + h0;
         float2 mine = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
-          if (g < G && lane < HD / 4) *reinterpret_cast<float4*>(p.part_o + (part + g) * HD + d) = a[g];
+        for (int g = 0; g < kPart; ++g) {
+          if (g < heads && lane < HD / 4) *reinterpret_cast<float4*>(p.part_o + (part + g) * HD + d) = a[g];
           if (lane == g) mine = make_float2(M[g], L[g]);
         }
-        if (lane < G) *reinterpret_cast<float2*>(p.part_ml + (part + lane) * 2) = mine;
-        const int per = Q * kWarps<HD>, begin = s_first[chain ? 1 : 0][first], ns = PairWalk<HD>::stages(ctx[pair / hkv]);
-        const int c0 = begin / per, n = (begin + ns - 1) / per - c0 + 1;  // its first CTA, its CTAs
+        if (lane < heads) *reinterpret_cast<float2*>(p.part_ml + (part + lane) * 2) = mine;
+        const int units = Q * kWarps<HD>, begin = s_first[chain ? 1 : 0][first], ns = PairWalk<HD>::stages(ctx[pair / hkv]);
+        const int c0 = begin / units, n = (begin + ns - 1) / units - c0 + 1;  // its first CTA, its CTAs
         __syncwarp();
-        if (lane == 0) {
+        bool last = false;
+        if (lane < heads) {
           __threadfence();
-          write = last_of(p.tickets + c0, p.nonce, n);
+          last = last_of(p.tickets + 8 * c0 + h0 + lane, p.nonce, n);
           __threadfence();
         }
-        write = __shfl_sync(0xffffffffu, write, 0);
+        write = __ballot_sync(0xffffffffu, last);
+        __syncwarp();
         if (write) {
           // All are there: CTA c0's last segment, then the first ones of the CTAs behind it.
 #pragma unroll
-          for (int g = 0; g < 8; ++g) {
+          for (int g = 0; g < kPart; ++g) {
             M[g] = -INFINITY;
             L[g] = 0.f;
             a[g] = make_float4(0.f, 0.f, 0.f, 0.f);
           }
 #pragma unroll 1
           for (int s = 0; s < n; ++s) {
-            const size_t at = (s == 0 ? 2 * (size_t)c0 + 1 : 2 * (size_t)(c0 + s)) * G;
-            float2 ml[8];
-            float4 y[8];
+            const size_t at = (s == 0 ? 2 * (size_t)c0 + 1 : 2 * (size_t)(c0 + s)) * G + h0;
+            float2 ml[kPart];
+            float4 y[kPart];
 #pragma unroll
-            for (int g = 0; g < 8; ++g) {
-              if (g < G) {
+            for (int g = 0; g < kPart; ++g) {
+              if (write >> g & 1) {
                 ml[g] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (at + g) * 2));
                 y[g] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (at + g) * HD + d));
               }
             }
 #pragma unroll
-            for (int g = 0; g < 8; ++g)
-              if (g < G) add(g, ml[g], y[g]);
+            for (int g = 0; g < kPart; ++g)
+              if (write >> g & 1) add(g, ml[g], y[g]);
           }
         }
       }
       if (write) {
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
+        for (int g = 0; g < kPart; ++g) {
           const float r = L[g] == 0.f ? 0.f : 8.f / L[g];
-          if (g < G && lane < HD / 4)
+          if ((write >> g & 1) && lane < HD / 4)
             *reinterpret_cast<float4*>(out + g * HD) = make_float4(a[g].x * r, a[g].y * r, a[g].z * r, a[g].w * r);
         }
       }
@@ -877,10 +891,8 @@ constexpr size_t kClusters = 32;
 
 }  // namespace
 
-// Tickets: one per CTA, or per head of the cluster form's pairs.
-static size_t ticket_floats() {
-  return 2 * std::max(ceil_div((size_t)sm_count(), (size_t)2) * 2, kClusters * 8);
-}
+// Tickets: one per head and CTA, or pair of the cluster form.
+static size_t ticket_floats() { return 2 * 8 * std::max((size_t)sm_count(), kClusters); }
 
 // The tickets and two partial segments per CTA (one that begins a pair, one that continues it).
 size_t attention_q4_workspace_floats(size_t num_heads, size_t num_kv_heads, size_t head_dim) {
