@@ -319,7 +319,8 @@ class DecodeSession:
     the free list live on the device, and glacier_cuda_kv_resize moves pages between them.  ``step``
     then grows every active lane by one position and takes the positions from there (a lane that
     gets no page has position -1 and ``grow_status`` GLACIER_CUDA_ENOMEM), ``prefill`` appends to a
-    lane, and ``resize`` sets lengths (0 ends a request).
+    lane, and ``resize`` sets lengths (0 ends a request).  A step with FP32 pages reports position -1 as any
+    that is out of range (glacier_cuda_device_status = 2); one with 4-bit pages takes the lane for idle.
     """
 
     def __init__(self, dm: DeviceModel, lanes: int, max_pages: int, reserve_lanes: int | None = None,
@@ -373,9 +374,11 @@ class DecodeSession:
         from . import ops
         if not self.shared:
             raise ValueError("resize needs a session with pool_pages")
-        s = stream if stream is not None else self.torch.cuda.current_stream()
-        with self.torch.cuda.stream(s):
-            self.targets.copy_(self.torch.as_tensor(targets, dtype=self.torch.int32))
+        targets = self.torch.as_tensor(targets, dtype=self.torch.int32)
+        if targets.shape != (self.lanes,):
+            raise ValueError(f"resize: {tuple(targets.shape)} lengths for {self.lanes} lanes")
+        with self.torch.cuda.stream(stream):
+            self.targets.copy_(targets)
         ops.kv_resize(self.lens, self.targets, self.block_tables, self.free_pages, self.free_count, self.grow_status,
                       stream=stream)
         return self.grow_status
@@ -437,14 +440,21 @@ class DecodeSession:
         dev = self.tokens.device
         toks = torch.as_tensor(prompt, dtype=torch.int32).to(dev).contiguous()
         if self.shared:
-            lens = self.lens.tolist()
-            start = lens[lane]
-            lens[lane] += toks.numel()
-            status = self.resize(lens, stream=stream)
-            if stream is not None:
-                stream.synchronize()
-            if int(status[lane]) != 0:
-                raise MemoryError(f"no pages for {toks.numel()} more positions of lane {lane}")
+            with torch.cuda.stream(stream):
+                before = self.lens.tolist()
+                start, after = before[lane], list(before)
+                after[lane] += toks.numel()
+                if int(self.resize(after, stream=stream)[lane]) != 0:
+                    raise MemoryError(f"no pages for {toks.numel()} more positions of lane {lane}")
+            try:
+                return self._prefill(toks, lane, start, eligible, logits, stream)
+            except Exception:
+                self.resize(before, stream=stream)
+                raise
+        return self._prefill(toks, lane, start, eligible, logits, stream)
+
+    def _prefill(self, toks, lane, start, eligible, logits, stream):
+        torch, dev = self.torch, self.tokens.device
         out = torch.empty(1, dtype=torch.int32, device=dev)
         status = torch.empty(1, dtype=torch.int32, device=dev)
         s = stream if stream is not None else torch.cuda.current_stream()

@@ -131,7 +131,8 @@ def argmax_eligible(logits, words=None, stream=None):
 # only a refusal looks for the tensor to name.
 
 _F32, _I32, _I64, _U8 = torch.float32, torch.int32, torch.int64, torch.uint8
-_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# The bare forms of torch.cuda.current_device and current_stream (absent from a torch without CUDA).
+_device, _raw_stream = (getattr(torch._C, n, None) for n in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
 
 
 def _refuse(dev, **tensors):

@@ -193,6 +193,41 @@ def test_an_fp32_pool_can_be_shared_too():
     dm.close()
 
 
+def test_a_prompt_that_is_refused_gives_its_pages_back():
+    from glacier_b200 import _lib
+    m, dm, sess, cos, sin = make(8, 2, 64, 2, 4, pool_pages=6)
+    sess.prefill([1, 2, 3], lane=0)
+    with pytest.raises(_lib.GlacierCudaError):  # a mask of the wrong width
+        sess.prefill([4] * 20, lane=1, eligible=torch.zeros((1, 3), dtype=torch.int64, device="cuda"))
+    assert sess.lens.tolist() == [3, 0] and int(sess.free_count) == 5
+    with pytest.raises(ValueError):
+        sess.resize([5])  # one length for two lanes
+    with pytest.raises(IndexError):
+        sess.prefill([1], lane=2)
+    assert sess.lens.tolist() == [3, 0]
+    sess.close()
+    dm.close()
+
+
+def test_a_prompt_on_another_stream_follows_what_that_stream_still_does():
+    m, dm, sess, cos, sin = make(8, 2, 64, 2, 4, pool_pages=6)
+    ref = int(sess.prefill([1, 2, 3, 4, 5], lane=1)[0])
+    sess.resize([0, 0])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(50):
+            torch.randn((2048, 2048), device="cuda") @ torch.randn((2048, 2048), device="cuda")
+    sess.resize([0, 3], stream=side)  # behind that work: the prompt has to go behind these positions
+    sess.resize([0, 0], stream=side)
+    first = sess.prefill([1, 2, 3], lane=1, stream=side)
+    second = sess.prefill([4, 5], lane=1, stream=side)
+    side.synchronize()
+    assert sess.lens.tolist() == [0, 5] and int(second[0]) == ref
+    sess.close()
+    dm.close()
+
+
 def test_refusals():
     from glacier_b200 import _lib
     from glacier_b200.model import DecodeSession, DeviceModel, ModelConfig, SyntheticModel

@@ -641,6 +641,143 @@ def test_attention_offsets_past_32_bits():
     np.testing.assert_array_equal(host(v)[0], held(x[0, -hd:].cpu().numpy()))
 
 
+# ---- longer and wider, against a vectorised reading of the format ----
+
+def all_values(pool, layer):
+    """float64 (K, V) [pages, hkv, 16, hd] of one layer of a Pool."""
+    hkv, hd = pool.hkv, pool.hd
+    blk = np.ascontiguousarray(np.asarray(pool.data).reshape(-1, pool.layers, hkv, 18 * hd)[:, layer])
+    n, ng = len(blk), hd // 32
+    k = blk[..., :8 * hd].reshape(n, hkv, 16, 4, ng, 4)  # [pos][t][g][byte]: dims 32g + 8t + 2 byte + nibble
+    k = np.stack((k & 15, k >> 4), -1).transpose(0, 1, 2, 4, 3, 5, 6).reshape(n, hkv, 16, hd)
+    v = blk[..., 8 * hd:16 * hd].reshape(n, hkv, 8, hd // 4, 2, 2)  # [pair][w][pos][byte]
+    v = np.stack((v & 15, v >> 4), -1).transpose(0, 1, 2, 4, 3, 5, 6).reshape(n, hkv, 16, hd)
+    s = np.ascontiguousarray(blk[..., 16 * hd:]).view(np.float16).reshape(n, hkv, 2, 8, ng, 2).astype(np.float64)
+    s = s.transpose(2, 0, 1, 3, 5, 4).reshape(2, n, hkv, 16, ng).repeat(32, -1)
+    return (k.astype(np.float64) - 7) * s[0], (v.astype(np.float64) - 7) * s[1]
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_the_vectorised_reading_agrees_with_the_one_by_cell(hd):
+    pool = Pool(random_pool(np.random.default_rng(hd), 3, 2, 2, hd), 2, 2, hd)
+    both = all_values(pool, 1)
+    for kind in (0, 1):
+        np.testing.assert_array_equal(both[kind][[2, 0], 1].reshape(32, hd), pool.rows([2, 0], 32, 1, 1, kind))
+
+
+def check_all(out, q, pool, table, ctxs, h, hkv, hd):
+    """check_attention for every lane, in 64 bits on the GPU."""
+    G = h // hkv
+    with np.errstate(invalid="ignore"):  # left-over scales are NaN and infinite
+        k, v = (torch.from_numpy(x).cuda() for x in all_values(pool, 1))
+    out, q = (torch.from_numpy(x).cuda().double().view(len(ctxs), hkv, G, hd) for x in (out, q))
+    for b, c in enumerate(ctxs):
+        if c == 0:
+            assert not out[b].any()
+            continue
+        pages = torch.from_numpy(table[b, :-(-c // 16)].astype(np.int64)).cuda()
+        kb, vb = (x[pages].transpose(0, 1).reshape(hkv, -1, hd)[:, :c] for x in (k, v))
+        ref = torch.softmax(q[b] @ kb.transpose(1, 2) / hd ** 0.5, -1) @ vb
+        size = (q[b].abs() @ kb.abs().transpose(1, 2)).amax((1, 2)) / hd ** 0.5
+        tol = 2.0 ** -24 * (2 * (hd + 16) * size + 64) * vb.abs().amax((1, 2))
+        err = (out[b] - ref).abs().amax((1, 2))
+        assert (err <= tol).all(), (b, c, err, tol)
+
+
+@gpu
+@pytest.mark.parametrize("ctxs", [[24001], [9000, 0, 7777], [3000, 1, 5000, 16, 2999]])
+@pytest.mark.parametrize("h,hkv,hd", [(14, 2, 64), (28, 4, 128), (4, 4, 128), (5, 1, 64), (8, 1, 128)])
+def test_attention_of_few_lanes_with_long_contexts(h, hkv, hd, ctxs):
+    from glacier_b200 import ops
+    rng = np.random.default_rng(sum(ctxs) + h)
+    q, pool, table = attention_case(rng, h, hkv, hd, ctxs)
+    pages = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd)))
+    out = host(ops.paged_attention_q4(dev(q), pages, dev(table), dev(np.array(ctxs, np.int32)), 2, 1, h, hkv, hd))
+    check_all(out, q, pool, table, ctxs, h, hkv, hd)
+
+
+@gpu
+@pytest.mark.parametrize("seed", range(24))
+def test_attention_of_random_batches(seed):
+    """Lane counts to 1024 and contexts of every spread: shares, pieces and cuts fall everywhere."""
+    from glacier_b200 import ops
+    rng = np.random.default_rng(1000 + seed)
+    h, hkv, hd = HEADS[seed % len(HEADS)]
+    lanes = 1024 if seed == 5 else int(np.exp(rng.uniform(0, np.log(500))))
+    most = max(1, min(6000, 200000 // (lanes * hkv)))
+    hi = int(np.exp(rng.uniform(0, np.log(most + 1))))
+    ctxs = rng.integers(0, hi + 1, lanes)
+    if seed % 3 == 0:
+        ctxs[rng.integers(lanes)] = most  # one lane much longer than the others
+    if seed % 4 == 1:
+        ctxs[:] = hi
+    ctxs = ctxs.tolist()
+    q, pool, table = attention_case(rng, h, hkv, hd, ctxs)
+    pages = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd)))
+    out = host(ops.paged_attention_q4(dev(q), pages, dev(table), dev(np.array(ctxs, np.int32)), 2, 1, h, hkv, hd))
+    check_all(out, q, pool, table, ctxs, h, hkv, hd)
+
+
+@gpu
+@pytest.mark.parametrize("h,hkv,hd", [(28, 4, 128), (8, 8, 64)])
+def test_one_workspace_serves_every_shape_and_graph(h, hkv, hd):
+    """Launches of different shapes, eager and replayed in turn, over a workspace that began with random bits."""
+    from glacier_b200 import ops
+    rng = np.random.default_rng(77)
+    ws = ops.paged_attention_q4_workspace(h, hkv, hd)
+    ws.view(torch.int32).random_(generator=torch.Generator("cuda").manual_seed(1))
+    runs = []
+    for ctxs in ([900, 0, 77], [4000], [100] * 40, list(range(1, 150)), [2500, 17] * 6):
+        q, pool, table = attention_case(rng, h, hkv, hd, ctxs)
+        args = (dev(q), dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd))), dev(table),
+                dev(np.array(ctxs, np.int32)), 2, 1, h, hkv, hd)
+        ref = ops.paged_attention_q4(*args)
+        out = torch.empty_like(ref)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.paged_attention_q4(*args, out=out, workspace=ws)
+        runs.append((args, ref, out, graph))
+    for i in rng.integers(0, 2 * len(runs), 200):
+        args, ref, out, graph = runs[i // 2]
+        out.zero_()
+        if i % 2:
+            graph.replay()
+        else:
+            ops.paged_attention_q4(*args, out=out, workspace=ws)
+        assert torch.equal(out, ref)
+
+
+@gpu
+def test_append_read_and_resize_run_on_the_stream_they_are_given():
+    from glacier_b200 import ops
+    h, hkv, hd = 8, 2, 64
+    i32 = dict(dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    lens, count, status = torch.zeros(3, **i32), torch.full((1,), 8, **i32), torch.full((3,), 9, **i32)
+    table, free = torch.full((3, 4), -1, **i32), torch.arange(8, **i32)
+    pos, who = torch.empty(3, **i32), torch.empty(3, **i32)
+    slots = torch.empty(3, dtype=torch.int64, device="cuda")
+    pages = torch.zeros((8, ops.kv_q4_page_bytes(1, hkv, hd)), dtype=torch.uint8, device="cuda")
+    cos, sin = torch.ones((4, hd // 2), device="cuda"), torch.zeros((4, hd // 2), device="cuda")
+    late, x = torch.zeros(3, **i32), torch.randn((3, (h + 2 * hkv) * hd), device="cuda")
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(50):  # work in front of the targets: another stream would see zeros
+            torch.randn((2048, 2048), device="cuda") @ torch.randn((2048, 2048), device="cuda")
+        late.fill_(1)
+    ops.kv_resize(lens, late, table, free, count, status, positions=pos, row_lanes=who, slots=slots, row_stride=1,
+                  stream=side)
+    q = ops.qkv_rope_append_q4(x, None, cos, sin, pos, slots, h, hkv, hd, pages, 1, 0, stream=side)
+    k, v = ops.kv_q4_read(pages, slots, 1, 0, hkv, hd, stream=side)
+    side.synchronize()
+    assert lens.tolist() == [1, 1, 1] and slots.tolist() == [7 * 16, 6 * 16, 5 * 16]
+    assert torch.equal(q, x[:, :h * hd])
+    for b in range(3):
+        rows = x[b].cpu().numpy().reshape(-1, hd)
+        np.testing.assert_array_equal(host(k)[b], np.concatenate([held(r) for r in rows[h:h + hkv]]))
+        np.testing.assert_array_equal(host(v)[b], np.concatenate([held(r) for r in rows[h + hkv:]]))
+
+
 # ---- together, as a decode loop uses them ----
 
 @gpu
