@@ -411,6 +411,44 @@ def test_resize(name):
         np.testing.assert_array_equal(host(t["free"])[:spare], free[:spare])
 
 
+@gpu
+@pytest.mark.parametrize("seed", range(20))
+def test_resize_of_random_batches(seed):
+    """Any mixture of growth and release, with rows and without: pages and rows from a few to many per thread."""
+    from glacier_b200 import ops
+    rng = np.random.default_rng(500 + seed)
+    lanes = 1024 if seed == 3 else int(np.exp(rng.uniform(0, np.log(700))))
+    max_pages = int(np.exp(rng.uniform(0, np.log(max(2, min(2000, 60000 // lanes))))))
+    kind = seed % 4
+    some = lambda: rng.integers(0, 16 * max_pages + 1, lanes)  # noqa: E731
+    lens = [some, lambda: 0 * some(), some, some][kind]()
+    targets = [some, some, lambda: 0 * some(), lambda: np.minimum(lens + rng.integers(0, 2, lanes), 16 * max_pages)][kind]()
+    pg = -(-lens // 16)
+    spare = int(rng.integers(0, max(2, int((-(-targets // 16)).sum()))) if seed % 5 == 0 else (-(-targets // 16)).sum())
+    perm = rng.permutation(int(pg.sum()) + spare).astype(np.int32)
+    table = np.full((lanes, max_pages), -9, np.int32)
+    table[np.arange(max_pages) < pg[:, None]] = perm[:pg.sum()]
+    free = np.full(len(perm) + 1, -7, np.int32)
+    free[:spare] = perm[pg.sum():]
+    rows = int(np.maximum(targets - lens, 0).sum()) + 3
+    i32 = dict(dtype=torch.int32, device="cuda")
+    new, table2, free2, count2, st, cells, off = resize_ref(lens.tolist(), targets.tolist(), table, free, spare, 0, rows)
+    for with_rows in (False, True):
+        if not with_rows and any(st):
+            continue  # rows that run out are refused too: the same answer only when nothing does
+        t = [dev(x) for x in (lens.astype(np.int32), table, free, np.array([spare], np.int32))]
+        status = torch.full((lanes,), 99, **i32)
+        pos, who = torch.full((rows,), 99, **i32), torch.full((rows,), 99, **i32)
+        slots = torch.full((rows,), 99, dtype=torch.int64, device="cuda")
+        more = dict(positions=pos, row_lanes=who, slots=slots) if with_rows else {}
+        ops.kv_resize(t[0], dev(targets.astype(np.int32)), t[1], t[2], t[3], status, **more)
+        assert host(status).tolist() == st and host(t[0]).tolist() == new and int(t[3]) == count2
+        np.testing.assert_array_equal(host(t[1]), table2)
+        np.testing.assert_array_equal(host(t[2])[:count2], free2[:count2])
+        if with_rows:
+            np.testing.assert_array_equal(np.stack([host(pos), host(who), host(slots)], 1), cells)
+
+
 # ---- attention ----
 
 CTX = {
