@@ -26,6 +26,15 @@
 //     rows 4-7 repeat heads 0-3, columns 4-7 take the low parts, and one instruction does both.
 // The cache's orders put every operand register's codes in one word of one thread: K's words
 // (t, g) and V's 16-bit units by position pair are the fragments of these instructions.
+//
+// What bounds it (B200, 7B heads, graph replay): 64 lanes of 2048 positions take 31.0 us, their 77 MB
+// at the measured copy rate 12.0; from there on 9.8 us for every 1000 positions more, against 5.8. The
+// arithmetic is the slope: 590 instructions per warp and 32 positions, 64 of them mma.sync of 8 to 9
+// cycles each, 935 to 1020 cycles in all with two warps per SM partition (twelve warps of the same code: 31.7
+// us). The rest, some 10 us, is fixed: launch, three dependent loads to the first stage, the merges. Of that
+// much is fetching code that runs once, so the stage and the loads stand in the kernel once (two copies of
+// each: 1 to 3 % slower). Few short contexts are all fixed costs (one lane of 40: 4.9 us, of 1000: 6.2).
+// The fp32 cache's kernel takes 98 us on the layer whose 64 lanes take 32 here.
 #include <algorithm>
 #include <atomic>
 #include <chrono>
@@ -39,8 +48,8 @@ namespace {
 constexpr int kMaxLanes = 1024;
 // Warps per CTA (one CTA per SM) and stages in a warp's ring.  Three warps per SM partition cover each
 // other's latencies better than two, but at hd 128 they have to spill at 168 registers: the 64-lane 7B
-// layer takes 33.6 us with eight warps and 35.5 with twelve, 128 lanes of 1 to 1999 positions at hd 64
-// 31.4 and 29.8 (64 lanes of 2048, with 3 stages a warp: 16.6 and 17.9).  147 and 166 KB of K/V per SM.
+// layer takes 32.3 us with eight warps and 33.3 with twelve (one lane of 1000 positions 6.2 and 7.4), 128
+// lanes of 1 to 1999 positions at hd 64 31.4 and 29.8.  147 and 166 KB of K/V per SM.
 template <int HD>
 constexpr int kWarps = HD == 128 ? 8 : 12;
 template <int HD>
@@ -140,31 +149,34 @@ struct QFrag {
   float f;                // raw score -> base-2 score
 };
 
-// This thread's dims of head lane / 4 (PACK: lane / 4 % 4): 8 t .. 8 t + 7 of every group (zeros past
-// the last head).
+// This thread's dims of head lane / 4 (PACK: lane / 4 % 4): v[2g][..], v[2g + 1][..] are dims 8 t .. 8 t + 7
+// of group g (zeros past the last head).
 template <int HD, bool PACK>
 __device__ __forceinline__ void load_q(const AttnQ4Params& p, int lid, int kvh, int G, int lane,
-                                       float (&v)[HD / 32][8]) {
+                                       float (&v)[HD / 16][4]) {
   const int h = PACK ? lane >> 2 & 3 : lane >> 2, t = lane & 3;
 #pragma unroll
   for (int g = 0; g < HD / 32; ++g) {
+    float x[8];
     if (h < G) {
-      load8(p.q + (size_t)lid * p.ldq + (size_t)(kvh * G + h) * HD + 8 * t + 32 * g, v[g]);
+      load8(p.q + (size_t)lid * p.ldq + (size_t)(kvh * G + h) * HD + 8 * t + 32 * g, x);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[g][i] = 0.f;
+      for (int i = 0; i < 8; ++i) x[i] = 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[2 * g + i / 4][i % 4] = x[i];
   }
 }
 
 template <int HD>
-__device__ __forceinline__ void split_q(const AttnQ4Params& p, const float (&v)[HD / 32][8], QFrag<HD>& q) {
+__device__ __forceinline__ void split_q(const AttnQ4Params& p, const float (&v)[HD / 16][4], QFrag<HD>& q) {
   constexpr int NG = HD / 32;
   float top = 0.f;
 #pragma unroll
   for (int g = 0; g < NG; ++g)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[g][i]));
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[2 * g + i / 4][i % 4]));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
   // A power of two that brings the head's largest |q| into [2^14, 2^15), from the exponent bits.
@@ -179,7 +191,7 @@ __device__ __forceinline__ void split_q(const AttnQ4Params& p, const float (&v)[
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // the word's nibbles pair dims (i, i + 4)
       uint32_t hi, lo;
-      split2(make_float2(v[g][i] * inv, v[g][i + 4] * inv), hi, lo);
+      split2(make_float2(v[2 * g][i] * inv, v[2 * g + 1][i] * inv), hi, lo);
       q.a[2 * g + (i >> 1)][(i & 1) * 2] = hi;
       q.a[2 * g + (i >> 1)][(i & 1) * 2 + 1] = lo;
       const float2 h = __half22float2(bits_h2(hi)), l = __half22float2(bits_h2(lo));
@@ -263,61 +275,65 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
   const float base = m == -INFINITY ? 0.f : -(m * q.f);
   // The stage's sums start from zero and are added with rounding: a tensor core's sums cut, always
   // towards zero, and over ten stages that was 1e-6 of the result (with this, 3e-7; 1.5 % of the time).
-  float sum[HD / 16][4];
+  uint32_t hi[2 * SP], lo[2 * SP];
+  __half2 s9[2 * SP], s8[2 * SP];
+  Words<NW> w[2 * SP];
 #pragma unroll
-  for (int i = 0; i < HD / 16; ++i)
+  for (int pj = 0; pj < 2 * SP; ++pj) {
+    float2 e = __ffma2_rn(sc[pj], make_float2(q.f, q.f), make_float2(base, base));
+    e.x = ex2(e.x);
+    e.y = ex2(e.y);
+    e = __fmul2_rn(e, make_float2(128.f, 128.f));
+    l = __fadd2_rn(l, e);
+    split2(e, hi[pj], lo[pj]);
+    if (PACK && n >= 4) hi[pj] = lo[pj];
+    const uint8_t* V = buf + pj / 2 * BLK + 8 * HD;
+    const uint8_t* S = buf + pj / 2 * BLK + 17 * HD + (n / (8 / NG)) * 4;
+    w[pj] = lds<NW>(V + (t + 4 * (pj & 1)) * HD + n * (4 * NW));
+    // Left-over scales may be anything, and 0 * NaN is NaN.
+    const uint32_t sb = *reinterpret_cast<const uint32_t*>(S + (t + 4 * (pj & 1)) * (4 * NG)) & keep[pj];
+    s9[pj] = __hmul2(bits_h2(sb), __float2half2_rn(9.f));
+    s8[pj] = __hmul2(bits_h2(sb), __float2half2_rn(-0.125f));
+  }
+  constexpr int KC = 2;  // words at a time: four tiles, whose instructions do not wait for one another
 #pragma unroll
-    for (int c = 0; c < 4; ++c) sum[i][c] = 0.f;
+  for (int k0 = 0; k0 < NW; k0 += KC) {
+    float sum[2 * KC][4];
 #pragma unroll
-  for (int pg = 0; pg < SP; ++pg) {
-    uint32_t hi[2], lo[2];
+    for (int i = 0; i < 2 * KC; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float2 e = __ffma2_rn(sc[2 * pg + j], make_float2(q.f, q.f), make_float2(base, base));
-      e.x = ex2(e.x);
-      e.y = ex2(e.y);
-      e = __fmul2_rn(e, make_float2(128.f, 128.f));
-      l = __fadd2_rn(l, e);
-      split2(e, hi[j], lo[j]);
-      if (PACK && n >= 4) hi[j] = lo[j];
-    }
-    const uint8_t* V = buf + pg * BLK + 8 * HD;
-    const uint8_t* S = buf + pg * BLK + 17 * HD + (n / (8 / NG)) * 4;
-    __half2 s9[2], s8[2];
-    Words<NW> w[2];
+      for (int c = 0; c < 4; ++c) sum[i][c] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      w[j] = lds<NW>(V + (t + 4 * j) * HD + n * (4 * NW));
-      // Left-over scales may be anything, and 0 * NaN is NaN.
-      const uint32_t sb = *reinterpret_cast<const uint32_t*>(S + (t + 4 * j) * (4 * NG)) & keep[2 * pg + j];
-      s9[j] = __hmul2(bits_h2(sb), __float2half2_rn(9.f));
-      s8[j] = __hmul2(bits_h2(sb), __float2half2_rn(-0.125f));
-    }
-    // A tile's rows g and g + 8 are dims 4k + i and 4k + i + 1 of this thread's sixteen (eight at hd 64).
+    for (int pg = 0; pg < SP; ++pg) {
+      // A tile's rows g and g + 8 are dims 4k + i and 4k + i + 1 of this thread's sixteen (eight at hd 64).
 #pragma unroll
-    for (int k = 0; k < NW; ++k) {
+      for (int k = 0; k < KC; ++k) {
 #pragma unroll
-      for (int i = 0; i < 4; i += 2) {
-        uint32_t a[4];
+        for (int i = 0; i < 4; i += 2) {
+          uint32_t a[4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t x = w[j].w[k];
-          a[2 * j] = h2_bits(__hfma2(bits_h2(v_bits(i == 0 ? x * 16u : x >> 4)), s8[j], s9[j]));
-          a[2 * j + 1] = h2_bits(__hfma2(bits_h2(v_bits(i == 0 ? x : x >> 8)), s8[j], s9[j]));
+          for (int j = 0; j < 2; ++j) {
+            const int pj = 2 * pg + j;
+            const uint32_t x = w[pj].w[k0 + k];
+            a[2 * j] = h2_bits(__hfma2(bits_h2(v_bits(i == 0 ? x * 16u : x >> 4)), s8[pj], s9[pj]));
+            a[2 * j + 1] = h2_bits(__hfma2(bits_h2(v_bits(i == 0 ? x : x >> 8)), s8[pj], s9[pj]));
+          }
+          float(&d)[4] = sum[2 * k + i / 2];
+          mma_f16(d, a, hi[2 * pg], hi[2 * pg + 1], d);
+          if constexpr (!PACK) mma_f16(d, a, lo[2 * pg], lo[2 * pg + 1], d);
         }
-        mma_f16(sum[2 * k + i / 2], a, hi[0], hi[1], sum[2 * k + i / 2]);
-        if constexpr (!PACK) mma_f16(sum[2 * k + i / 2], a, lo[0], lo[1], sum[2 * k + i / 2]);
       }
     }
+#pragma unroll
+    for (int i = 0; i < 2 * KC; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; c += 2) {
+        float(&d)[4] = o[2 * k0 + i];
+        const float2 r = __fadd2_rn(make_float2(d[c], d[c + 1]), make_float2(sum[i][c], sum[i][c + 1]));
+        d[c] = r.x;
+        d[c + 1] = r.y;
+      }
   }
-#pragma unroll
-  for (int i = 0; i < HD / 16; ++i)
-#pragma unroll
-    for (int c = 0; c < 4; c += 2) {
-      const float2 r = __fadd2_rn(make_float2(o[i][c], o[i][c + 1]), make_float2(sum[i][c], sum[i][c + 1]));
-      o[i][c] = r.x;
-      o[i][c + 1] = r.y;
-    }
 }
 
 // A walk over the pairs of a warp's share [g0, g1) and its segment [sb, se) of each.  All (lane,
@@ -616,8 +632,8 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
   __syncwarp();  // ctx and the state word are this warp's own writes
 
   if (use.lid >= 0) {
-    float v[HD / 32][8];
-    load_q<HD, PACK>(p, use.lid, use.kvh, G, lane, v);
+    float o[HD / 16][4];  // between pairs it holds the next one's q, which costs no registers then
+    load_q<HD, PACK>(p, use.lid, use.kvh, G, lane, o);
     // ---- loads: the warp's stages in order, the ring kept full ----
     PairWalk<HD> ld = use;
     const uint64_t pol = l2_evict_first_policy();
@@ -677,50 +693,55 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
 
     // ---- arithmetic ----
     int slot = 0;
-    bool more = true;
+    bool fresh = true;  // a pair begins
     const int h = lane >> 2, t = lane & 3;
-    while (more) {
-      QFrag<HD> q;
-      split_q<HD>(p, v, q);
-      const PairWalk<HD> done = use;
-      more = use.next(ctx, hkv, g0, g1);
-      if (more) load_q<HD, PACK>(p, use.lid, use.kvh, G, lane, v);  // arrives while this pair is worked on
-      float m = -INFINITY;
-      float2 l2 = make_float2(0.f, 0.f);
-      float o[HD / 16][4];
-#pragma unroll
-      for (int i = 0; i < HD / 16; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
-      int left = ctx[done.lid] - SPOS * done.sb;  // positions from this stage on
-      for (int st = done.sb; st < done.se; ++st, left -= SPOS) {
-        __syncwarp();  // nobody reads the slot of the stage before any more
+    QFrag<HD> q;
+    float m = -INFINITY;
+    float2 l2 = make_float2(0.f, 0.f);
+    int st = 0, left = 0;
 #pragma unroll 1
-        for (; ahead < NST; ++ahead) issue();
-        --ahead;
-        cp_async_wait<NST - 1>();
-        __syncwarp();  // this stage is there for every thread
-        const uint32_t pages = (loaded >> (SP * slot)) & ALL;
-        const uint8_t* buf = ring + slot * (SP * BLK);
-        float2 sc[2 * SP];
-        stage_scores<HD>(buf, q, sc, lane);
-        uint32_t keep[2 * SP];
+    for (;;) {
+      __syncwarp();  // nobody reads the slot of the stage before any more
+#pragma unroll 1
+      for (; ahead < NST; ++ahead) issue();
+      --ahead;
+      if (fresh) {
+        split_q<HD>(p, o, q);
+        m = -INFINITY;
+        l2 = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 2 * SP; ++i) keep[i] = 0xffffffffu;
-        if (left < SPOS || pages != ALL) {
-          // Positions past the context, and of pages that are not there.
+        for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
-          for (int i = 0; i < 2 * SP; ++i) {
-            const int in = (pages >> (i / 2) & 1) ? left - 8 * i - 2 * t : 0;  // this thread's two positions
-            if (in < 1) sc[i].x = -INFINITY;
-            if (in < 2) sc[i].y = -INFINITY;
-            keep[i] = in < 1 ? 0u : in < 2 ? 0xffffu : 0xffffffffu;
-          }
-        }
-        stage_values<HD, PACK>(buf, q, sc, keep, m, l2, o, lane);
-        slot = slot + 1 == NST ? 0 : slot + 1;
+          for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
+        st = use.sb;
+        left = ctx[use.lid] - SPOS * st;  // positions from this stage on
+        fresh = false;
       }
+      cp_async_wait<NST - 1>();
+      __syncwarp();  // this stage is there for every thread
+      const uint32_t pages = (loaded >> (SP * slot)) & ALL;
+      const uint8_t* buf = ring + slot * (SP * BLK);
+      float2 sc[2 * SP];
+      stage_scores<HD>(buf, q, sc, lane);
+      uint32_t keep[2 * SP];
+#pragma unroll
+      for (int i = 0; i < 2 * SP; ++i) keep[i] = 0xffffffffu;
+      if (left < SPOS || pages != ALL) {
+        // Positions past the context, and of pages that are not there.
+#pragma unroll
+        for (int i = 0; i < 2 * SP; ++i) {
+          const int in = (pages >> (i / 2) & 1) ? left - 8 * i - 2 * t : 0;  // this thread's two positions
+          if (in < 1) sc[i].x = -INFINITY;
+          if (in < 2) sc[i].y = -INFINITY;
+          keep[i] = in < 1 ? 0u : in < 2 ? 0xffffu : 0xffffffffu;
+        }
+      }
+      stage_values<HD, PACK>(buf, q, sc, keep, m, l2, o, lane);
+      slot = slot + 1 == NST ? 0 : slot + 1;
+      left -= SPOS;
+      if (++st < use.se) continue;
       __syncwarp();  // the last stage is read
+      const PairWalk<HD> done = use;
       float l = l2.x + l2.y;
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -759,6 +780,9 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
         if (begins || warp == 0) s_first[which][warp] = done.P + 1;
         s_pair[which][warp] = done.lid * hkv + done.kvh;
       }
+      if (!use.next(ctx, hkv, g0, g1)) break;
+      load_q<HD, PACK>(p, use.lid, use.kvh, G, lane, o);
+      fresh = true;
     }
   }
   if constexpr (CLUSTER) {
