@@ -28,13 +28,14 @@
 // (t, g) and V's 16-bit units by position pair are the fragments of these instructions.
 //
 // What bounds it (B200, 7B heads, graph replay): 64 lanes of 2048 positions take 31.0 us, their 77 MB
-// at the measured copy rate 12.0; from there on 9.8 us for every 1000 positions more, against 5.8. The
-// arithmetic is the slope: 590 instructions per warp and 32 positions, 64 of them mma.sync of 8 to 9
-// cycles each, 935 to 1020 cycles in all with two warps per SM partition (twelve warps of the same code: 31.7
-// us). The rest, some 10 us, is fixed: launch, three dependent loads to the first stage, the merges. Of that
-// much is fetching code that runs once, so the stage and the loads stand in the kernel once (two copies of
-// each: 1 to 3 % slower). Few short contexts are all fixed costs (one lane of 40: 4.9 us, of 1000: 6.2).
-// The fp32 cache's kernel takes 98 us on the layer whose 64 lanes take 32 here.
+// at the measured copy rate 12.0; from there on 9.6 us for every 1000 positions more, against 5.7. The
+// slope is arithmetic and its dependences (with all pages in L2 it is the same, and the loads alone run
+// at the copy rate): 640 instructions per warp and 32 positions, 64 of them mma.sync of 8 cycles, with two
+// warps per SM partition take 1400 cycles, twice what their issue does. The rest, some 10 us, is
+// fixed: launch, three dependent loads to the first stage, the merges. Of that much is fetching code that
+// runs once, so the stage and the loads stand in the kernel once (two copies of each: 1 to 3 % slower). Few
+// short contexts are all fixed costs (one lane of 40: 4.8 us, of 1000: 6.2). The FP32 cache's kernel takes 98
+// us on the layer whose 64 lanes (256 to 4096 positions) take 32 here.
 #include <algorithm>
 #include <atomic>
 #include <chrono>

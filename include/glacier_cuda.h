@@ -245,7 +245,8 @@ int glacier_cuda_kv_q4_read_f32(const void *pool, size_t num_pages, size_t num_l
  * of a page id outside the pool are left out and raise the bad-input status.  Scores, the softmax
  * and its sums are float32; held values enter the products exactly.  q, out and workspace are
  * 16-byte aligned; workspace: glacier_cuda_paged_attention_q4_workspace() floats, any contents,
- * not shared with a call that may run at the same time. */
+ * not shared with a call that may run at the same time.  At most 2^26 pages per lane, and lanes *
+ * num_kv_heads * max_pages below 2^31; a page has less than 2^32 bytes. */
 size_t glacier_cuda_paged_attention_q4_workspace(size_t num_heads, size_t num_kv_heads, size_t head_dim);
 int glacier_cuda_paged_attention_q4(const float *q, const void *pool, size_t num_pages, size_t num_layers,
                                     const int32_t *block_tables, size_t max_pages, const int32_t *ctx_lens,
@@ -267,7 +268,8 @@ int glacier_cuda_paged_attention_q4(const float *q, const void *pool, size_t num
  * The new positions as rows (all three arrays or none): positions, row_lanes and slots (page * 16 + row)
  * of `rows` rows, -1 in rows without a position.  row_stride 0 packs the lanes' rows one after another;
  * row_stride s gives lane b the rows from b * s (rows = lanes * s).  row_offsets [lanes + 1] (may be
- * NULL): each lane's first row and the end.  lens, targets and the outputs are different arrays. */
+ * NULL): each lane's first row and the end.  lens, targets and the outputs are different arrays.  At
+ * most 2^26 pages per lane; lanes * max_pages, capacity and rows are below 2^31. */
 int glacier_cuda_kv_resize(int32_t *lens, const int32_t *targets, size_t lanes, int32_t *block_tables,
                            size_t max_pages, int32_t *free_pages, size_t capacity, int32_t *free_count,
                            int32_t *status, size_t row_stride, size_t rows, int32_t *positions,
