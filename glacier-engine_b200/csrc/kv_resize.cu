@@ -206,8 +206,8 @@ __global__ void __launch_bounds__(kMaxLanes, 1) kv_resize_kernel(const ResizePar
     } else {
       // A lane's pages to a group of threads (as many as a lane has pages on average, a warp at most), or
       // to several when there are more groups than lanes: four per thread, loads before stores.
-      const int size = 1 << min(5, 31 - __clz(max(1, moves / p.lanes)));
-      const int groups = (int)(all / size), per = max(1, groups / p.lanes), group = (int)(me / size);
+      const int log = min(5, 31 - __clz(max(1, moves / p.lanes))), size = 1 << log;
+      const int groups = (int)(all >> log), per = max(1, groups / p.lanes), group = (int)(me >> log);
 #pragma unroll 1
       for (int b = group / per; b < p.lanes; b += groups / per) {
         const int old_pages = pages_of(s_old[b]), diff = s_new[b] < 0 ? 0 : pages_of(s_new[b]) - old_pages;

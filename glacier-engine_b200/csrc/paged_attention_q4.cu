@@ -31,10 +31,10 @@
 // at the measured copy rate 12.0; from there on 9.6 us for every 1000 positions more, against 5.7. The
 // slope is arithmetic and its dependences (with all pages in L2 it is the same, and the loads alone run
 // at the copy rate): 640 instructions per warp and 32 positions, 64 of them mma.sync of 8 cycles, with two
-// warps per SM partition take 1400 cycles, twice what their issue does. The rest, some 10 us, is
-// fixed: launch, three dependent loads to the first stage, the merges. Of that much is fetching code that
-// runs once, so the stage and the loads stand in the kernel once (two copies of each: 1 to 3 % slower). Few
-// short contexts are all fixed costs (one lane of 40: 4.8 us, of 1000: 6.2). The FP32 cache's kernel takes 98
+// warps per SM partition take 1400 cycles, twice what their issue does. The rest, some 10 us (7 when no
+// pair is cut between CTAs), is fixed: launch, three dependent loads to the first stage, the merges. Of that
+// much is fetching code that runs once, so the stage and the loads stand in the kernel once (two copies of each: 1 to 3 % slower). Few
+// short contexts are all fixed costs (one lane of 40: 4.7 us, of 1000: 6.1). The FP32 cache's kernel takes 98
 // us on the layer whose 64 lanes (256 to 4096 positions) take 32 here.
 #include <algorithm>
 #include <atomic>
@@ -49,7 +49,7 @@ namespace {
 constexpr int kMaxLanes = 1024;
 // Warps per CTA (one CTA per SM) and stages in a warp's ring.  Three warps per SM partition cover each
 // other's latencies better than two, but at hd 128 they have to spill at 168 registers: the 64-lane 7B
-// layer takes 32.3 us with eight warps and 33.3 with twelve (one lane of 1000 positions 6.2 and 7.4), 128
+// layer takes 32.3 us with eight warps and 33.3 with twelve (one lane of 1000 positions 6.1 and 7.4), 128
 // lanes of 1 to 1999 positions at hd 64 31.4 and 29.8.  147 and 166 KB of K/V per SM.
 template <int HD>
 constexpr int kWarps = HD == 128 ? 8 : 12;
@@ -401,10 +401,30 @@ __device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ct
   const int warps = gridDim.x * kWarps<HD>;
   const int Q = max(1, (int)(((unsigned)total + warps - 1) / (unsigned)warps));
   start.lid = -1;
-  g0 = g1 = 0;
-  if ((long long)gw * Q >= total) return Q;
-  g0 = gw * Q;
-  g1 = min(total - g0, Q) + g0;
+  // Whole pairs to every CTA, if that is a unit per warp more at most: then no pair is cut between CTAs,
+  // and there is no merge over memory (7B heads, 64 lanes of 100 positions: 10.6 us with cuts, 7.6
+  // without; of 1200 22.0 and 21.0). Two units more are too many (20 lanes of 1200 13.0 and 13.5).
+  const unsigned ctas = gridDim.x, hkv = p.num_kv_heads, pairs = p.lanes * hkv;
+  const int longest = __reduce_max_sync(0xffffffffu, max(max(ns[0], ns[1]), max(ns[2], ns[3])));
+  if (p.lanes <= 128 && (unsigned long long)((pairs + ctas - 1) / ctas) * longest <= (Q + 1ull) * kWarps<HD>) {
+    const int e = incl - (ns[0] + ns[1] + ns[2] + ns[3]);
+    auto first_unit = [&](unsigned pair) {
+      const unsigned b = pair / hkv, i = b & 3;
+      const int before = e + (i > 0 ? ns[0] : 0) + (i > 1 ? ns[1] : 0) + (i > 2 ? ns[2] : 0);
+      const int n = i == 0 ? ns[0] : i == 1 ? ns[1] : i == 2 ? ns[2] : ns[3];
+      const int first = __shfl_sync(0xffffffffu, before, b >> 2) * hkv + (pair - b * hkv) * __shfl_sync(0xffffffffu, n, b >> 2);
+      return pair == pairs ? total : first;  // c * pairs < 2^32: 128 lanes of 1024 heads
+    };
+    const unsigned c = blockIdx.x;
+    const int w = gw - c * kWarps<HD>, from = first_unit(c * pairs / ctas), to = first_unit((c + 1) * pairs / ctas);
+    const int each = (to - from + kWarps<HD> - 1) / kWarps<HD>;
+    g0 = min(from + w * each, to);
+    g1 = min(g0 + each, to);
+  } else {
+    g0 = (int)min((long long)gw * Q, (long long)total);
+    g1 = min(total - g0, Q) + g0;
+  }
+  if (g0 >= g1) return Q;
   const int at = (unsigned)g0 / (unsigned)p.num_kv_heads;  // lane b holds g0 when its sums straddle `at`
   int before = 0;
   for (int b0 = 0;; b0 += 128) {
@@ -620,10 +640,12 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
     if (part >= nclusters) return;  // the whole cluster
     if (part == 0 && nclusters > 1 && cluster_ctarank() == 0 && threadIdx.x < G)
       open_ticket(p.tickets + pair * G + threadIdx.x, p.nonce);
-    constexpr long long W = kClusterCtas * kWarps<HD>;
-    const long long w = part * W + (int)cluster_ctarank() * kWarps<HD> + warp, all = nclusters * W;
-    use.sb = g0 = (int)(use.ns * w / all);
-    use.se = g1 = (int)(use.ns * (w + 1) / all);
+    // [ns w / all, ns (w + 1) / all), in 32 bits (a 64-bit division takes 0.1 us here).
+    constexpr unsigned W = kClusterCtas * kWarps<HD>;
+    const unsigned w = part * W + cluster_ctarank() * kWarps<HD> + warp, all = nclusters * W;
+    const unsigned each = use.ns / all, rest = use.ns - each * all;
+    use.sb = g0 = (int)(each * w + rest * w / all);
+    use.se = g1 = (int)(each * (w + 1) + rest * (w + 1) / all);
     if (use.sb == use.se) use.lid = -1;
   } else {
     if (threadIdx.x < G) open_ticket(p.tickets + 8 * blockIdx.x + threadIdx.x, p.nonce);

@@ -459,6 +459,11 @@ CTX = {
     "one long": [2111],
     "ragged": [1, 700, 33, 1290, 64, 2, 255, 16],
     "many short lanes": [(i * 37) % 90 for i in range(300)],
+    "37 lanes alike": [333] * 37,
+    "127 lanes nearly alike": [64 + i % 9 for i in range(127)],
+    "128 lanes alike": [100] * 128,
+    "129 lanes alike": [100] * 129,
+    "lanes alike, some empty": [0 if i % 5 == 4 else 200 for i in range(90)],
 }
 HEADS = [(14, 2, 64), (28, 4, 128), (8, 8, 64), (3, 3, 128), (16, 2, 128), (5, 1, 64), (8, 2, 64), (6, 1, 128)]
 
