@@ -27,15 +27,16 @@
 // The cache's orders put every operand register's codes in one word of one thread: K's words
 // (t, g) and V's 16-bit units by position pair are the fragments of these instructions.
 //
-// What bounds it (B200, 7B heads, graph replay): 64 lanes of 2048 positions take 31.0 us, their 77 MB
-// at the measured copy rate 12.0; from there on 9.6 us for every 1000 positions more, against 5.7. The
+// What bounds it (B200, 7B heads, graph replay): 64 lanes of 2048 positions take 30.2 us, their 77 MB
+// at the measured copy rate 12.0; from there on 8.6 us for every 1000 positions more, against 5.7. The
 // slope is arithmetic and its dependences (with all pages in L2 it is the same, and the loads alone run
-// at the copy rate): 640 instructions per warp and 32 positions, 64 of them mma.sync of 8 cycles, with two
-// warps per SM partition take 1400 cycles, twice what their issue does. The rest, some 10 us (7 when no
-// pair is cut between CTAs), is fixed: launch, three dependent loads to the first stage, the merges. Of that
-// much is fetching code that runs once, so the stage and the loads stand in the kernel once (two copies of each: 1 to 3 % slower). Few
-// short contexts are all fixed costs (one lane of 40: 4.7 us, of 1000: 6.1). The FP32 cache's kernel takes 98
-// us on the layer whose 64 lanes (256 to 4096 positions) take 32 here.
+// at the copy rate): some 600 instructions per warp and 32 positions, 64 of them mma.sync of 8 cycles, with
+// two warps per SM partition take 1250 cycles, twice what their issue does. The rest, some 10 us (7 when no
+// pair is cut between CTAs), is fixed: launch, three dependent loads to the first stage, the merges. Of
+// that much is fetching code that runs once, so the stage and the loads stand in the kernel once (two
+// copies of each: 1 to 3 % slower). Few short contexts are all fixed costs (one lane of 40: 4.7 us, of
+// 1000: 6.1). The FP32 cache's kernel takes 98 us on the layer whose 64 lanes (256 to 4096 positions) take
+// 30 here.
 #include <algorithm>
 #include <atomic>
 #include <chrono>
@@ -47,22 +48,22 @@ namespace glacier {
 namespace {
 
 constexpr int kMaxLanes = 1024;
-// Warps per CTA (one CTA per SM) and stages in a warp's ring.  Three warps per SM partition cover each
-// other's latencies better than two, but at hd 128 they have to spill at 168 registers: the 64-lane 7B
-// layer takes 32.3 us with eight warps and 33.3 with twelve (one lane of 1000 positions 6.1 and 7.4), 128
-// lanes of 1 to 1999 positions at hd 64 31.4 and 29.8.  147 and 166 KB of K/V per SM.
+// Warps per CTA (one CTA per SM).  Three warps per SM partition cover each other's latencies better than
+// two, but at hd 128 they have to spill at 168 registers: with stages of 32 positions the 64-lane 7B layer takes
+// 32.3 us with eight warps and 33.3 with twelve (one lane of 1000 positions 6.1 and 7.4), 128 lanes of 1 to 1999 positions at hd 64 31.4
+// and 29.8.
 template <int HD>
 constexpr int kWarps = HD == 128 ? 8 : 12;
-template <int HD>
-constexpr int kStages = HD == 128 ? 4 : 3;
+// Pages per stage: 64 positions, which spread the softmax's chain and the loop over twice the products
+// of 32 (the 64-lane 7B layer 30.1 and 32.2 us; 64 lanes of 512 13.7 and 13.0).  The cluster form at hd 128
+// takes 32: one lane of 1000 positions 6.1 us, with 64 6.7; of 2000 7.6 and 7.1, of 6000 10.3 and 11.9.
+template <int HD, bool CLUSTER>
+constexpr int kStagePages = HD == 128 && CLUSTER ? 2 : 4;
+// Stages in a warp's ring: 147 and 166 KB of K/V per SM.
+template <int HD, bool CLUSTER>
+constexpr int kStages = HD == 64 ? 3 : CLUSTER ? 4 : 2;
 constexpr int kClusterCtas = 4;
 constexpr int kPart = 4;  // heads that a warp merges at once, at most
-// Pages per stage: 4608 bytes at either head size.
-template <int HD>
-constexpr int kStagePages = HD == 128 ? 2 : 4;
-template <int HD>
-constexpr int kStagePos = kStagePages<HD> * kQ4Page;
-
 struct AttnQ4Params {
   const float* q;
   size_t ldq;
@@ -210,14 +211,14 @@ __device__ __forceinline__ void split_q(const AttnQ4Params& p, const float (&v)[
 
 // Raw scores of one stage: sc[2 page + half] = the scores of head lane / 4 with the positions
 // 8 half + 2 (lane % 4) + {0, 1} of the page.
-template <int HD>
+template <int HD, int SP>
 __device__ __forceinline__ void stage_scores(const uint8_t* __restrict__ buf, const QFrag<HD>& q,
-                                             float2 (&sc)[2 * kStagePages<HD>], int lane) {
+                                             float2 (&sc)[2 * SP], int lane) {
   constexpr int NG = HD / 32;  // scale groups = words per thread and position
   constexpr int BLK = 18 * HD;
   const int n = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int pg = 0; pg < kStagePages<HD>; ++pg) {
+  for (int pg = 0; pg < SP; ++pg) {
     const uint8_t* K = buf + pg * BLK;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -245,12 +246,12 @@ __device__ __forceinline__ void stage_scores(const uint8_t* __restrict__ buf, co
 // below 2^15 and their low parts normal fp16 numbers.  l: this thread's share of their
 // sum; o: sums of weight * v / 8.
 // keep: masks of the V scales, one per eight positions (two positions a word).
-template <int HD, bool PACK>
+template <int HD, int SP, bool PACK>
 __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, const QFrag<HD>& q,
-                                             float2 (&sc)[2 * kStagePages<HD>], const uint32_t (&keep)[2 * kStagePages<HD>],
+                                             float2 (&sc)[2 * SP], const uint32_t (&keep)[2 * SP],
                                              float& m, float2& l, float (&o)[HD / 16][4], int lane) {
   constexpr int NG = HD / 32, NW = HD / 32;  // scale groups; words per thread and position pair
-  constexpr int BLK = 18 * HD, SP = kStagePages<HD>;
+  constexpr int BLK = 18 * HD;
   const int n = lane >> 2, t = lane & 3;
   float mx = fmaxf(sc[0].x, sc[0].y);
 #pragma unroll
@@ -341,11 +342,11 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
 // kv head) pairs are laid end to end, lane-major, each with a unit for every stage and one in front
 // for the change of pair (it takes about a stage's time), and warp w of the grid takes units
 // [w Q, (w + 1) Q): every warp does the same work.
-template <int HD>
+template <int SP>
 struct PairWalk {
   int lid, kvh, ns, sb, se;
   int P;  // the pair's first unit
-  __device__ __forceinline__ static int stages(int ctx) { return (ctx + kStagePos<HD> - 1) / kStagePos<HD>; }
+  __device__ __forceinline__ static int stages(int ctx) { return (ctx + SP * kQ4Page - 1) / (SP * kQ4Page); }
   __device__ __forceinline__ static int units(int ctx) { return ctx > 0 ? stages(ctx) + 1 : 0; }
   __device__ __forceinline__ void set(const int* ctx, int g0, int g1) {
     ns = stages(ctx[lid]);
@@ -370,8 +371,8 @@ struct PairWalk {
 // holds the share's first one.  ctx: clamped contexts, for the block.  Returns Q; start.lid = -1 when
 // the share is empty.  A chunk of 128 lanes is four consecutive ones per thread; the first chunk
 // stays in registers.
-template <int HD>
-__device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ctx, PairWalk<HD>& start, int& g0,
+template <int HD, int SP>
+__device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ctx, PairWalk<SP>& start, int& g0,
                                           int& g1) {
   const int lane = threadIdx.x & 31;
   const int cap = p.max_pages * kQ4Page;
@@ -382,7 +383,7 @@ __device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ct
       const int b = b0 + 4 * lane + i;
       const int c = b < p.lanes ? min(max(p.ctx_lens[b], 0), cap) : 0;
       if (b < p.lanes) ctx[b] = c;  // every warp writes the same values, and reads its own
-      ns[i] = PairWalk<HD>::units(c);
+      ns[i] = PairWalk<SP>::units(c);
     }
     __syncwarp();
     incl = ns[0] + ns[1] + ns[2] + ns[3];
@@ -607,8 +608,8 @@ __device__ __forceinline__ void merge_cluster(const AttnQ4Params& p, uint8_t* sm
 // distributed shared memory in rank order.
 template <int HD, bool CLUSTER, bool PACK>
 __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ4Params p) {
-  constexpr int BLK = 18 * HD, SP = kStagePages<HD>, SPOS = kStagePos<HD>;
-  constexpr int NST = kStages<HD>, IDS = 32 / SP;
+  constexpr int BLK = 18 * HD, SP = kStagePages<HD, CLUSTER>, SPOS = SP * kQ4Page;
+  constexpr int NST = kStages<HD, CLUSTER>, IDS = 32 / SP;
   constexpr uint32_t ALL = (1u << SP) - 1;
   constexpr int ROW = HD + 4;  // floats per head of a state
   constexpr int RING = NST * SP * BLK;
@@ -623,7 +624,7 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
   griddep_wait();  // q, the pages, tables and lengths come from earlier kernels
   uint8_t* ring = smem + (size_t)warp * RING;
   float* state_a = reinterpret_cast<float*>(smem + (size_t)kWarps<HD> * RING);  // [warps][G][ROW]
-  PairWalk<HD> use;
+  PairWalk<SP> use;
   int g0 = 0, g1 = 0;
   int Q = 0, pair = 0, nclusters = 1;  // cluster form: the CTA's pair and its clusters
   if constexpr (CLUSTER) {
@@ -633,7 +634,7 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
     use.kvh = pair - use.lid * hkv;
     const int c = min(max(p.ctx_lens[use.lid], 0), p.max_pages * kQ4Page);
     ctx[use.lid] = c;  // every warp writes the same value
-    use.ns = PairWalk<HD>::stages(c);
+    use.ns = PairWalk<SP>::stages(c);
     use.P = 0;
     nclusters = pair_clusters<HD>(use.ns, p.clusters);
     const int part = cluster - pair * p.clusters;
@@ -649,7 +650,7 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
     if (use.sb == use.se) use.lid = -1;
   } else {
     if (threadIdx.x < G) open_ticket(p.tickets + 8 * blockIdx.x + threadIdx.x, p.nonce);
-    Q = find_share<HD>(p, blockIdx.x * kWarps<HD> + warp, ctx, use, g0, g1);
+    Q = find_share<HD, SP>(p, blockIdx.x * kWarps<HD> + warp, ctx, use, g0, g1);
   }
   if (lane == 0) s_state[warp] = 0;
   __syncwarp();  // ctx and the state word are this warp's own writes
@@ -658,7 +659,7 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
     float o[HD / 16][4];  // between pairs it holds the next one's q, which costs no registers then
     load_q<HD, PACK>(p, use.lid, use.kvh, G, lane, o);
     // ---- loads: the warp's stages in order, the ring kept full ----
-    PairWalk<HD> ld = use;
+    PairWalk<SP> ld = use;
     const uint64_t pol = l2_evict_first_policy();
     int ld_st = 0, ld_at = 0;  // next stage; its place among the stages whose page ids `ids` holds
     int32_t ids = 0;
@@ -745,7 +746,7 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
       const uint32_t pages = (loaded >> (SP * slot)) & ALL;
       const uint8_t* buf = ring + slot * (SP * BLK);
       float2 sc[2 * SP];
-      stage_scores<HD>(buf, q, sc, lane);
+      stage_scores<HD, SP>(buf, q, sc, lane);
       uint32_t keep[2 * SP];
 #pragma unroll
       for (int i = 0; i < 2 * SP; ++i) keep[i] = 0xffffffffu;
@@ -759,12 +760,12 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
           keep[i] = in < 1 ? 0u : in < 2 ? 0xffffu : 0xffffffffu;
         }
       }
-      stage_values<HD, PACK>(buf, q, sc, keep, m, l2, o, lane);
+      stage_values<HD, SP, PACK>(buf, q, sc, keep, m, l2, o, lane);
       slot = slot + 1 == NST ? 0 : slot + 1;
       left -= SPOS;
       if (++st < use.se) continue;
       __syncwarp();  // the last stage is read
-      const PairWalk<HD> done = use;
+      const PairWalk<SP> done = use;
       float l = l2.x + l2.y;
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -883,7 +884,7 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
           if (lane == g) mine = make_float2(M[g], L[g]);
         }
         if (lane < heads) *reinterpret_cast<float2*>(p.part_ml + (part + lane) * 2) = mine;
-        const int units = Q * kWarps<HD>, begin = s_first[chain ? 1 : 0][first], ns = PairWalk<HD>::stages(ctx[pair / hkv]);
+        const int units = Q * kWarps<HD>, begin = s_first[chain ? 1 : 0][first], ns = PairWalk<SP>::stages(ctx[pair / hkv]);
         const int c0 = begin / units, n = (begin + ns - 1) / units - c0 + 1;  // its first CTA, its CTAs
         __syncwarp();
         bool last = false;
@@ -1003,10 +1004,12 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
                                 attn_q4_kernel<128, false, false>, attn_q4_kernel<128, false, true>,
                                 attn_q4_kernel<128, true, false>,  attn_q4_kernel<128, true, true>};
   const Kern kern = kerns[(head_dim == 128 ? 4 : 0) + (cluster ? 2 : 0) + (G <= 4 ? 1 : 0)];
-  const size_t pages = head_dim == 128 ? kStagePages<128> : kStagePages<64>;
   const size_t warps = head_dim == 128 ? kWarps<128> : kWarps<64>;
-  const size_t stages = head_dim == 128 ? kStages<128> : kStages<64>;
-  const size_t smem = warps * (stages * pages * q4_block_bytes(head_dim) + G * (head_dim + 4) * sizeof(float));
+  const size_t pages = head_dim == 128 ? (cluster ? kStagePages<128, true> * kStages<128, true>
+                                                  : kStagePages<128, false> * kStages<128, false>)
+                                       : kStagePages<64, true> * kStages<64, true>;  // of a warp's ring
+  static_assert(kStagePages<64, true> * kStages<64, true> == kStagePages<64, false> * kStages<64, false>);
+  const size_t smem = warps * (pages * q4_block_bytes(head_dim) + G * (head_dim + 4) * sizeof(float));
   if ((rc = allow_dynamic_smem((const void*)kern, (int)smem))) return rc;
   if (cluster)
     return launch_pdl(kern, dim3((unsigned)(pairs * p.clusters * kClusterCtas)), dim3((unsigned)warps * 32), smem,
