@@ -70,11 +70,11 @@ __device__ __forceinline__ int holder(const int* first, int n, int i) {
 __device__ __forceinline__ int pages_of(int positions) { return (positions + kQ4Page - 1) / kQ4Page; }
 
 // Every CTA works the whole batch out for itself (a thread per lane, two scans over the warps that
-// have lanes): that takes less time than passing results on.  The stack's order is arithmetic: pages that shrinking
-// lanes give back lie above the old top so that the next pops return them in lane and page order
-// (growing again undoes the shrink), and growing lanes pop in lane order.  A page that is
-// given back and taken in one call is therefore found in the table it comes from, and nothing waits
-// for another thread's writes.  Once the pages or rows run out, that lane and every later one that
+// have lanes): that takes less time than passing results on.  The stack's order is arithmetic: pages
+// that shrinking lanes give back lie above the old top so that the next pops return them in lane and page
+// order (growing again undoes the shrink), and growing lanes pop in lane order.  A page that is given back
+// and taken in one call is therefore found in the table it comes from, and nothing waits for another
+// thread's writes.  Once the pages or rows run out, that lane and every later one that
 // needs any is refused and left as it was.  No atomics: the result depends on the inputs alone.
 //
 // MOVE writes rows and pages: nothing in it reads what it writes (rows read the pages that a lane
@@ -85,8 +85,8 @@ __device__ __forceinline__ int pages_of(int positions) { return (positions + kQ4
 // The time is latency: the floor of 64 lanes' bytes is a nanosecond.  A decode step's call takes 2.8 us (64
 // lanes, most with no page to move), half of it the launch and the first loads; code that runs once is
 // fetched for it, so the form for few rows takes a row and a page per thread (four of each, laid out
-// straight, took 5.6).  128 prompts of 1 to 4096 positions (267,000 rows, 16,800
-// pages): 17.7 us to grow and to give back.
+// straight, took 5.6).  128 prompts of 1 to 4096 positions (267,000 rows, 16,800 pages): 17.9 us to grow
+// and to give back.
 template <bool MOVE, bool STATE>
 __global__ void __launch_bounds__(kMaxLanes, 1) kv_resize_kernel(const ResizeParams p) {
   __shared__ long long sh_want[3][32];
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kMaxLanes, 1) kv_resize_kernel(const ResizePar
     const int limit = p.max_pages * kQ4Page;
     valid = lane_on && old_len >= 0 && old_len <= limit && target >= 0 && target <= limit &&
             (p.row_stride == 0 || target - old_len <= p.row_stride);
-    const int have = valid ? (old_len + kQ4Page - 1) / kQ4Page : 0, want = valid ? (target + kQ4Page - 1) / kQ4Page : 0;
+    const int have = valid ? pages_of(old_len) : 0, want = valid ? pages_of(target) : 0;
     const int give = max(have - want, 0), need = max(want - have, 0), grow = valid ? max(target - old_len, 0) : 0;
 
     long long want_sum[3] = {give, need, grow}, want_all[3];
@@ -286,7 +286,8 @@ int kv_resize(int32_t* lens, const int32_t* targets, size_t lanes, int32_t* bloc
     return launch_pdl(kv_resize_kernel<true, true>, dim3(1), dim3(threads), 0, stream, 1, p);
   }
   const unsigned ctas = (unsigned)std::min<size_t>((size_t)sm_count(), ceil_div(rows, (size_t)kRowsPerCta));
-  const int rc = launch_pdl(kv_resize_kernel<true, false>, dim3(ctas), dim3(std::max(512u, lane_threads)), 0, stream, 1, p);
+  const dim3 threads(std::max(512u, lane_threads));
+  const int rc = launch_pdl(kv_resize_kernel<true, false>, dim3(ctas), threads, 0, stream, 1, p);
   if (rc) return rc;
   return launch_pdl(kv_resize_kernel<false, true>, dim3(1), dim3(std::max(128u, lane_threads)), 0, stream, 1, p);
 }

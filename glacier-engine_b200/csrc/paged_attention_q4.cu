@@ -49,9 +49,9 @@ namespace {
 
 constexpr int kMaxLanes = 1024;
 // Warps per CTA (one CTA per SM).  Three warps per SM partition cover each other's latencies better than
-// two, but at hd 128 they have to spill at 168 registers: with stages of 32 positions the 64-lane 7B layer takes
-// 32.3 us with eight warps and 33.3 with twelve (one lane of 1000 positions 6.1 and 7.4), 128 lanes of 1 to 1999 positions at hd 64 31.4
-// and 29.8.
+// two, but at hd 128 they have to spill at 168 registers: with stages of 32 positions the 64-lane 7B
+// layer takes 32.3 us with eight warps and 33.3 with twelve (one lane of 1000 positions 6.1 and 7.4), 128
+// lanes of 1 to 1999 positions at hd 64 31.4 and 29.8.
 template <int HD>
 constexpr int kWarps = HD == 128 ? 8 : 12;
 // Pages per stage: 64 positions, which spread the softmax's chain and the loop over twice the products
@@ -182,7 +182,8 @@ __device__ __forceinline__ void split_q(const AttnQ4Params& p, const float (&v)[
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
   // A power of two that brings the head's largest |q| into [2^14, 2^15), from the exponent bits.
-  const int e = top > 0.f && top <= 3.4028235e38f ? min(max((int)(__float_as_uint(top) >> 23) - 127 - 14, -100), 100) : 0;
+  const int top_e = (int)(__float_as_uint(top) >> 23) - 127 - 14;
+  const int e = top > 0.f && top <= 3.4028235e38f ? min(max(top_e, -100), 100) : 0;
   const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
   q.f = __uint_as_float((uint32_t)(127 + e) << 23) * 0x1p20f * p.scale_log2;
 #pragma unroll
@@ -413,7 +414,8 @@ __device__ __forceinline__ int find_share(const AttnQ4Params& p, int gw, int* ct
       const unsigned b = pair / hkv, i = b & 3;
       const int before = e + (i > 0 ? ns[0] : 0) + (i > 1 ? ns[1] : 0) + (i > 2 ? ns[2] : 0);
       const int n = i == 0 ? ns[0] : i == 1 ? ns[1] : i == 2 ? ns[2] : ns[3];
-      const int first = __shfl_sync(0xffffffffu, before, b >> 2) * hkv + (pair - b * hkv) * __shfl_sync(0xffffffffu, n, b >> 2);
+      const int lane_first = __shfl_sync(0xffffffffu, before, b >> 2) * hkv;
+      const int first = lane_first + (pair - b * hkv) * __shfl_sync(0xffffffffu, n, b >> 2);
       return pair == pairs ? total : first;  // c * pairs < 2^32: 128 lanes of 1024 heads
     };
     const unsigned c = blockIdx.x;
@@ -577,7 +579,8 @@ __device__ __forceinline__ void merge_cluster(const AttnQ4Params& p, uint8_t* sm
     const int hkv = p.num_kv_heads;
     const size_t at = (size_t)(blockIdx.x / kClusterCtas) * G + head;
     const float r = !whole ? 1.f : L == 0.f ? 0.f : 8.f / L;
-    float* dst = whole ? p.out + (size_t)(pair / hkv) * p.ldo + (size_t)((pair % hkv) * G + head) * HD : p.part_o + at * HD;
+    float* dst = whole ? p.out + (size_t)(pair / hkv) * p.ldo + (size_t)((pair % hkv) * G + head) * HD
+                       : p.part_o + at * HD;
     if (lane < HD / 4) *reinterpret_cast<float4*>(dst + d) = make_float4(a.x * r, a.y * r, a.z * r, a.w * r);
     if (!whole && lane == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
   }
@@ -864,8 +867,8 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
       for (int w = first; w < end; ++w) {
         const bool b = chain && w == first;
         const float(*ml)[2] = s_ml[b ? 1 : 0][w] + h0;
-        const float* src =
-            (b ? reinterpret_cast<const float*>(smem + (size_t)w * RING) : state_a + (size_t)w * G * ROW) + h0 * ROW + d;
+        const float* src = b ? reinterpret_cast<const float*>(smem + (size_t)w * RING) : state_a + (size_t)w * G * ROW;
+        src += h0 * ROW + d;
 #pragma unroll
         for (int g = 0; g < kPart; ++g)
           if (g < heads)
@@ -884,7 +887,8 @@ __global__ void __launch_bounds__(kWarps<HD> * 32, 1) attn_q4_kernel(const AttnQ
           if (lane == g) mine = make_float2(M[g], L[g]);
         }
         if (lane < heads) *reinterpret_cast<float2*>(p.part_ml + (part + lane) * 2) = mine;
-        const int units = Q * kWarps<HD>, begin = s_first[chain ? 1 : 0][first], ns = PairWalk<SP>::stages(ctx[pair / hkv]);
+        const int units = Q * kWarps<HD>, begin = s_first[chain ? 1 : 0][first];
+        const int ns = PairWalk<SP>::stages(ctx[pair / hkv]);
         const int c0 = begin / units, n = (begin + ns - 1) / units - c0 + 1;  // its first CTA, its CTAs
         __syncwarp();
         bool last = false;
@@ -979,7 +983,8 @@ int paged_attention_q4(const float* q, size_t ldq, const void* pool, size_t num_
   p.ldo = ldo;
   // Every launch marks its tickets with a number of its own; a captured one keeps its, and finds the
   // tickets cleared by the replay before.
-  static std::atomic<unsigned long long> launches{(unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
+  static std::atomic<unsigned long long> launches{
+      (unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
   do p.nonce = launches.fetch_add(1, std::memory_order_relaxed) & 0xffffffffffffull;
   while (p.nonce == 0);
   p.tickets = reinterpret_cast<unsigned long long*>(workspace);

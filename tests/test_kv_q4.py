@@ -422,7 +422,8 @@ def test_resize_of_random_batches(seed):
     kind = seed % 4
     some = lambda: rng.integers(0, 16 * max_pages + 1, lanes)  # noqa: E731
     lens = [some, lambda: 0 * some(), some, some][kind]()
-    targets = [some, some, lambda: 0 * some(), lambda: np.minimum(lens + rng.integers(0, 2, lanes), 16 * max_pages)][kind]()
+    one_more = lambda: np.minimum(lens + rng.integers(0, 2, lanes), 16 * max_pages)  # noqa: E731
+    targets = [some, some, lambda: 0 * some(), one_more][kind]()
     pg = -(-lens // 16)
     spare = int(rng.integers(0, max(2, int((-(-targets // 16)).sum()))) if seed % 5 == 0 else (-(-targets // 16)).sum())
     perm = rng.permutation(int(pg.sum()) + spare).astype(np.int32)
