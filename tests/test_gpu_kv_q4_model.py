@@ -260,3 +260,58 @@ def test_a_position_or_page_out_of_range_is_reported():
         assert max_err_vs_row_max(logits[b].cpu().numpy(), ref) <= DECODE_LOGIT_TOL
     sess.close()
     dm.close()
+
+
+def captured_tokens(sess, stream, kept, active=None):
+    """One replay; the tokens of the lanes that advanced go to `kept`."""
+    if active is not None:
+        sess.active.copy_(torch.tensor(active, dtype=torch.int32))
+    out = sess.replay_greedy_step().tolist()
+    for b, p in enumerate(sess.positions.tolist()):
+        if p >= 0:
+            kept[b].append(out[b])
+
+
+@pytest.mark.parametrize("kv_format", ["q4", "f32"])
+def test_a_captured_loop_keeps_the_token_of_a_lane_that_waits(kv_format):
+    """A lane that gets no page, and one that is paused, go on from their own tokens: every lane's tokens are
+    those of a session in which nobody waits."""
+    from glacier_b200.model import DecodeSession
+    prompts = [[3, 9, 27, 81, 243, 729, 5, 15, 45, 135, 405, 2, 6, 18], list(range(40, 55)), [7, 77, 777, 70]]
+    m, dm, own, cos, sin = make(8, 2, 64, 3, 3)
+    own.close()
+    own = DecodeSession(dm, 3, 3, kv_format=kv_format)
+    cur = [int(own.prefill(p, lane=b)[0]) for b, p in enumerate(prompts)]
+    free_run = [[] for _ in prompts]
+    for k in range(9):
+        cur = own.step(tokens=cur, positions=[len(p) + k for p in prompts]).tolist()
+        for b in range(3):
+            free_run[b].append(cur[b])
+    own.close()
+    sess = DecodeSession(dm, 3, 3, kv_format=kv_format, pool_pages=4)
+    for b, p in enumerate(prompts):
+        sess.tokens[b] = int(sess.prefill(p, lane=b)[0])
+    s, kept = torch.cuda.Stream(), [[], [], []]
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        sess.capture_greedy_step(stream=s)
+        for _ in range(2):
+            captured_tokens(sess, s, kept)
+        assert sess.lens.tolist() == [16, 17, 6] and int(sess.free_count) == 0
+        pending = int(sess.tokens[0])
+        captured_tokens(sess, s, kept)  # lane 0 gets no page
+        assert sess.grow_status.tolist() == [-3, 0, 0] and sess.positions.tolist() == [-1, 17, 6]
+        assert int(sess.tokens[0]) == pending
+        captured_tokens(sess, s, kept, active=[1, 0, 1])  # and lane 1 is paused
+        assert sess.positions.tolist() == [-1, -1, 7] and int(sess.tokens[0]) == pending
+        sess.resize([16, 18, 0], stream=s)  # request 2 ends: its page goes to lane 0
+        for _ in range(3):
+            captured_tokens(sess, s, kept, active=[1, 0, 0])
+        for _ in range(3):
+            captured_tokens(sess, s, kept, active=[1, 1, 0])
+    s.synchronize()
+    assert [len(k) for k in kept] == [8, 6, 4]
+    assert kept == [run[:len(k)] for run, k in zip(free_run, kept)]
+    status_word()  # an FP32 pool reports the lanes that waited
+    sess.close()
+    dm.close()
