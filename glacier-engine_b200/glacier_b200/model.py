@@ -414,16 +414,20 @@ class DecodeSession:
     def capture_greedy_step(self, stream=None):
         """Records one greedy continuation step as a CUDA graph: decode_step on self.tokens and
         self.positions, then tokens <- the new token ids and positions += 1.  With a shared pool a lane that
-        got no position (no page, or not active) keeps its token, which a later replay feeds.
-        replay_greedy_step() runs it again; all of its inputs live in device memory, so a replay is the
-        same step as a fresh launch sequence, minus the host launch work and inter-launch gaps."""
+        got no position (no page, or not active) keeps its token, which a later replay feeds; so does an
+        idle lane of 4-bit pages (position -1), which stays idle.  replay_greedy_step() runs it again;
+        all of its inputs live in device memory, so a replay is the same step as a fresh launch
+        sequence, minus the host launch work and inter-launch gaps."""
         torch = self.torch
         s = stream if stream is not None else torch.cuda.current_stream()
         self._graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self._graph, stream=s):
             out = self.step(stream=s)
-            if self.shared:  # `out` of a lane without a position means nothing
-                torch.where(self.positions >= 0, out, self.tokens, out=self.tokens)
+            if self.shared or self.kv_format == "q4":  # `out` of a lane without a position means nothing
+                live = self.positions >= 0
+                torch.where(live, out, self.tokens, out=self.tokens)
+                if not self.shared:
+                    self.positions.add_(live)
             else:
                 self.tokens.copy_(out)
                 self.positions.add_(1)

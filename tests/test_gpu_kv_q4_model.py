@@ -315,3 +315,27 @@ def test_a_captured_loop_keeps_the_token_of_a_lane_that_waits(kv_format):
     status_word()  # an FP32 pool reports the lanes that waited
     sess.close()
     dm.close()
+
+
+def test_an_idle_lane_of_a_captured_loop_stays_idle():
+    """Lanes with their own pages: position -1 is no position that a replay counts on from."""
+    m, dm, sess, cos, sin = make(8, 2, 64, 2, 2)
+    ref = [int(sess.prefill([3, 9, 27], lane=0)[0])]
+    for k in range(4):
+        ref.append(int(sess.step(tokens=[ref[-1], 5], positions=[3 + k, -1])[0]))
+    sess.tokens.copy_(torch.tensor([ref[0], 5]))
+    sess.positions.copy_(torch.tensor([3, -1]))
+    before = sess.pages()[2:].clone()
+    s, got = torch.cuda.Stream(), []
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        sess.capture_greedy_step(stream=s)
+        for _ in range(4):
+            got.append(int(sess.replay_greedy_step()[0]))
+    s.synchronize()
+    assert got == ref[1:]
+    assert sess.positions.tolist() == [7, -1] and int(sess.tokens[1]) == 5
+    assert torch.equal(sess.pages()[2:], before)  # nothing was written for the idle lane
+    assert status_word() == 0
+    sess.close()
+    dm.close()
