@@ -393,22 +393,29 @@ class DecodeSession:
 
     def step(self, tokens=None, positions=None, eligible=None, logits=None, stream=None):
         """One decode step on device tensors already in self.tokens / self.positions (with a shared pool the
-        positions come from the lanes' lengths)."""
+        positions come from the lanes' lengths, and a step that is refused takes its growth back)."""
         torch = self.torch
+        if self.shared and positions is not None:
+            raise ValueError("a session with pool_pages keeps its own positions")
         if tokens is not None:
             self.tokens.copy_(torch.as_tensor(tokens, dtype=torch.int32))
         if positions is not None:
-            if self.shared:
-                raise ValueError("a session with pool_pages keeps its own positions")
             self.positions.copy_(torch.as_tensor(positions, dtype=torch.int32))
         s = stream if stream is not None else torch.cuda.current_stream()
         if self.shared:
             self._grow(s)
         words = 0 if eligible is None else eligible.shape[-1]
-        _lib.call("glacier_cuda_decode_step", self.dm.h, self.kv, self.lanes, self.tokens.data_ptr(),
-                  self.positions.data_ptr(), self.block_tables.data_ptr(), self.max_pages,
-                  None if eligible is None else eligible.data_ptr(), words, self.out.data_ptr(),
-                  self.status.data_ptr(), None if logits is None else logits.data_ptr(), s.cuda_stream)
+        try:
+            _lib.call("glacier_cuda_decode_step", self.dm.h, self.kv, self.lanes, self.tokens.data_ptr(),
+                      self.positions.data_ptr(), self.block_tables.data_ptr(), self.max_pages,
+                      None if eligible is None else eligible.data_ptr(), words, self.out.data_ptr(),
+                      self.status.data_ptr(), None if logits is None else logits.data_ptr(), s.cuda_stream)
+        except Exception:
+            if self.shared:  # a lane that grew had the length that is its position now
+                with torch.cuda.stream(s):
+                    before = torch.where(self.positions >= 0, self.positions, self.lens)
+                self.resize(before, stream=s)
+            raise
         return self.out
 
     def capture_greedy_step(self, stream=None):

@@ -339,3 +339,27 @@ def test_an_idle_lane_of_a_captured_loop_stays_idle():
     assert status_word() == 0
     sess.close()
     dm.close()
+
+
+def test_a_refused_step_leaves_the_session_as_it_was():
+    from glacier_b200 import _lib
+    m, dm, sess, cos, sin = make(8, 2, 64, 2, 3, pool_pages=4)
+    cur = [int(sess.prefill(list(range(b + 1, b + n)), lane=b)[0]) for b, n in ((0, 17), (1, 6))]  # 16 and 5 positions
+    sess.active.copy_(torch.tensor([1, 0]))
+    sess.tokens.copy_(torch.tensor(cur))
+    state = lambda: [t.clone() for t in (sess.lens, sess.free_count, sess.free_pages[:2], sess.block_tables[1],  # noqa: E731
+                                         sess.block_tables[0, :1], sess.tokens)]
+    before = state()
+    with pytest.raises(_lib.GlacierCudaError):  # a mask of the wrong width: lane 0 had taken a page by then
+        sess.step(eligible=torch.zeros((2, 3), dtype=torch.int64, device="cuda"))
+    assert all(torch.equal(a, b) for a, b in zip(state(), before))
+    with pytest.raises(ValueError):
+        sess.step(tokens=[1, 2], positions=[16, 5])
+    assert all(torch.equal(a, b) for a, b in zip(state(), before))
+    logits = torch.empty((2, 1000), dtype=torch.float32, device="cuda")
+    sess.step(logits=logits)
+    assert sess.positions.tolist() == [16, -1]
+    assert max_err_vs_row_max(logits[0].cpu().numpy(), twin(m, sess, 0, cur[0], 16, cos, sin)) <= DECODE_LOGIT_TOL
+    assert status_word() == 0
+    sess.close()
+    dm.close()
