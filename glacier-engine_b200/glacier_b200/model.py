@@ -445,17 +445,20 @@ class DecodeSession:
         self._graph.replay()
         return self.out
 
-    def prefill(self, prompt, lane: int = 0, start: int = 0, eligible=None, logits=None, stream=None):
+    def prefill(self, prompt, lane: int = 0, start: int | None = None, eligible=None, logits=None, stream=None):
         """Feeds prompt tokens (host sequence or device int32 tensor) of one request at positions
-        start.. through lane `lane`'s block table; returns the device int32 tensor [1] holding
+        start.. (0 unless given) through lane `lane`'s block table; returns the device int32 tensor [1] holding
         the greedy token that follows (generate.zig prompt loop, batched).  With a shared pool the prompt goes
-        behind the lane's positions, whose pages it takes first (MemoryError when there are not enough)."""
+        behind the lane's positions (a start that is given has to be their number), whose pages it takes first
+        (MemoryError when there are not enough)."""
         torch = self.torch
         dev = self.tokens.device
         toks = torch.as_tensor(prompt, dtype=torch.int32).to(dev).contiguous()
         if self.shared:
             with torch.cuda.stream(stream):
                 before = self.lens.tolist()
+                if start is not None and start != before[lane]:
+                    raise ValueError(f"start {start}: lane {lane} of a shared pool goes on at {before[lane]}")
                 start, after = before[lane], list(before)
                 after[lane] += toks.numel()
                 if int(self.resize(after, stream=stream)[lane]) != 0:
@@ -465,7 +468,7 @@ class DecodeSession:
             except Exception:
                 self.resize(before, stream=stream)
                 raise
-        return self._prefill(toks, lane, start, eligible, logits, stream)
+        return self._prefill(toks, lane, start or 0, eligible, logits, stream)
 
     def _prefill(self, toks, lane, start, eligible, logits, stream):
         torch, dev = self.torch, self.tokens.device

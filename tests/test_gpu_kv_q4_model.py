@@ -363,3 +363,19 @@ def test_a_refused_step_leaves_the_session_as_it_was():
     assert status_word() == 0
     sess.close()
     dm.close()
+
+
+def test_a_prompt_of_a_shared_pool_starts_behind_the_lane():
+    """A start that is not the lane's length is refused, not dropped."""
+    m, dm, sess, cos, sin = make(8, 2, 64, 2, 4, pool_pages=6)
+    whole = int(sess.prefill([1, 2, 3, 4, 5], lane=1)[0])
+    sess.resize([0, 0])
+    sess.prefill([1, 2, 3], lane=1, start=0)
+    for start in (0, 2, 4, -1):
+        with pytest.raises(ValueError):
+            sess.prefill([4, 5], lane=1, start=start)
+    assert sess.lens.tolist() == [0, 3] and int(sess.free_count) == 5
+    assert int(sess.prefill([4, 5], lane=1, start=3)[0]) == whole
+    assert sess.lens.tolist() == [0, 5]
+    sess.close()
+    dm.close()
