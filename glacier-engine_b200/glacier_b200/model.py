@@ -450,7 +450,7 @@ class DecodeSession:
         start.. (0 unless given) through lane `lane`'s block table; returns the device int32 tensor [1] holding
         the greedy token that follows (generate.zig prompt loop, batched).  With a shared pool the prompt goes
         behind the lane's positions (a start that is given has to be their number), whose pages it takes first
-        (MemoryError when there are not enough)."""
+        (MemoryError when the pool has too few of them now)."""
         torch = self.torch
         dev = self.tokens.device
         toks = torch.as_tensor(prompt, dtype=torch.int32).to(dev).contiguous()
@@ -461,6 +461,9 @@ class DecodeSession:
                     raise ValueError(f"start {start}: lane {lane} of a shared pool goes on at {before[lane]}")
                 start, after = before[lane], list(before)
                 after[lane] += toks.numel()
+                if after[lane] > 16 * self.max_pages:  # as for a lane with its own pages
+                    raise _lib.GlacierCudaError(_lib.EINVAL, f"prefill: positions {start}..{after[lane] - 1} exceed "
+                                                             "the block table")
                 if int(self.resize(after, stream=stream)[lane]) != 0:
                     raise MemoryError(f"no pages for {toks.numel()} more positions of lane {lane}")
             try:

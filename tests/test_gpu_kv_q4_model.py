@@ -379,3 +379,20 @@ def test_a_prompt_of_a_shared_pool_starts_behind_the_lane():
     assert sess.lens.tolist() == [0, 5]
     sess.close()
     dm.close()
+
+
+def test_a_prompt_that_no_pages_could_hold_is_not_short_of_memory():
+    """MemoryError is for a pool that has no pages now; a prompt longer than the block table never fits."""
+    from glacier_b200 import _lib
+    m, dm, sess, cos, sin = make(8, 2, 64, 2, 4, pool_pages=6)
+    sess.prefill([1] * 20, lane=0)
+    for lane, n in ((0, 45), (1, 65), (1, 1000)):
+        with pytest.raises(_lib.GlacierCudaError) as e:
+            sess.prefill([1] * n, lane=lane)
+        assert e.value.code == _lib.EINVAL
+    sess.prefill([1] * 33, lane=1)  # three of the four pages that were left
+    with pytest.raises(MemoryError):
+        sess.prefill([1] * 44, lane=0)
+    assert sess.lens.tolist() == [20, 33] and int(sess.free_count) == 1
+    sess.close()
+    dm.close()
