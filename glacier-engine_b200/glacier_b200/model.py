@@ -451,38 +451,42 @@ class DecodeSession:
         the greedy token that follows (generate.zig prompt loop, batched).  With a shared pool the prompt goes
         behind the lane's positions (a start that is given has to be their number), whose pages it takes first
         (MemoryError when the pool has too few of them now)."""
-        torch = self.torch
-        dev = self.tokens.device
-        toks = torch.as_tensor(prompt, dtype=torch.int32).to(dev).contiguous()
-        if self.shared:
-            with torch.cuda.stream(stream):
-                before = self.lens.tolist()
-                if start is not None and start != before[lane]:
-                    raise ValueError(f"start {start}: lane {lane} of a shared pool goes on at {before[lane]}")
-                start, after = before[lane], list(before)
-                after[lane] += toks.numel()
-                if after[lane] > 16 * self.max_pages:  # as for a lane with its own pages
-                    raise _lib.GlacierCudaError(_lib.EINVAL, f"prefill: positions {start}..{after[lane] - 1} exceed "
-                                                             "the block table")
-                if int(self.resize(after, stream=stream)[lane]) != 0:
-                    raise MemoryError(f"no pages for {toks.numel()} more positions of lane {lane}")
+        with self.torch.cuda.stream(stream):  # what is allocated and copied here belongs to the stream that uses it
+            toks = self._int32(prompt).to(self.tokens.device).contiguous()
+            if not self.shared:
+                return self._prefill(toks, lane, start or 0, eligible, logits)
+            before = self.lens.tolist()
+            if start is not None and start != before[lane]:
+                raise ValueError(f"start {start}: lane {lane} of a shared pool goes on at {before[lane]}")
+            start, after = before[lane], list(before)
+            after[lane] += toks.numel()
+            if after[lane] > 16 * self.max_pages:  # as for a lane with its own pages
+                raise _lib.GlacierCudaError(_lib.EINVAL, f"prefill: positions {start}..{after[lane] - 1} exceed "
+                                                         "the block table")
+            if int(self.resize(after)[lane]) != 0:
+                raise MemoryError(f"no pages for {toks.numel()} more positions of lane {lane}")
             try:
-                return self._prefill(toks, lane, start, eligible, logits, stream)
+                return self._prefill(toks, lane, start, eligible, logits)
             except Exception:
-                self.resize(before, stream=stream)
+                self.resize(before)
                 raise
-        return self._prefill(toks, lane, start or 0, eligible, logits, stream)
 
-    def _prefill(self, toks, lane, start, eligible, logits, stream):
+    def _int32(self, x):
+        """x as int32, read by the current stream: memory of a device tensor is kept until that has happened."""
+        torch = self.torch
+        if isinstance(x, torch.Tensor) and x.is_cuda:
+            x.record_stream(torch.cuda.current_stream(x.device))
+        return torch.as_tensor(x, dtype=torch.int32)
+
+    def _prefill(self, toks, lane, start, eligible, logits):
         torch, dev = self.torch, self.tokens.device
         out = torch.empty(1, dtype=torch.int32, device=dev)
         status = torch.empty(1, dtype=torch.int32, device=dev)
-        s = stream if stream is not None else torch.cuda.current_stream()
         words = 0 if eligible is None else eligible.shape[-1]
         _lib.call("glacier_cuda_prefill", self.dm.h, self.kv, toks.data_ptr(), toks.numel(), start,
                   self.block_tables[lane].data_ptr(), self.max_pages,
                   None if eligible is None else eligible.data_ptr(), words, out.data_ptr(), status.data_ptr(),
-                  None if logits is None else logits.data_ptr(), s.cuda_stream)
+                  None if logits is None else logits.data_ptr(), torch.cuda.current_stream().cuda_stream)
         self.last_status = status
         return out
 

@@ -396,3 +396,42 @@ def test_a_prompt_that_no_pages_could_hold_is_not_short_of_memory():
     assert sess.lens.tolist() == [20, 33] and int(sess.free_count) == 1
     sess.close()
     dm.close()
+
+
+def busy(stream, n=60):
+    """Work that keeps `stream` behind the host for a while."""
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        a = torch.randn((4096, 4096), device="cuda")
+        for _ in range(n):
+            a @ a
+
+
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("on_device", [False, True])
+def test_prompts_on_another_stream_keep_their_tokens(shared, on_device):
+    """Two prompts of several chunks, one behind the other on a stream that is busy: neither sees the other's
+    tokens, nor what is allocated when the caller has dropped its prompt."""
+    more = dict(pool_pages=8) if shared else {}
+    m, dm, sess, cos, sin = make(8, 2, 64, 2, 4, reserve_lanes=8, **more)
+    rng = np.random.default_rng(9)
+    prompts = [rng.integers(0, 1000, 40).tolist() for _ in range(2)]
+    ref = [int(sess.prefill(p, lane=b)[0]) for b, p in enumerate(prompts)]
+    if shared:
+        sess.resize([0, 0])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    busy(side)
+    first = []
+    for b, p in enumerate(prompts):
+        p = torch.tensor(p, dtype=torch.int32, device="cuda") if on_device else p
+        if on_device:
+            torch.cuda.current_stream().synchronize()  # the prompt is there; how long it stays is not the caller's care
+        first.append(sess.prefill(p, lane=b, stream=side))
+        del p
+        junk = [torch.zeros(40, dtype=torch.int32, device="cuda") for _ in range(4)]
+    side.synchronize()
+    assert [int(t) for t in first] == ref and len(junk) == 4
+    assert status_word() == 0
+    sess.close()
+    dm.close()
