@@ -374,10 +374,10 @@ class DecodeSession:
         from . import ops
         if not self.shared:
             raise ValueError("resize needs a session with pool_pages")
-        targets = self.torch.as_tensor(targets, dtype=self.torch.int32)
-        if targets.shape != (self.lanes,):
-            raise ValueError(f"resize: {tuple(targets.shape)} lengths for {self.lanes} lanes")
         with self.torch.cuda.stream(stream):
+            targets = self._int32(targets)
+            if targets.shape != (self.lanes,):
+                raise ValueError(f"resize: {tuple(targets.shape)} lengths for {self.lanes} lanes")
             self.targets.copy_(targets)
         ops.kv_resize(self.lens, self.targets, self.block_tables, self.free_pages, self.free_count, self.grow_status,
                       stream=stream)
@@ -397,10 +397,11 @@ class DecodeSession:
         torch = self.torch
         if self.shared and positions is not None:
             raise ValueError("a session with pool_pages keeps its own positions")
-        if tokens is not None:
-            self.tokens.copy_(torch.as_tensor(tokens, dtype=torch.int32))
-        if positions is not None:
-            self.positions.copy_(torch.as_tensor(positions, dtype=torch.int32))
+        with torch.cuda.stream(stream):  # behind the steps that still read the ones before
+            if tokens is not None:
+                self.tokens.copy_(self._int32(tokens))
+            if positions is not None:
+                self.positions.copy_(self._int32(positions))
         s = stream if stream is not None else torch.cuda.current_stream()
         if self.shared:
             self._grow(s)

@@ -435,3 +435,33 @@ def test_prompts_on_another_stream_keep_their_tokens(shared, on_device):
     assert status_word() == 0
     sess.close()
     dm.close()
+
+
+def test_steps_on_another_stream_take_their_inputs_there():
+    """Tokens, positions and lengths are copied behind the steps that still read the ones before."""
+    m, dm, sess, cos, sin = make(8, 2, 64, 2, 4)
+    inputs = [([3 + k, 500 + k], [k, k]) for k in range(4)]
+    ref = [torch.empty((2, 1000), device="cuda") for _ in inputs]
+    for (tokens, positions), logits in zip(inputs, ref):
+        sess.step(tokens=tokens, positions=positions, logits=logits)
+    sess.pages().zero_()
+    got = [torch.empty_like(r) for r in ref]
+    side = torch.cuda.Stream()
+    busy(side)
+    for (tokens, positions), logits in zip(inputs, got):
+        sess.step(tokens=torch.tensor(tokens).pin_memory(), positions=torch.tensor(positions).pin_memory(), logits=logits,
+                  stream=side)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    sess.close()
+    m, dm2, sess, cos, sin = make(8, 2, 64, 2, 4, pool_pages=6)
+    late = torch.zeros(2, dtype=torch.int64, device="cuda")
+    busy(side)
+    with torch.cuda.stream(side):
+        late.copy_(torch.tensor([20, 7]).pin_memory(), non_blocking=True)
+    sess.resize(late, stream=side)
+    side.synchronize()
+    assert sess.lens.tolist() == [20, 7]
+    sess.close()
+    dm.close()
+    dm2.close()
