@@ -863,6 +863,13 @@ int glacier_cuda_model_reserve(glacier_cuda_model* m, size_t max_lanes, size_t m
   return GLACIER_CUDA_OK;
 }
 
+// Bytes of one page of the model's pools.  FP32: 16 positions of K and V for every layer
+// (paged_kv_cache.zig:1-16).
+static size_t kv_page_bytes(const glacier_cuda_model* m, bool q4) {
+  const size_t layers = m->cfg.num_layers;
+  return q4 ? layers * m->cfg.num_kv_heads * q4_block_bytes(m->cfg.head_dim) : layers * 2 * 16 * m->kv_dim * 4;
+}
+
 glacier_cuda_kv* glacier_cuda_kv_create(const glacier_cuda_model* m, size_t num_pages) {
   if (!m || num_pages == 0) {
     set_error(GLACIER_CUDA_EINVAL, "kv_create: null model or zero pages");
@@ -871,9 +878,8 @@ glacier_cuda_kv* glacier_cuda_kv_create(const glacier_cuda_model* m, size_t num_
   if (bind_device(m)) return nullptr;
   auto kv = std::make_unique<glacier_cuda_kv>();
   kv->num_pages = num_pages;
-  // One page = 16 positions of K and V for every layer (paged_kv_cache.zig:1-16).
-  kv->page_floats = (size_t)m->cfg.num_layers * 2 * 16 * m->kv_dim;
-  kv->page_bytes = kv->page_floats * 4;
+  kv->page_bytes = kv_page_bytes(m, false);
+  kv->page_floats = kv->page_bytes / 4;
   if (kv->pool.alloc(num_pages * kv->page_bytes)) return nullptr;
   if (cudaMemset(kv->pool.p, 0, kv->pool.bytes) != cudaSuccess) {
     set_error(GLACIER_CUDA_ECUDA, "kv_create: memset failed");
@@ -896,7 +902,7 @@ glacier_cuda_kv* glacier_cuda_kv_create_q4(const glacier_cuda_model* m, size_t n
   auto kv = std::make_unique<glacier_cuda_kv>();
   kv->num_pages = num_pages;
   kv->q4 = true;
-  kv->page_bytes = (size_t)c.num_layers * c.num_kv_heads * q4_block_bytes(c.head_dim);
+  kv->page_bytes = kv_page_bytes(m, true);
   if (kv->pool.alloc(num_pages * kv->page_bytes)) return nullptr;
   if (cudaMemset(kv->pool.p, 0, kv->pool.bytes) != cudaSuccess) {
     set_error(GLACIER_CUDA_ECUDA, "kv_create_q4: memset failed");
@@ -1122,6 +1128,7 @@ int glacier_cuda_decode_step(glacier_cuda_model* m, glacier_cuda_kv* kv, size_t 
   GLC_REQUIRE(max_pages > 0 && max_pages <= m->max_pages, "decode_step: %zu pages per lane, %zu reserved", max_pages,
               m->max_pages);
   GLC_REQUIRE(tokens && positions && block_tables && tokens_out, "decode_step: null argument");
+  GLC_REQUIRE(kv->page_bytes == kv_page_bytes(m, kv->q4), "decode_step: the pool's pages are another model's");
   if (eligible)
     GLC_REQUIRE(eligible_words == ceil_div(m->cfg.vocab, 64), "decode_step: eligible mask needs %zu words per lane",
                 ceil_div(m->cfg.vocab, 64));
@@ -1135,6 +1142,7 @@ int glacier_cuda_prefill(glacier_cuda_model* m, glacier_cuda_kv* kv, const int32
                          void* stream_ptr) {
   GLC_REQUIRE(m && kv && m->finalized && m->max_lanes > 0, "prefill: model not finalized and reserved");
   GLC_REQUIRE(tokens && block_table && token_out && count > 0 && start >= 0, "prefill: null or empty argument");
+  GLC_REQUIRE(kv->page_bytes == kv_page_bytes(m, kv->q4), "prefill: the pool's pages are another model's");
   GLC_REQUIRE(max_pages > 0 && max_pages <= m->max_pages, "prefill: %zu pages, %zu reserved", max_pages,
               m->max_pages);
   GLC_REQUIRE((size_t)start + count <= max_pages * 16, "prefill: positions %d..%zu exceed the block table", start,

@@ -365,7 +365,8 @@ size_t glacier_cuda_kv_page_bytes(const glacier_cuda_kv *kv);     /* of either *
  * With 4 lanes or fewer the eligible argmax runs in the LM head's epilogue (logitless greedy,
  * int4_neon.c:1075-1254): logits are written only to a given logits_out.  A position outside
  * the RoPE table or past the block table gives that lane context 0, writes no K/V and raises
- * the bad-input device status (glacier_cuda_device_status = 2).  With a 4-bit pool, position -1 is
+ * the bad-input device status (glacier_cuda_device_status = 2).  A pool whose pages are not this
+ * model's is refused, here and by glacier_cuda_prefill.  With a 4-bit pool, position -1 is
  * an idle lane: context 0 and no K/V without the status, and its token means nothing. */
 int glacier_cuda_decode_step(glacier_cuda_model *model, glacier_cuda_kv *kv, size_t lanes,
                              const int32_t *tokens, const int32_t *positions, const int32_t *block_tables,

@@ -465,3 +465,31 @@ def test_steps_on_another_stream_take_their_inputs_there():
     sess.close()
     dm.close()
     dm2.close()
+
+
+@pytest.mark.parametrize("kv_format", ["q4", "f32"])
+def test_a_pool_of_another_model_is_refused(kv_format):
+    """A pool's pages have to be the model's: one of smaller pages would be written past its end."""
+    from glacier_b200 import _lib
+    from glacier_b200.model import DecodeSession, DeviceModel, ModelConfig, SyntheticModel
+    i32 = dict(dtype=torch.int32, device="cuda")
+    dms, sess = [], []
+    for layers in (1, 3):
+        cfg = ModelConfig(num_layers=layers, dim=256, hidden=512, num_heads=8, num_kv_heads=2, head_dim=64, vocab=100)
+        dms.append(DeviceModel(SyntheticModel(cfg, seed=7), max_positions=64))
+        sess.append(DecodeSession(dms[-1], 2, 4, kv_format=kv_format))
+    prompt, out = torch.ones(3, **i32), torch.zeros(1, **i32)
+    for a in (0, 1):
+        s, kv = sess[a], sess[1 - a].kv
+        for name, args in (("glacier_cuda_decode_step",
+                            (2, s.tokens.data_ptr(), s.positions.data_ptr(), s.block_tables.data_ptr(), 4, None, 0,
+                             s.out.data_ptr(), None, None, None)),
+                           ("glacier_cuda_prefill", (prompt.data_ptr(), 3, 0, s.block_tables.data_ptr(), 4, None, 0,
+                                                     out.data_ptr(), None, None, None))):
+            with pytest.raises(_lib.GlacierCudaError) as e:
+                _lib.call(name, dms[a].h, kv, *args)
+            assert e.value.code == _lib.EINVAL
+        assert int(s.prefill([1, 2, 3])[0]) >= 0 and len(s.step(positions=[3, 0]).tolist()) == 2
+    assert status_word() == 0
+    for x in sess + dms:
+        x.close()
