@@ -130,10 +130,11 @@ __global__ void __launch_bounds__(kMaxLanes, 1) kv_resize_kernel(const ResizePar
   }
   __syncthreads();
   const int given = s_given, taken = s_taken, avail = (int)min((long long)count + given, (long long)p.capacity);
+  const unsigned top = (unsigned)count + given;  // of the stack with all of them: up to 2^32
   // Entry `at` of the stack after the shrinking lanes gave their pages back.
   auto stack = [&](int at) -> const int32_t* {
     if (at < count) return p.free_pages + at;
-    const int j = count + given - 1 - at, b = holder(s_give, p.lanes, j);
+    const int j = (int)(top - 1 - at), b = holder(s_give, p.lanes, j);
     return p.tables + (size_t)b * p.max_pages + pages_of(s_new[b]) + j - s_give[b];
   };
   // Page k of lane b, of those it held (h) or takes.
@@ -196,8 +197,9 @@ __global__ void __launch_bounds__(kMaxLanes, 1) kv_resize_kernel(const ResizePar
       // Laid end to end, one per thread; the block's last threads begin, beside the first ones' rows.
       const int i = (int)(me - tid) + (int)blockDim.x - 1 - tid;
       if (i < given) {
-        const int b = holder(s_give, p.lanes, i), at = count + given - 1 - i;
-        if (at < p.capacity)  // more pages than the stack holds are dropped
+        const int b = holder(s_give, p.lanes, i);
+        const unsigned at = top - 1 - i;
+        if (at < (unsigned)p.capacity)  // more pages than the stack holds are dropped
           p.free_pages[at] = p.tables[(size_t)b * p.max_pages + pages_of(s_new[b]) + i - s_give[b]];
       } else if (i < moves) {
         const int j = i - given, b = holder(s_first, p.lanes, j);
@@ -222,9 +224,10 @@ __global__ void __launch_bounds__(kMaxLanes, 1) kv_resize_kernel(const ResizePar
           }
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const int x = x0 + size * c, at = count + given - 1 - (s_give[b] + x);
+            const int x = x0 + size * c;
+            const unsigned at = top - 1 - (s_give[b] + x);
             if (x < abs(diff) && diff > 0) table[x] = page[c];
-            if (x < -diff && at < p.capacity) p.free_pages[at] = page[c];
+            if (x < -diff && at < (unsigned)p.capacity) p.free_pages[at] = page[c];
           }
         }
       }

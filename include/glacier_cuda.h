@@ -261,7 +261,7 @@ int glacier_cuda_paged_attention_q4(const float *q, const void *pool, size_t num
  *                a lane's pages are left as they were
  *   free_pages   [capacity] stack of free page ids, free_count[0] of them: pages come off the top in lane
  *                order.  Shrinking lanes give theirs back first, in the order that lets the same growth take
- *                the same pages again
+ *                the same pages again; pages that the stack has no room for are dropped
  *   status       [lanes]: 0; GLACIER_CUDA_ENOMEM when the free pages (or rows) run out at this lane or
  *                before it; GLACIER_CUDA_EINVAL for a length outside [0, 16 * max_pages] or growth past
  *                row_stride.  A lane not served keeps its length, pages and table.

@@ -867,3 +867,50 @@ def test_a_decode_loop_over_a_shared_pool(h, hkv, hd):
                 err = np.abs(out[b].reshape(h, hd)[j * h // hkv:(j + 1) * h // hkv] - attend64(qs, ks, vs)).max()
                 assert err <= tolerance(qs, ks, vs), (step, b, j)
     assert status_word() == 0
+
+
+@gpu
+@pytest.mark.parametrize("rows", [0, 128, 4096])
+def test_resize_near_the_largest_stack(rows):
+    """The stack's size and the pages given back add up to more than 2^31: what does not fit is dropped, what is
+    taken comes from the top, and nothing lands in front of the stack."""
+    from glacier_b200 import ops
+    i32 = dict(dtype=torch.int32, device="cuda")
+    capacity = 2 ** 31 - 1
+    count, n = capacity - 5, 1000
+    whole = torch.empty(4096 + capacity, **i32)  # the stack lies behind 4096 entries of ours
+    front, free = whole[:4096], whole[4096:]
+    front.fill_(-7)
+    free[:4096] = -8
+    free[count - 8:] = torch.arange(2000, 2013, **i32)
+    table = torch.full((2, n), -9, **i32)
+    table[0] = torch.arange(n, **i32)
+    lens, targets = torch.tensor([16 * n, 0], **i32), torch.tensor([0, 128], **i32)
+    counts, status = torch.tensor([count], **i32), torch.full((2,), 99, **i32)
+    more = {}
+    if rows:
+        more = dict(positions=torch.empty(rows, **i32), row_lanes=torch.empty(rows, **i32),
+                    slots=torch.empty(rows, dtype=torch.int64, device="cuda"))
+    ops.kv_resize(lens, targets, table, free, counts, status, **more)
+    assert status.tolist() == [0, 0] and lens.tolist() == [0, 128]
+    taken = [995, 996, 997, 998, 999, 2007, 2006, 2005]  # the five that fitted, then three of the old top
+    assert int(counts) == capacity - 8 and table[1, :9].tolist() == taken + [-9]
+    assert free[count - 8:count - 3].tolist() == [2000, 2001, 2002, 2003, 2004]
+    assert free[count:].tolist() == [999, 998, 997, 996, 995]
+    assert (front == -7).all() and (free[:4096] == -8).all()
+    if rows:
+        assert more["slots"][:128].tolist() == [16 * p + r for p in taken for r in range(16)]
+    # one lane of the longest block table that there can be, by many threads per lane
+    del table
+    n, count = 2 ** 26, capacity - 10
+    table = torch.arange(n, **i32).view(1, n)
+    lens, targets = torch.tensor([16 * n], **i32), torch.tensor([0], **i32)
+    counts.fill_(count)
+    free[count:] = -1
+    if rows:
+        more["positions"].fill_(5)
+    ops.kv_resize(lens, targets, table, free, counts, status[:1], **more)
+    assert int(status[0]) == 0 and int(lens) == 0 and int(counts) == capacity
+    assert free[count:].tolist() == [n - 1 - k for k in range(10)]
+    assert (front == -7).all() and (free[:4096] == -8).all()
+    assert not rows or (more["positions"] == -1).all()
