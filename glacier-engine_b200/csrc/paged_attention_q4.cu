@@ -275,7 +275,8 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
       o[i][3] *= a1;
     }
   }
-  const float base = m == -INFINITY ? 0.f : -(m * q.f);
+  // The difference first: of products with q.f, the rounding alone could be an exponent above fp16's.
+  const float ref = m == -INFINITY ? 0.f : -m;
   // The stage's sums start from zero and are added with rounding: a tensor core's sums cut, always
   // towards zero, and over ten stages that was 1e-6 of the result (with this, 3e-7; 1.5 % of the time).
   uint32_t hi[2 * SP], lo[2 * SP];
@@ -283,7 +284,7 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
   Words<NW> w[2 * SP];
 #pragma unroll
   for (int pj = 0; pj < 2 * SP; ++pj) {
-    float2 e = __ffma2_rn(sc[pj], make_float2(q.f, q.f), make_float2(base, base));
+    float2 e = __fmul2_rn(__fadd2_rn(sc[pj], make_float2(ref, ref)), make_float2(q.f, q.f));
     e.x = ex2(e.x);
     e.y = ex2(e.y);
     e = __fmul2_rn(e, make_float2(128.f, 128.f));

@@ -914,3 +914,26 @@ def test_resize_near_the_largest_stack(rows):
     assert free[count:].tolist() == [n - 1 - k for k in range(10)]
     assert (front == -7).all() and (free[:4096] == -8).all()
     assert not rows or (more["positions"] == -1).all()
+
+
+@gpu
+@pytest.mark.parametrize("h,hkv,hd", [(4, 2, 64), (7, 1, 128)])
+@pytest.mark.parametrize("exponent", [30, 60, 99, 115])
+def test_attention_of_large_scores(h, hkv, hd, exponent):
+    """Scores that are float32 numbers put all weight on one position, however large."""
+    from glacier_b200 import ops
+    ctx = 150
+    rng = np.random.default_rng(exponent)
+    q, pool, table = attention_case(rng, h, hkv, hd, [ctx])
+    q = q.reshape(h, hd)
+    q[:, 4:] = 0  # four dims: scores stay below 2^127
+    q = np.ldexp(q / np.abs(q).max(1, keepdims=True), exponent).astype(np.float32) * np.float32(1.9)
+    pages = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd)))
+    out = host(ops.paged_attention_q4(dev(q.reshape(1, -1)), pages, dev(table), dev(np.array([ctx], np.int32)), 2, 1, h,
+                                      hkv, hd)).reshape(h, hd)
+    for g in range(h):
+        k, v = (pool.rows(table[0], ctx, 1, g // (h // hkv), kind) for kind in (0, 1))
+        s = k @ q[g].astype(np.float64)
+        best, second = np.argsort(s)[[-1, -2]]
+        assert s[best] - s[second] > 2.0 ** -12 * np.abs(s).max()  # far above the scores' rounding, 2^-17
+        assert np.abs(out[g] - v[best]).max() <= 2.0 ** -20 * np.abs(v).max(), g
