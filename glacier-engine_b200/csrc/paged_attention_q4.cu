@@ -241,10 +241,12 @@ __device__ __forceinline__ void stage_scores(const uint8_t* __restrict__ buf, co
   }
 }
 
-// The online softmax of one stage's scores and its weighted V.  Weights are 2^7 2^(s - m) in
+// The online softmax of one stage's scores and its weighted V.  Weights are 2^13 2^(s - m) in
 // base-2 scores s: m is a reference near the running maximum of head lane / 4, moved
-// (and everything rescaled) only when a score passes it by more than 2^8, so the weights stay
-// below 2^15 and their low parts normal fp16 numbers.  l: this thread's share of their
+// (and everything rescaled) only when a score passes it by more than 2^2, so the weights stay
+// below 2^15.  Their two fp16 parts hold them to 22 bits above 2^-3, and to 2^-25 below: n positions
+// lose up to n 2^-38 of max |v| (with 2^7 and 2^8 in these places it was n 2^-32, 2.8e-7 where 64 lanes of
+// 4000 positions have one 22 nats above the others; the time is the same).  l: this thread's share of their
 // sum; o: sums of weight * v / 8.
 // keep: masks of the V scales, one per eight positions (two positions a word).
 template <int HD, int SP, bool PACK>
@@ -259,7 +261,7 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
   for (int i = 1; i < 2 * SP; ++i) mx = fmaxf(mx, fmaxf(sc[i].x, sc[i].y));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-  const bool move = (mx - m) * q.f > 8.f;  // false for NaN: no score yet
+  const bool move = (mx - m) * q.f > 2.f;  // false for NaN: no score yet
   if (__any_sync(0xffffffffu, move)) {
     const float mn = move ? mx : m;
     const float a = m == -INFINITY ? 0.f : ex2((m - mn) * q.f);
@@ -287,7 +289,7 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
     float2 e = __fmul2_rn(__fadd2_rn(sc[pj], make_float2(ref, ref)), make_float2(q.f, q.f));
     e.x = ex2(e.x);
     e.y = ex2(e.y);
-    e = __fmul2_rn(e, make_float2(128.f, 128.f));
+    e = __fmul2_rn(e, make_float2(8192.f, 8192.f));
     l = __fadd2_rn(l, e);
     split2(e, hi[pj], lo[pj]);
     if (PACK && n >= 4) hi[pj] = lo[pj];

@@ -937,3 +937,37 @@ def test_attention_of_large_scores(h, hkv, hd, exponent):
         best, second = np.argsort(s)[[-1, -2]]
         assert s[best] - s[second] > 2.0 ** -12 * np.abs(s).max()  # far above the scores' rounding, 2^-17
         assert np.abs(out[g] - v[best]).max() <= 2.0 ** -20 * np.abs(v).max(), g
+
+
+# ---- weights far below the largest ----
+
+@gpu
+@pytest.mark.parametrize("h,hkv,hd,lanes,ctx", [(1, 1, 128, 1, 32), (7, 1, 64, 1, 64), (8, 8, 64, 64, 4000),
+                                                (28, 4, 128, 100, 4000)])
+def test_attention_counts_weights_far_below_the_largest(h, hkv, hd, lanes, ctx):
+    """Position 0 is 22.2 nats (2^-32) above all others, and its V is zero: the output is what the others add.
+
+    A weight is held to half a step of the smallest fp16 number, 2^-25, at 2^13 for the largest: 2^-38 of it
+    each.  The 16 positions whose products one instruction sums with the largest weight's may lose all that lies
+    2^-24 below its product's place.  Exponents near 32 have errors of 2^-19, two of them 2^-18."""
+    from glacier_b200 import ops
+    pages = -(-ctx // 16)
+    blk = np.zeros((pages, hkv, 18 * hd), np.uint8)
+    blk[..., :8 * hd] = 0x66  # K -1, V 1, scales 1
+    blk[..., 8 * hd:16 * hd] = 0x88
+    blk[..., 16 * hd:] = np.frombuffer(np.float16(1).tobytes() * hd, np.uint8)
+    for q in range(hd // 4):  # position 0: K 0, V 0
+        at = ((q % 8 // 2) * (hd // 32) + q // 8) * 4 + q % 2 * 2
+        blk[0, :, at:at + 2] = 0x77
+        blk[0, :, 8 * hd + q * 4:8 * hd + q * 4 + 2] = 0x77
+    pool = Pool(blk.reshape(pages, -1), 1, hkv, hd)
+    k, v = (pool.rows(list(range(pages)), 17, 0, hkv - 1, kind) for kind in (0, 1))
+    assert not k[0].any() and not v[0].any() and (k[1:] == -1).all() and (v[1:] == 1).all()
+    q = np.zeros((lanes, h, hd), np.float32)
+    q[..., 5] = 22.2 * math.sqrt(hd)
+    table = np.tile(np.arange(pages, dtype=np.int32), (lanes, 1))  # every lane reads the same pages
+    out = host(ops.paged_attention_q4(dev(q.reshape(lanes, -1)), dev(pool.data.reshape(pages, -1)), dev(table),
+                                      dev(np.full(lanes, ctx, np.int32)), 1, 0, h, hkv, hd))
+    tail = (ctx - 1) * math.exp(-float(q[0, 0, 5]) / math.sqrt(hd))
+    ref = tail / (1 + tail)
+    assert np.abs(out - ref).max() <= ctx * 2.0 ** -38 + 16 * 2.0 ** -32 + 2.0 ** -18 * ref
