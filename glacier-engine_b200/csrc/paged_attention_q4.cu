@@ -181,11 +181,12 @@ __device__ __forceinline__ void split_q(const AttnQ4Params& p, const float (&v)[
     for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[2 * g + i / 4][i % 4]));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  // A power of two that brings the head's largest |q| into [2^14, 2^15), from the exponent bits.
+  // A power of two that brings the head's largest |q| into [2^14, 2^15), from the exponent bits: up to
+  // 2^125, where q.f is still a float32 number.
   const int top_e = (int)(__float_as_uint(top) >> 23) - 127 - 14;
-  const int e = top > 0.f && top <= 3.4028235e38f ? min(max(top_e, -100), 100) : 0;
+  const int e = top > 0.f && top <= 3.4028235e38f ? min(max(top_e, -100), 110) : 0;
   const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-  q.f = __uint_as_float((uint32_t)(127 + e) << 23) * 0x1p20f * p.scale_log2;
+  q.f = __uint_as_float((uint32_t)(127 + e) << 23) * (0x1p20f * p.scale_log2);
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     // High and low parts keep sums of their own: the high row then adds numbers of few bits, which the

@@ -243,8 +243,9 @@ int glacier_cuda_kv_q4_read_f32(const void *pool, size_t num_pages, size_t num_l
 /* glacier_cuda_paged_attention_f32 over a 4-bit pool, for up to 1024 lanes: lane b attends
  * positions 0..ctx_lens[b]-1, clamped to the block table; a lane of context 0 gets zeros.  The positions
  * of a page id outside the pool are left out and raise the bad-input status.  Scores, the softmax
- * and its sums are float32; held values enter the products exactly, q and the weights as two fp16 parts (22
- * bits, a weight to 2^-38 of the largest at least).  q, out and workspace are
+ * and its sums are float32; held values enter the products exactly, q and the weights as two fp16
+ * parts (22 bits, a weight to 2^-38 of the largest at least).  |q| is below 2^125: a head with a larger
+ * one may come out NaN, as one whose scores pass float32's range does.  q, out and workspace are
  * 16-byte aligned; workspace: glacier_cuda_paged_attention_q4_workspace() floats, any contents,
  * not shared with a call that may run at the same time.  At most 2^26 pages per lane, and lanes *
  * num_kv_heads * max_pages below 2^31; a page has less than 2^32 bytes. */

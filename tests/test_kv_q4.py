@@ -971,3 +971,26 @@ def test_attention_counts_weights_far_below_the_largest(h, hkv, hd, lanes, ctx):
     tail = (ctx - 1) * math.exp(-float(q[0, 0, 5]) / math.sqrt(hd))
     ref = tail / (1 + tail)
     assert np.abs(out - ref).max() <= ctx * 2.0 ** -38 + 16 * 2.0 ** -32 + 2.0 ** -18 * ref
+
+
+@gpu
+@pytest.mark.parametrize("h,hkv,hd", [(4, 2, 64), (7, 1, 128)])
+@pytest.mark.parametrize("exponent", [116, 120, 124])
+def test_attention_of_queries_near_float32s_largest(h, hkv, hd, exponent):
+    """Scores that are float32 numbers put all weight on one position, whatever the size of q (below 2^125)."""
+    from glacier_b200 import ops
+    ctx = 150
+    rng = np.random.default_rng(exponent)
+    q, pool, table = attention_case(rng, h, hkv, hd, [ctx])
+    q = q.reshape(h, hd)
+    q[:, 4:] = 0  # four dims: scores stay below 2^127
+    q = np.ldexp(q / np.abs(q).max(1, keepdims=True), exponent).astype(np.float32) * np.float32(1.9)
+    pages = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd)))
+    out = host(ops.paged_attention_q4(dev(q.reshape(1, -1)), pages, dev(table), dev(np.array([ctx], np.int32)), 2, 1, h,
+                                      hkv, hd)).reshape(h, hd)
+    for g in range(h):
+        k, v = (pool.rows(table[0], ctx, 1, g // (h // hkv), kind) for kind in (0, 1))
+        s = k @ q[g].astype(np.float64)
+        best, second = np.argsort(s)[[-1, -2]]
+        assert s[best] - s[second] > 2.0 ** -12 * np.abs(s).max()  # far above the scores' rounding, 2^-17
+        assert np.abs(out[g] - v[best]).max() <= 2.0 ** -20 * np.abs(v).max(), g
