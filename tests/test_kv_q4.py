@@ -994,3 +994,78 @@ def test_attention_of_queries_near_float32s_largest(h, hkv, hd, exponent):
         best, second = np.argsort(s)[[-1, -2]]
         assert s[best] - s[second] > 2.0 ** -12 * np.abs(s).max()  # far above the scores' rounding, 2^-17
         assert np.abs(out[g] - v[best]).max() <= 2.0 ** -20 * np.abs(v).max(), g
+
+
+# ---- both fp16 parts of q and of the weights are there ----
+# The tolerance above is a worst case, and a kernel without the low part of either operand would stay inside
+# it.  Roundings that are independent add in squares: the n + 16 half steps of a score become sqrt(n + 16) of
+# them, 8 more cover the weights' and sums' own, and a weighted mean of values whose weights are each off by such
+# a relative error is off by the same in norm.  Over the heads of one kv head:
+#
+#     |out - ref|^2 <= sum_heads (2^-24 * (sqrt(n + 16) * max_p sum |q k| / sqrt(n) + 8))^2 |ref|^2
+#
+# One fp16 part alone has 11 bits: relative errors near 2^-13 for a weight or a q, 2 to 5 times the bound at least
+# (the host model below).
+
+NORM_CTX = {"few": [700, 64, 1290], "many": [200 + i * 53 % 900 for i in range(40)]}
+NORM_HEADS = [(14, 2, 64), (8, 8, 64), (8, 2, 64), (28, 4, 128), (3, 3, 128), (16, 2, 128)]
+
+
+def norm_excess(out, q, k, v):
+    """|out - ref| over its bound, all heads of one kv head together."""
+    n = q.shape[1]
+    ref = attend64(q, k, v)
+    size = (np.abs(q.astype(np.float64)) @ np.abs(k).T).max(1) / math.sqrt(n)
+    bound = 2.0 ** -24 * (math.sqrt(n + 16) * size + 8) * np.linalg.norm(ref, axis=1)
+    return np.linalg.norm(out - ref) / np.linalg.norm(bound)
+
+
+def norm_case(name, h, hkv, hd):
+    rng = np.random.default_rng(100 * len(name) + h + hd)
+    q, pool, table = attention_case(rng, h, hkv, hd, NORM_CTX[name])
+    with np.errstate(invalid="ignore"):
+        k, v = all_values(pool, 1)
+
+    def rows(b, j):
+        c, ids = NORM_CTX[name][b], table[b, :-(-NORM_CTX[name][b] // 16)]
+        return (q[b].reshape(hkv, h // hkv, hd)[j], k[ids, j].reshape(-1, hd)[:c], v[ids, j].reshape(-1, hd)[:c])
+    return q, pool, table, rows
+
+
+@gpu
+@pytest.mark.parametrize("name", list(NORM_CTX))
+@pytest.mark.parametrize("h,hkv,hd", NORM_HEADS)
+def test_attention_error_in_norm(name, h, hkv, hd):
+    from glacier_b200 import ops
+    q, pool, table, rows = norm_case(name, h, hkv, hd)
+    pages = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd)))
+    out = host(ops.paged_attention_q4(dev(q), pages, dev(table), dev(np.array(NORM_CTX[name], np.int32)), 2, 1, h, hkv,
+                                      hd)).reshape(-1, hkv, h // hkv, hd)
+    for b in range(len(out)):
+        for j in range(hkv):
+            assert norm_excess(out[b, j], *rows(b, j)) <= 1, (b, j)
+
+
+@pytest.mark.parametrize("name", list(NORM_CTX))
+@pytest.mark.parametrize("h,hkv,hd", NORM_HEADS)
+def test_one_fp16_part_alone_is_outside_the_norm_bound(name, h, hkv, hd):
+    """A host model of the kernel's operands, each of q and the weights in one part instead of two."""
+    _, _, _, rows = norm_case(name, h, hkv, hd)
+    worst_q, worst_p, both = [], [], []
+    for b in range(len(NORM_CTX[name])):
+        for j in range(hkv):
+            q, k, v = rows(b, j)
+
+            def model(q, part):
+                s = q @ k.T / math.sqrt(hd)
+                e = np.exp(s - s.max(1, keepdims=True)) * 128
+                return part(e) @ v / e.sum(1, keepdims=True)
+            one = lambda x: x.astype(np.float16).astype(np.float64)  # noqa: E731
+            two = lambda x: one(x) + one(x - one(x))  # noqa: E731
+            q64 = q.astype(np.float64)
+            up = 2.0 ** (14 - np.floor(np.log2(np.abs(q64).max(1, keepdims=True))))  # as the kernel scales q
+            worst_q.append(norm_excess(model(one(q64 * up) / up, two), q, k, v))
+            worst_p.append(norm_excess(model(two(q64 * up) / up, one), q, k, v))
+            both.append(norm_excess(model(two(q64 * up) / up, two), q, k, v))
+    assert max(both) < 0.1
+    assert max(worst_q) > 2 and max(worst_p) > 2
