@@ -194,7 +194,7 @@ int qkv_rope_append_q4(const float* qkv, size_t ld, size_t split_stride, int nsp
                        const int64_t* slots, size_t batch, size_t num_heads, size_t num_kv_heads, size_t head_dim,
                        float* q_out, size_t ldq, void* pool, size_t num_pages, size_t num_layers, size_t layer,
                        cudaStream_t stream) {
-  GLC_REQUIRE(qkv && cos_t && sin_t && pos && slots && q_out, "qkv_rope_append_q4: null argument");
+  GLC_REQUIRE(cos_t && sin_t && ((qkv && pos && slots && q_out) || batch == 0), "qkv_rope_append_q4: null argument");
   int rc = q4_check_pool("qkv_rope_append_q4", pool, num_pages, num_layers, layer, num_heads, num_kv_heads, head_dim);
   if (rc) return rc;
   const size_t nrows = num_heads + 2 * num_kv_heads;
@@ -219,7 +219,7 @@ int qkv_rope_append_q4(const float* qkv, size_t ld, size_t split_stride, int nsp
 
 int kv_q4_read(const void* pool, size_t num_pages, size_t num_layers, size_t layer, size_t num_kv_heads,
                size_t head_dim, const int64_t* slots, size_t rows, float* k_out, float* v_out, cudaStream_t stream) {
-  GLC_REQUIRE(slots && k_out && v_out && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
+  GLC_REQUIRE(((slots && k_out && v_out) || rows == 0) && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
               "kv_q4_read: null or unaligned argument");
   int rc = q4_check_pool("kv_q4_read", pool, num_pages, num_layers, layer, num_kv_heads, num_kv_heads, head_dim);
   if (rc) return rc;

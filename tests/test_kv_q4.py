@@ -1069,3 +1069,29 @@ def test_one_fp16_part_alone_is_outside_the_norm_bound(name, h, hkv, hd):
             both.append(norm_excess(model(two(q64 * up) / up, two), q, k, v))
     assert max(both) < 0.1
     assert max(worst_q) > 2 and max(worst_p) > 2
+
+
+def test_no_rows_are_no_error():
+    """An empty tensor's pointer is null: nothing to append or to read is not a missing argument."""
+    a = dict(qkv=None, ld=768, bias=None, cos=4096, sin=4096, positions=64, pos=None, slots=None, batch=0, h=8, hkv=2,
+             hd=64, q=None, ldq=512, pool=4096, num_pages=8, num_layers=2, layer=1)
+    r = dict(pool=4096, num_pages=8, num_layers=2, layer=1, hkv=2, hd=64, slots=None, rows=0, k=None, v=None)
+    assert capi("glacier_cuda_qkv_rope_append_q4", *a.values(), None) == 0
+    assert capi("glacier_cuda_kv_q4_read_f32", *r.values(), None) == 0
+    for over in (dict(hd=96), dict(layer=2), dict(pool=None)):  # the rest is checked all the same
+        assert capi("glacier_cuda_qkv_rope_append_q4", *{**a, **over}.values(), None) == EINVAL
+        assert capi("glacier_cuda_kv_q4_read_f32", *{**r, **over}.values(), None) == EINVAL
+
+
+@gpu
+def test_wrappers_take_no_rows():
+    from glacier_b200 import ops
+    h, hkv, hd = 8, 2, 64
+    pages = torch.zeros((2, ops.kv_q4_page_bytes(1, hkv, hd)), dtype=torch.uint8, device="cuda")
+    none = torch.empty(0, dtype=torch.int64, device="cuda")
+    k, v = ops.kv_q4_read(pages, none, 1, 0, hkv, hd)
+    assert k.shape == v.shape == (0, hkv * hd)
+    cos = torch.ones((4, hd // 2), device="cuda")
+    q = ops.qkv_rope_append_q4(torch.empty((0, (h + 2 * hkv) * hd), device="cuda"), None, cos, cos, none.int(), none, h,
+                               hkv, hd, pages, 1, 0)
+    assert q.shape == (0, h * hd) and not host(pages).any()
