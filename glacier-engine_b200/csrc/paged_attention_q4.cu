@@ -278,8 +278,12 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
       o[i][3] *= a1;
     }
   }
-  // The difference first: of products with q.f, the rounding alone could be an exponent above fp16's.
-  const float ref = m == -INFINITY ? 0.f : -m;
+  // The state's maximum is the rounded m q.f, so the weights refer to it and its error cancels.  Beyond
+  // base-2 scores of 2^18 that error could move a weight out of fp16's range, and is taken back.  (Weights
+  // from q.f (s - m) need no such step, but each has the difference's rounding then: errors up to a quarter larger,
+  // and the same time.)
+  const float m0 = m == -INFINITY ? 0.f : m, top = m0 * q.f, err = fmaf(m0, q.f, -top);
+  const float back = fabsf(err) > 0x1p-6f ? -err : 0.f;
   // The stage's sums start from zero and are added with rounding: a tensor core's sums cut, always
   // towards zero, and over ten stages that was 1e-6 of the result (with this, 3e-7; 1.5 % of the time).
   uint32_t hi[2 * SP], lo[2 * SP];
@@ -287,7 +291,8 @@ __device__ __forceinline__ void stage_values(const uint8_t* __restrict__ buf, co
   Words<NW> w[2 * SP];
 #pragma unroll
   for (int pj = 0; pj < 2 * SP; ++pj) {
-    float2 e = __fmul2_rn(__fadd2_rn(sc[pj], make_float2(ref, ref)), make_float2(q.f, q.f));
+    float2 e = __ffma2_rn(sc[pj], make_float2(q.f, q.f), make_float2(-top, -top));
+    e = __fadd2_rn(e, make_float2(back, back));
     e.x = ex2(e.x);
     e.y = ex2(e.y);
     e = __fmul2_rn(e, make_float2(8192.f, 8192.f));
