@@ -2,8 +2,8 @@
 //
 // A page holds 16 positions of every layer (PagedKVCache's page,
 // src/paged_kv_cache.zig:16).  The block of one (page, layer, kv head) is
-// 18 * head_dim contiguous bytes, so one bulk copy brings a page's K and V of one
-// head to shared memory with their scales:
+// 18 * head_dim contiguous bytes, K and V with their scales, a multiple of 16: the
+// attention kernel copies them in 16-byte chunks, the pages of a stage end to end:
 //
 //   K codes   [16 positions][4 t][head_dim/32 g]  u32: dims 32g+8t .. 32g+8t+7
 //   V codes   [8 position pairs][head_dim/4 w][2] u16: dims 4w .. 4w+3

@@ -7,8 +7,10 @@
 // G <= 8 query heads of a group need 4 G hd products on them: on the fp32 pipe that
 // is more time than the bytes take, so both products run as mma.sync m16n8k16
 // (fp16 in, fp32 sums).  q and the softmax weights go in as a high and a low fp16 part, 22
-// bits together; the held values are exact.  (A tcgen05.mma needs 64 or 128 rows and its
-// operands in shared memory as fp16: the codes would be unpacked, written and read once more.)
+// bits together; the held values are exact.  (tcgen05.mma would take the unpacked codes as its A operand
+// in tensor memory, 128 positions or dims a tile, with q or the weights as sixteen columns in shared
+// memory.  Every operand register would go there by tcgen05.st first, and the accumulators would leave the
+// register file; this form has not been built or measured.)
 //   * q K^T: M is the query heads, and eight of them would leave half of the sixteen rows
 //     idle: rows 0-7 hold q's high and rows 8-15 its low parts.  A code c at bits 4-7 is used as
 //     the subnormal fp16 number that these bits are, c * 2^-20: three shifts and four ANDs make
@@ -27,8 +29,8 @@
 // The cache's orders put every operand register's codes in one word of one thread: K's words
 // (t, g) and V's 16-bit units by position pair are the fragments of these instructions.
 //
-// What bounds it (B200, 7B heads, graph replay): 64 lanes of 2048 positions take 30.2 us, their 77 MB
-// at the measured copy rate 12.0; from there on 8.6 us for every 1000 positions more, against 5.7. The
+// What bounds it (B200, 7B heads, graph replay): 64 lanes of 2048 positions take 30.1 us, their 77 MB
+// at the measured copy rate 12.0; from there on 8.5 us for every 1000 positions more, against 5.7. The
 // slope is arithmetic and its dependences (with all pages in L2 it is the same, and the loads alone run
 // at the copy rate): some 600 instructions per warp and 32 positions, 64 of them mma.sync of 8 cycles, with
 // two warps per SM partition take 1250 cycles, twice what their issue does. The rest, some 10 us (7 when no

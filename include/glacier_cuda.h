@@ -369,7 +369,8 @@ size_t glacier_cuda_kv_page_bytes(const glacier_cuda_kv *kv);     /* of either *
  * the RoPE table or past the block table gives that lane context 0, writes no K/V and raises
  * the bad-input device status (glacier_cuda_device_status = 2).  A pool whose pages are not this
  * model's is refused, here and by glacier_cuda_prefill.  With a 4-bit pool, position -1 is
- * an idle lane: context 0 and no K/V without the status, and its token means nothing. */
+ * an idle lane: context 0 and no K/V without the status, and the token that comes out for it means
+ * nothing (the one that goes in is embedded all the same: any id of the vocabulary). */
 int glacier_cuda_decode_step(glacier_cuda_model *model, glacier_cuda_kv *kv, size_t lanes,
                              const int32_t *tokens, const int32_t *positions, const int32_t *block_tables,
                              size_t max_pages, const uint64_t *eligible, size_t eligible_words,
