@@ -403,9 +403,9 @@ class DecodeSession:
             if positions is not None:
                 self.positions.copy_(self._int32(positions))
         s = stream if stream is not None else torch.cuda.current_stream()
+        words = 0 if eligible is None else eligible.shape[-1]
         if self.shared:
             self._grow(s)
-        words = 0 if eligible is None else eligible.shape[-1]
         try:
             _lib.call("glacier_cuda_decode_step", self.dm.h, self.kv, self.lanes, self.tokens.data_ptr(),
                       self.positions.data_ptr(), self.block_tables.data_ptr(), self.max_pages,

@@ -493,3 +493,15 @@ def test_a_pool_of_another_model_is_refused(kv_format):
     assert status_word() == 0
     for x in sess + dms:
         x.close()
+
+
+def test_a_mask_that_is_no_tensor_leaves_the_session_as_it_was():
+    m, dm, sess, cos, sin = make(8, 2, 64, 2, 3, pool_pages=4)
+    sess.prefill([1] * 16, lane=0)
+    with pytest.raises(AttributeError):
+        sess.step(tokens=[1, 2], eligible=[1, 2])
+    with pytest.raises(AttributeError):
+        sess.prefill([1, 2], lane=1, eligible=[1, 2])
+    assert sess.lens.tolist() == [16, 0] and int(sess.free_count) == 3
+    sess.close()
+    dm.close()
