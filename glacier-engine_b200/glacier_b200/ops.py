@@ -126,7 +126,8 @@ def argmax_eligible(logits, words=None, stream=None):
 
 # ---- the KV cache held in 4 bits ----
 # These run on the device their tensors are on, whichever is current; what they allocate belongs
-# to the stream they run on.  Tensors of another type, shape, layout or device are refused.
+# to the stream they run on, and what they are given is kept until a stream= has done with it.  Tensors of
+# another type, shape, layout or device are refused.
 # A decode step makes them every layer, so the checks are plain comparisons (about 2 us a call) and
 # only a refusal looks for the tensor to name.
 
@@ -151,13 +152,17 @@ def _fits(t, dtype, shape, dev):
 
 
 class _On:
-    """Makes another device, or a given stream, current around a call."""
+    """Makes another device, or a given stream, current around a call; the call's tensors may be dropped behind it."""
 
-    def __init__(self, dev, stream):
+    def __init__(self, dev, stream, *tensors):
         if dev < 0:
             _refuse(dev)
         if stream is not None and stream.device.index != dev:
             raise GlacierCudaError(EINVAL, f"a stream of {stream.device} for tensors on GPU {dev}")
+        if stream is not None:
+            for t in tensors:
+                if t is not None and t.get_device() == dev:
+                    t.record_stream(stream)
         self.ctx = torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(dev))
 
     def __enter__(self):
@@ -179,7 +184,7 @@ def qkv_rope_append_q4(qkv, bias, cos, sin, pos, slots, num_heads, num_kv_heads,
     [batch, num_heads * head_dim].  ``qkv`` may be a view with a row stride."""
     dev = qkv.get_device()
     if stream is not None or dev < 0 or dev != _device():
-        with _On(dev, stream):
+        with _On(dev, stream, qkv, bias, cos, sin, pos, slots, pages, q_out):
             return qkv_rope_append_q4(qkv, bias, cos, sin, pos, slots, num_heads, num_kv_heads, head_dim, pages,
                                       num_layers, layer, q_out)
     qd, kvd = num_heads * head_dim, num_kv_heads * head_dim
@@ -206,7 +211,7 @@ def kv_q4_read(pages, slots, num_layers, layer, num_kv_heads, head_dim, stream=N
     """The K and V values held at ``slots``: two float32 [rows, num_kv_heads * head_dim] (zeros for slot -1)."""
     dev = pages.get_device()
     if stream is not None or dev < 0 or dev != _device():
-        with _On(dev, stream):
+        with _On(dev, stream, pages, slots):
             return kv_q4_read(pages, slots, num_layers, layer, num_kv_heads, head_dim)
     rows, num_pages, kvd = slots.numel(), pages.shape[0], num_kv_heads * head_dim
     page = (num_pages, 18 * num_layers * kvd)
@@ -230,7 +235,7 @@ def paged_attention_q4(q, pages, block_tables, ctx_lens, num_layers, layer, num_
     """paged_attention_f32 over a 4-bit pool, one query row per lane."""
     dev = q.get_device()
     if stream is not None or dev < 0 or dev != _device():
-        with _On(dev, stream):
+        with _On(dev, stream, q, pages, block_tables, ctx_lens, out, workspace):
             return paged_attention_q4(q, pages, block_tables, ctx_lens, num_layers, layer, num_heads, num_kv_heads,
                                       head_dim, out, workspace)
     lanes, num_pages, max_pages = q.shape[0], pages.shape[0], block_tables.shape[-1]
@@ -261,7 +266,8 @@ def kv_resize(lens, targets, block_tables, free_pages, free_count, status, posit
     see glacier_cuda_kv_resize for the order in which lanes are served and the statuses."""
     dev = lens.get_device()
     if stream is not None or dev < 0 or dev != _device():
-        with _On(dev, stream):
+        with _On(dev, stream, lens, targets, block_tables, free_pages, free_count, status, positions, row_lanes, slots,
+                 row_offsets):
             return kv_resize(lens, targets, block_tables, free_pages, free_count, status, positions, row_lanes, slots,
                              row_offsets, row_stride)
     n, max_pages, capacity = lens.shape[0], block_tables.shape[-1], free_pages.numel()

@@ -1095,3 +1095,46 @@ def test_wrappers_take_no_rows():
     q = ops.qkv_rope_append_q4(torch.empty((0, (h + 2 * hkv) * hd), device="cuda"), None, cos, cos, none.int(), none, h,
                                hkv, hd, pages, 1, 0)
     assert q.shape == (0, h * hd) and not host(pages).any()
+
+
+@gpu
+def test_operators_on_another_stream_keep_what_the_caller_drops():
+    """Inputs that are dropped after the call, and whose memory goes to other tensors, while the stream is busy."""
+    from glacier_b200 import ops
+    h, hkv, hd, ctxs = 8, 2, 64, [100, 37]
+    rng = np.random.default_rng(31)
+    q, pool, table = attention_case(rng, h, hkv, hd, ctxs)
+    pages = dev(pool.data.reshape(-1, ops.kv_q4_page_bytes(2, hkv, hd)))
+    lengths, t = dev(np.array(ctxs, np.int32)), dev(table)
+    ref = host(ops.paged_attention_q4(dev(q), pages, t, lengths, 2, 1, h, hkv, hd))
+    x = rng.standard_normal((2, (h + 2 * hkv) * hd), dtype=np.float32)
+    one, zero = torch.ones((1, hd // 2), device="cuda"), torch.zeros((1, hd // 2), device="cuda")
+    side = torch.cuda.Stream()
+    args = [dev(q), t.clone(), lengths.clone()]
+    more = [dev(x), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.tensor([0, 17], device="cuda")]
+    held_pages = torch.zeros_like(pages)
+    grow = [torch.zeros(2, dtype=torch.int32, device="cuda"), torch.tensor([20, 5], dtype=torch.int32, device="cuda")]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    blocks, free, count, status = torch.full((2, 4), -1, **i32), torch.arange(6, **i32), torch.tensor([6], **i32), torch.ones(2, **i32)
+    torch.cuda.synchronize()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a = torch.randn((4096, 4096), device="cuda")
+        for _ in range(60):
+            a @ a
+    out = ops.paged_attention_q4(args[0], pages, args[1], args[2], 2, 1, h, hkv, hd, stream=side)
+    rot = ops.qkv_rope_append_q4(more[0], None, one, zero, more[1], more[2], h, hkv, hd, held_pages, 2, 1, stream=side)
+    k, v = ops.kv_q4_read(held_pages, more[2], 2, 1, hkv, hd, stream=side)
+    ops.kv_resize(grow[0], grow[1], blocks, free, count, status, stream=side)
+    shapes = [(y.shape, y.dtype) for y in args + more + grow[1:]]
+    del args, more, grow[1:]
+    junk = [torch.full(s, 9, dtype=d, device="cuda") for s, d in shapes for _ in range(3)]
+    side.synchronize()
+    assert len(junk) == 21
+    np.testing.assert_array_equal(out.cpu().numpy(), ref)
+    np.testing.assert_array_equal(rot.cpu().numpy(), x[:, :h * hd])
+    for b in range(2):
+        rows = x[b].reshape(-1, hd)
+        np.testing.assert_array_equal(k[b].cpu().numpy(), np.concatenate([held(r) for r in rows[h:h + hkv]]))
+        np.testing.assert_array_equal(v[b].cpu().numpy(), np.concatenate([held(r) for r in rows[h + hkv:]]))
+    assert status.tolist() == [0, 0] and grow[0].tolist() == [20, 5]
