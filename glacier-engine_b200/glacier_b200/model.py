@@ -383,13 +383,14 @@ class DecodeSession:
                       stream=stream)
         return self.grow_status
 
-    def _grow(self, s):
+    def _grow(self, stream):
         """Shared pool: one position more for every active lane; their positions, -1 for the others."""
         from . import ops
-        with self.torch.cuda.stream(s):
+        with self.torch.cuda.stream(stream):
             self.torch.add(self.lens, self.active, out=self.targets)
         ops.kv_resize(self.lens, self.targets, self.block_tables, self.free_pages, self.free_count, self.grow_status,
-                      positions=self.positions, row_lanes=self._row_lanes, slots=self._slots, row_stride=1, stream=s)
+                      positions=self.positions, row_lanes=self._row_lanes, slots=self._slots, row_stride=1,
+                      stream=stream)
 
     def step(self, tokens=None, positions=None, eligible=None, logits=None, stream=None):
         """One decode step on device tensors already in self.tokens / self.positions (with a shared pool the
@@ -402,10 +403,11 @@ class DecodeSession:
                 self.tokens.copy_(self._int32(tokens))
             if positions is not None:
                 self.positions.copy_(self._int32(positions))
+            self._keep(eligible, logits)
         s = stream if stream is not None else torch.cuda.current_stream()
         words = 0 if eligible is None else eligible.shape[-1]
         if self.shared:
-            self._grow(s)
+            self._grow(stream)
         try:
             _lib.call("glacier_cuda_decode_step", self.dm.h, self.kv, self.lanes, self.tokens.data_ptr(),
                       self.positions.data_ptr(), self.block_tables.data_ptr(), self.max_pages,
@@ -454,6 +456,7 @@ class DecodeSession:
         (MemoryError when the pool has too few of them now)."""
         with self.torch.cuda.stream(stream):  # what is allocated and copied here belongs to the stream that uses it
             toks = self._int32(prompt).to(self.tokens.device).contiguous()
+            self._keep(eligible, logits)
             if not self.shared:
                 return self._prefill(toks, lane, start or 0, eligible, logits)
             before = self.lens.tolist()
@@ -472,12 +475,16 @@ class DecodeSession:
                 self.resize(before)
                 raise
 
+    def _keep(self, *tensors):
+        """Device tensors of the caller's that the current stream uses: their memory stays until it has."""
+        for t in tensors:
+            if isinstance(t, self.torch.Tensor) and t.is_cuda:
+                t.record_stream(self.torch.cuda.current_stream(t.device))
+
     def _int32(self, x):
-        """x as int32, read by the current stream: memory of a device tensor is kept until that has happened."""
-        torch = self.torch
-        if isinstance(x, torch.Tensor) and x.is_cuda:
-            x.record_stream(torch.cuda.current_stream(x.device))
-        return torch.as_tensor(x, dtype=torch.int32)
+        """x as int32, for the current stream."""
+        self._keep(x)
+        return self.torch.as_tensor(x, dtype=self.torch.int32)
 
     def _prefill(self, toks, lane, start, eligible, logits):
         torch, dev = self.torch, self.tokens.device

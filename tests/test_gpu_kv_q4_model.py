@@ -505,3 +505,32 @@ def test_a_mask_that_is_no_tensor_leaves_the_session_as_it_was():
     assert sess.lens.tolist() == [16, 0] and int(sess.free_count) == 3
     sess.close()
     dm.close()
+
+
+def test_masks_and_logits_on_another_stream_are_kept():
+    """A mask that the caller drops, and logits memory that nobody else may get, while the step is still to come."""
+    m, dm, sess, cos, sin = make(8, 2, 64, 2, 4, reserve_lanes=8)
+    words = torch.zeros((2, 16), dtype=torch.int64, device="cuda")
+    words[:, 3] = 1 << 7  # token 199 alone
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    busy(side)
+    mask, logits = words.clone(), torch.empty((2, 1000), device="cuda")
+    torch.cuda.current_stream().synchronize()
+    out = sess.step(positions=torch.zeros(2, dtype=torch.int32, device="cuda"), eligible=mask, logits=logits, stream=side)
+    del mask, logits
+    junk = [torch.full((2, 16), -1, dtype=torch.int64, device="cuda") for _ in range(4)]
+    rows = [torch.full((2, 1000), 3.0, device="cuda") for _ in range(4)]
+    side.synchronize()
+    assert out.tolist() == [199, 199] and len(junk) == 4 and all((r == 3).all() for r in rows)
+    busy(side)
+    prompt = torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda")
+    mask = words[:1].clone()
+    torch.cuda.current_stream().synchronize()
+    first = sess.prefill(prompt, lane=1, eligible=mask, stream=side)
+    del mask
+    junk = [torch.full((1, 16), -1, dtype=torch.int64, device="cuda") for _ in range(4)]
+    side.synchronize()
+    assert int(first) == 199
+    sess.close()
+    dm.close()
